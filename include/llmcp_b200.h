@@ -215,6 +215,66 @@ int llmcp_dev_gated_delta_net_noalloc(const uint16_t *conv, const uint16_t *a, c
                                       int64_t nk, int64_t nv, int64_t dk, int64_t dv, int b_activated,
                                       uint16_t *out, void *stream);
 
+/* No counterpart in the reference, whose cache is one contiguous row range per sequence
+ * (lib/Runtime/AotRuntime.cpp:41-43).  A key/value cache in pages that any number of sequences share, on device
+ * pointers, enqueued on `stream` (a cudaStream_t) of the current device, not synchronised; nothing is allocated.
+ *
+ * llmcp_b200_paged_kv, one layer's cache.  pages: [num_pages][2: keys, values][kv_heads][page_size][head_dim], bf16
+ * where scales is null; else 4 bits: a byte holds two dimensions (even one in the low half) as code + 8, code -7 .. 7,
+ * and scales [num_pages][2][kv_heads][page_size][head_dim / 32] f16 multiply them.  head_dim 64, 128 or 256, page_size
+ * 16 to 256 (a power of two); both arrays 16-byte aligned.
+ * llmcp_b200_paged_batch, which rows a call is about.  Sequence b owns rows q_start[b] .. q_start[b + 1] - 1 of q, k, v
+ * and out (q_start ascending, from 0); they are the last tokens of the kv_len[b] it has, these included, so row i of n
+ * has position kv_len - n + i.  Its token j lies in page page_table[b * table_stride + j / page_size] (table_width
+ * entries a row).  The three arrays are int32 device memory and may change between replays of a captured call;
+ * tokens (rows of q, k, v and out), max_q and max_kv bound them on the host: no sequence may have more rows or a greater kv_len.  Rows from
+ * q_start[sequences] on are left as they are (padding).
+ *
+ *   llmcp_dev_paged_append   : the first half of llmcp.attention (LowerAttention.cpp:54-265) for a batch: q [tokens]
+ *                              [heads][head_dim] and k, v [tokens][kv_heads][head_dim], bf16 with row and head strides
+ *                              in elements.  q and k rows are normalised where q_norm / k_norm ([head_dim] bf16, may be
+ *                              null) are given, x / sqrt(mean(x^2) + eps) * (1 + w), and their first rot dimensions rotated by
+ *                              rows `position` of cos and sin ([cos_rows][rot] f32, as llmcp_b200_make_cos_sin writes them),
+ *                              in f64, rounded once.  q goes to q_out [tokens][heads][head_dim]; k and v to their
+ *                              pages, in 4 bits as d = f16(min(max |y| / 7, 65504)), code = round-to-even(y / d) held to
+ *                              -7 .. 7 per 32 dimensions.  heads may be 0 (keys and values only).  rot: a multiple of head_dim / 16.
+ *                              No two rows of a call may have the same place in the cache.
+ *   llmcp_dev_paged_read     : the cached keys and values of the batch's rows as f32 or bf16 (out_dtype 0 or 1),
+ *                              k_out and v_out [tokens][kv_heads][head_dim].  max_q = max_kv reads whole sequences.
+ *   llmcp_dev_paged_attention: the second half (LowerAttention.cpp:266-601): out [tokens][heads][head_dim] bf16 =
+ *                              softmax(score) v * sigmoid(gate).  score = q k scale; softcap > 0: softcap *
+ *                              tanh(score / softcap); slopes ([heads] f32, may be null): minus slope * |p - j| for the
+ *                              key j of a row at position p.  Keys j <= p are seen, and j < prefix[b] where prefix ([sequences] int32) is
+ *                              given, none from kv_len on; a row that sees none gets zeros.  gate (may be null): bf16 with
+ *                              strides.  heads: a multiple of kv_heads.  Products on the tensor cores, sums and softmax in
+ *                              f32.  What the pages hold from kv_len on has no influence, whatever it is; the keys and
+ *                              values before it have to be finite.  workspace: device memory of
+ *                              llmcp_dev_paged_attention_workspace bytes (-1 on error; depends on the host's figures only) that no other call uses
+ *                              meanwhile, captured graphs that may run at the same time included; needs no clearing.
+ * status (device int, may be null; not cleared): bit 1 is raised if a bounded wait inside a kernel ran out (out is then
+ * incomplete), bit 4 if lengths or page indices do not fit the figures above: sequences whose lengths do not fit are left out (their
+ * rows of out unwritten), a token whose page does not exist is not stored, and counts as zeros in attention. */
+typedef struct llmcp_b200_paged_kv {
+  void *pages;
+  uint16_t *scales;
+  int64_t num_pages, page_size, kv_heads, head_dim;
+} llmcp_b200_paged_kv;
+typedef struct llmcp_b200_paged_batch {
+  const int32_t *q_start, *kv_len, *page_table;
+  int64_t sequences, table_width, table_stride, tokens, max_q, max_kv;
+} llmcp_b200_paged_batch;
+int llmcp_dev_paged_append(const llmcp_b200_paged_kv *kv, const llmcp_b200_paged_batch *batch, const uint16_t *q, int64_t q_row,
+                           int64_t q_head, int64_t heads, const uint16_t *k, int64_t k_row, int64_t k_head, const uint16_t *v,
+                           int64_t v_row, int64_t v_head, const uint16_t *q_norm, const uint16_t *k_norm, float eps, const float *cos,
+                           const float *sin, int64_t cos_rows, int64_t rot, uint16_t *q_out, int *status, void *stream);
+int llmcp_dev_paged_read(const llmcp_b200_paged_kv *kv, const llmcp_b200_paged_batch *batch, void *k_out, void *v_out, int out_dtype,
+                         int *status, void *stream);
+int64_t llmcp_dev_paged_attention_workspace(const llmcp_b200_paged_kv *kv, const llmcp_b200_paged_batch *batch, int64_t heads);
+int llmcp_dev_paged_attention(const llmcp_b200_paged_kv *kv, const llmcp_b200_paged_batch *batch, const uint16_t *q, int64_t q_row,
+                              int64_t q_head, int64_t heads, float scale, float softcap, const float *slopes, const int32_t *prefix,
+                              const uint16_t *gate, int64_t gate_row, int64_t gate_head, uint16_t *out, void *workspace,
+                              int64_t workspace_bytes, int *status, void *stream);
+
 /* ---- 3. engine --------------------------------------------------------------------- */
 
 typedef struct llmcp_b200_dims {

@@ -79,6 +79,7 @@ size_t elem(int dtype) { return dtype == kBF16 ? 2 : 4; }
 
 namespace llmcp_b200 {
 void report_error(const std::string &message) { set_error(message); }
+void count_launches(uint64_t launches) { g_launches += launches; }
 } // namespace llmcp_b200
 
 namespace {
