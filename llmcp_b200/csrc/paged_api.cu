@@ -43,10 +43,10 @@ PagedKv to_kv(const llmcp_b200_paged_kv *kv) {
 
 PagedBatch to_batch(const llmcp_b200_paged_batch *b) {
   require(b != nullptr, "no batch");
-  constexpr int64_t most = (int64_t(1) << 31) - 1024; // tile arithmetic on positions stays in 31 bits
+  constexpr int64_t most = int64_t(1) << 30; // arithmetic on positions and tiles stays in 31 bits
   require(b->sequences >= 0 && b->sequences <= 65535, "sequences has to be 0 to 65535");
   require(b->tokens >= 0 && b->tokens <= most && b->max_q >= 0 && b->max_q <= most && b->max_kv >= 0 && b->max_kv <= most,
-          "tokens, max_q and max_kv have to be 0 to 2^31 - 1024");
+          "tokens, max_q and max_kv have to be 0 to 2^30");
   require(b->table_width >= 0 && b->table_width <= most && (b->table_stride >= b->table_width || b->sequences <= 1),
           "a row of the page table has table_width entries, rows lie table_stride apart");
   require(b->sequences == 0 || b->tokens == 0 || (b->q_start && b->kv_len && (b->page_table || b->table_width == 0)),
@@ -181,7 +181,7 @@ extern "C" int llmcp_dev_paged_attention(const llmcp_b200_paged_kv *kv, const ll
     a.gate = gate, a.gate_row = gate_row, a.gate_head = gate_head;
     a.out = out, a.workspace = workspace;
     int launches = 0;
-    check(launch_paged_attention(c, b, a, status, static_cast<cudaStream_t>(stream), &launches), "paged attention");
+    check(launch_paged_attention(c, b, a, status, sms, static_cast<cudaStream_t>(stream), &launches), "paged attention");
     count_launches(static_cast<uint64_t>(launches));
   });
 }

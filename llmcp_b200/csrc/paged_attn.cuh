@@ -1,0 +1,107 @@
+// What the attention kernels over the paged cache share: how a sequence's keys are split, the score's functions, the
+// rows of out and of the workspace, the tensor maps.
+#pragma once
+
+#include "paged.h"
+#include "tc_common.cuh"
+
+namespace llmcp_b200 {
+
+// Sequences are cut into `chunks` pieces of `chunk` keys (the last ones of a short sequence empty); 1: nothing to join.
+struct PagedSplit {
+  int chunk, chunks;
+};
+constexpr int kMaxChunks = 512;
+
+PagedSplit paged_rows_split(const PagedKv &kv, const PagedBatch &batch, int sms);
+int paged_rows_tile(const PagedKv &kv); // keys that a CTA of the few-rows kernel takes at a time
+cudaError_t launch_paged_rows(const PagedKv &kv, const PagedBatch &batch, const PagedAttention &call, const PagedSplit &split, int *status,
+                              cudaStream_t stream);
+
+// Joins the chunks of every row.  Workspace of a call: [row][chunk][head_dim] f32 sums, then [row][chunk] (maximum in
+// units of log 2, sum of weights), row = token * heads + head.
+cudaError_t launch_paged_merge(const PagedKv &kv, const PagedBatch &batch, const PagedAttention &call, const PagedSplit &split, cudaStream_t stream);
+
+inline size_t paged_parts_bytes(const PagedKv &kv, const PagedBatch &batch, int heads, const PagedSplit &split) {
+  return split.chunks == 1 ? 0 : static_cast<size_t>(batch.tokens) * heads * split.chunks * (kv.head_dim + 2) * sizeof(float);
+}
+
+// Rows of values (or codes) in boxes of box_rows rows x 64 bf16 dimensions, or a whole row of codes, swizzled.
+inline bool paged_value_map(CUtensorMap *map, const PagedKv &kv, int64_t rows, int box_rows) {
+  tc::EncodeTiled encode = tc::encode_tiled();
+  if (!encode)
+    return false;
+  const bool q4 = kv.scales != nullptr;
+  const cuuint64_t cols = q4 ? kv.head_dim / 2 : kv.head_dim;
+  const cuuint64_t dims[2] = {cols, static_cast<cuuint64_t>(rows)}, strides[1] = {q4 ? cols : 2 * cols};
+  const cuuint32_t box[2] = {q4 ? static_cast<cuuint32_t>(cols) : 64u, static_cast<cuuint32_t>(box_rows)}, elem[2] = {1, 1};
+  const int span = q4 ? kv.head_dim / 2 : 128;
+  return encode(map, q4 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, kv.pages, dims, strides, box, elem,
+                CU_TENSOR_MAP_INTERLEAVE_NONE,
+                span == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : span == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// The scales of 16 rows (head_dim bytes) as one row of the map.
+inline bool paged_scale_map(CUtensorMap *map, const PagedKv &kv, int64_t rows, int box_rows) {
+  tc::EncodeTiled encode = tc::encode_tiled();
+  if (!encode)
+    return false;
+  const cuuint64_t cols = kv.head_dim / 2, dims[2] = {cols, static_cast<cuuint64_t>(rows / 16)}, strides[1] = {2 * cols};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(cols), static_cast<cuuint32_t>(box_rows / 16)}, elem[2] = {1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, kv.scales, dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+#ifdef __CUDACC__
+// 2^x by the hardware's instruction (relative error about 2^-22; 0 for -infinity).
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// cap tanh(x / cap) in units of log 2.  tanh(y) = 1 - 2 / (1 + e^2y) loses its relative precision next to 0, but what
+// counts is the score's absolute error, cap * 2^-22 or so.
+__device__ __forceinline__ float capped_log2(float x, float cap, float over_cap) {
+  constexpr float kLog2e = 1.4426950408889634f;
+  const float e = exp2_approx(x * over_cap * (2.0f * kLog2e));
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return cap * kLog2e * __fmaf_rn(-2.0f, r, 1.0f);
+}
+
+// Four dimensions of a finished row: the sum over its weights' total (0 where there are none), the gate, bf16.
+template <int D>
+__device__ __forceinline__ void paged_store_out(const PagedAttention &call, int token, int head, int d, float4 acc, float total) {
+  const float inv = total == 0.0f ? 0.0f : __fdiv_rn(1.0f, total);
+  float v[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+  if (call.gate) {
+    const uint2 raw = *reinterpret_cast<const uint2 *>(call.gate + token * call.gate_row + head * call.gate_head + d);
+    const float gate[4] = {__uint_as_float(raw.x << 16), __uint_as_float(raw.x & 0xffff0000u), __uint_as_float(raw.y << 16),
+                           __uint_as_float(raw.y & 0xffff0000u)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v[i] = __fdividef(v[i], 1.0f + __expf(-fmaxf(gate[i], -80.0f))); // below -80 the gate is 0 to every bit of a bf16 sum
+  }
+  uint2 words;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(words.x) : "f"(v[1]), "f"(v[0]));
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(words.y) : "f"(v[3]), "f"(v[2]));
+  *reinterpret_cast<uint2 *>(call.out + (static_cast<int64_t>(token) * call.heads + head) * D + d) = words;
+}
+
+__device__ __forceinline__ float2 *paged_part_sums(const PagedAttention &call, int tokens, int chunks, int head_dim) {
+  return reinterpret_cast<float2 *>(static_cast<float *>(call.workspace) + static_cast<int64_t>(tokens) * call.heads * chunks * head_dim);
+}
+
+template <int D>
+__device__ __forceinline__ void paged_store_part(const PagedAttention &call, int tokens, int chunks, int chunk, int token, int head, int d, float4 acc,
+                                                 float top, float total) {
+  const int64_t row = (static_cast<int64_t>(token) * call.heads + head) * chunks + chunk;
+  *reinterpret_cast<float4 *>(static_cast<float *>(call.workspace) + row * D + d) = acc;
+  if (d == 0)
+    paged_part_sums(call, tokens, chunks, D)[row] = make_float2(top, total);
+}
+#endif
+
+} // namespace llmcp_b200

@@ -1,0 +1,650 @@
+// Attention over the paged cache for few rows: the tokens of one sequence times the query heads that share a key head are
+// at most 16 rows (one to a few new tokens of every sequence).
+//
+//   score s_rj = scale q_r . k_j (capped, biased, masked);  p = 2^(s log2 e - m);  o_r = sum_j p_rj v_j / sum_j p_rj
+//
+// Bound by HBM: every key and value is read once (4 bytes per dimension of a bf16 pair, 1.125 in 4 bits), and even one
+// multiply-add per row and element on the CUDA cores would take longer than the read.  So both products run on mma.sync
+// (m16n8k16) with the keys and the value dimensions as the 16-row side and the rows as the 8-column side (padded), one
+// or two such columns: the instruction, not tcgen05, because a tile has 8 or 16 rows and its operands come straight from
+// registers.  A tile's scores transposed, P^T, become the second product's operand by movmatrix.
+//
+// One CTA takes `chunk` keys of one (sequence, key head); its four warps take tiles of them in turn, each with a ring of
+// its own that a lane or four of the warp feed by TMA (the hardware swizzle makes the ldmatrix reads free of conflicts),
+// and running maximum, sum and output of its own; no barrier joins the warps before the end.  Several chunks of a
+// sequence are joined by paged_merge_kernel.
+//
+// bf16 pages: weights are split into two bf16 values (high and rest) that both multiply V, so that their rounding (2^-17)
+// does not show.
+// 4-bit pages: codes + 8, 0 to 15, are used as f16 bit patterns in place: the four bits of an even nibble are the
+// subnormal value code * 2^-24, those of an odd one 16 times that, so one mask makes two operands and the factors go
+// into q (exactly: powers of two) or into the end.  For the keys the 8 is taken off through the accumulator (a block's score
+// starts at -8 sum q); for the values before the product, since a dimension in which a row's heavy key is 0 would
+// otherwise be the difference of two large sums.  q is scaled by a power of two per row so that its largest element lies
+// in [2^14, 2^15): f16 holds every bf16 value that matters beside it.  A block's score is multiplied by its key scale in
+// f32; the value scale goes into the weight, p' = f16(p d 2^k), k such that the largest d so far keeps p' just below
+// 2^15 (it moves as the running maximum does): relative rounding 2^-11 for weights down to 2^-29 of the largest.
+
+#include "common.cuh"
+#include "paged.h"
+#include "paged_attn.cuh"
+#include "tc_common.cuh"
+
+namespace llmcp_b200 {
+
+namespace {
+
+using namespace tc;
+
+constexpr int kWarps = 4;
+
+template <int D, bool Q4> struct Shape {
+  static constexpr int keys = Q4 ? (D == 256 ? 32 : 64) : 4096 / D; // keys per tile of a warp: 8 KB of bf16, 4 or 2 of codes
+  static constexpr int row_bytes = Q4 ? D / 2 : 128;                // shared-memory row: the swizzle's span
+  static constexpr int slabs = Q4 ? 1 : D / 64;                     // a bf16 row lies in slabs of 64 dimensions
+  static constexpr int value_bytes = keys * row_bytes * slabs;
+  static constexpr int scale_bytes = Q4 ? keys * D / 16 : 0;
+  static constexpr int slot_bytes = (value_bytes + (D == 64 ? 2 : 1) * scale_bytes + 1023) / 1024 * 1024;
+  static constexpr int slots = 3;
+  static constexpr int blocks = D / 32;
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t address) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(address) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t address) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(address) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+template <bool F16> __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t a0, const uint32_t a1, const uint32_t a2, const uint32_t a3, const uint32_t b0, const uint32_t b1) {
+  if constexpr (F16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float f16_at(uint32_t word, int high) { return f16_bits_to_f32(static_cast<uint16_t>(high ? word >> 16 : word)); }
+
+__device__ __forceinline__ uint32_t sub_f16(uint32_t x, uint32_t y) {
+  uint32_t z;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(z) : "r"(x), "r"(y));
+  return z;
+}
+
+struct Rows {
+  PagedKv kv;
+  PagedBatch batch;
+  PagedAttention call;
+  int chunk, chunks, box_rows;
+  int out_of_range; // a row coordinate past the last row of the cache: reads as zeros
+  uint32_t spin_limit;
+};
+
+template <int D, bool Q4, int NT>
+__global__ void __launch_bounds__(32 * kWarps, NT == 1 && Q4 ? 3 : 2)
+paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_constant__ CUtensorMap map_scales,
+                  const __grid_constant__ Rows p, int *__restrict__ status) {
+  using S = Shape<D, Q4>;
+  constexpr int KT = S::keys, M = KT / 16, NB = S::blocks, MT = D / 16;
+  constexpr bool kQueriesShared = NT * D > 256; // the queries' fragments in shared memory: no registers left for them
+  extern __shared__ uint8_t raw_smem[];
+  __shared__ uint64_t full[kWarps][S::slots];
+  __shared__ float2 queries_sum[Q4 ? NT : 1][NB][4]; // -8 sum q of a block, two rows
+  __shared__ float warp_max[kWarps][NT * 8], warp_sum[kWarps][NT * 8];
+  __shared__ int failed;
+  uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int chunk_index = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+  if (lane == 0)
+    for (int i = 0; i < S::slots; ++i)
+      mbar_init(&full[warp][i], 1);
+  if (tid == 0)
+    failed = 0;
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  __syncthreads();
+  grid_dependency_sync();
+  const PagedSequence seq = paged_sequence(p.batch, p.kv.page_shift, b, tid == 0 && chunk_index == 0 && kvh == 0 ? status : nullptr);
+  const int group = p.call.heads / p.kv.kv_heads, rows = seq.count * group;
+  const int key0 = chunk_index * p.chunk, key1 = min(seq.length, key0 + p.chunk);
+  if (rows == 0 || (key0 >= key1 && chunk_index > 0))
+    return;
+  const int tiles_all = max(0, key1 - key0 + KT - 1) / KT, tiles = tiles_all > warp ? (tiles_all - warp + kWarps - 1) / kWarps : 0;
+
+  // ---- the ring: item 2 i + which is tile i's keys or values; lanes below `boxes` issue a box each ----------------------
+  const int sub_boxes = KT / p.box_rows, boxes = S::slabs * sub_boxes;
+  const int slab = lane / sub_boxes, sub = lane % sub_boxes; // of this lane's box
+  uint8_t *ring = base + warp * (S::slots * S::slot_bytes);
+  const int32_t *table = p.batch.page_table + b * p.batch.table_stride;
+  const int head_rows = p.kv.kv_heads << p.kv.page_shift;
+  // scales of 16 rows; a box of them starts on a 128-byte boundary
+  const int scale_pitch = D == 64 && p.box_rows == 16 ? 128 : D;
+  auto first_key = [&](int i) { return key0 + (warp + i * kWarps) * KT; };
+  auto page_of = [&](int i) { // of this lane's rows in tile i; -1: past the sequence
+    const int key = first_key(i) + sub * p.box_rows;
+    return i < tiles && lane < boxes && key < seq.length ? table[key >> p.kv.page_shift] : -1;
+  };
+  int page_now = page_of(0), page_next = page_of(1), issued = 0;
+  auto issue = [&]() {
+    const int i = issued >> 1, which = issued & 1, s = issued % S::slots;
+    if (i < tiles) {
+      if (lane == 0)
+        mbar_expect_tx(&full[warp][s], S::value_bytes + S::scale_bytes);
+      __syncwarp();
+      if (lane < boxes) {
+        const int key = first_key(i) + sub * p.box_rows;
+        int row = p.out_of_range;
+        if (key < seq.length) {
+          if (page_now >= 0 && page_now < p.kv.num_pages)
+            row = (page_now * 2 + which) * head_rows + (kvh << p.kv.page_shift) + (key & ((1 << p.kv.page_shift) - 1));
+          else if (status)
+            atomicOr(status, kStatusBadBatch);
+        }
+        uint8_t *slot = ring + s * S::slot_bytes;
+        tma_load_2d(slot + (slab * KT + sub * p.box_rows) * S::row_bytes, &map_values, slab * 64, row, &full[warp][s]);
+        if (Q4)
+          tma_load_2d(slot + S::value_bytes + sub * (p.box_rows / 16) * scale_pitch, &map_scales, 0, row >> 4, &full[warp][s]);
+      }
+      if (which) {
+        page_now = page_next;
+        page_next = page_of(i + 2);
+      }
+      ++issued;
+    }
+  };
+  for (int i = 0; i < S::slots; ++i)
+    issue();
+
+  // ---- the queries: row 8 nt + g is token row / group, head kvh * group + row % group --------------------------------------
+  uint32_t queries[kQueriesShared ? 1 : NT][Q4 ? NB * 4 : MT * 2];
+  uint4 *queries_sm = reinterpret_cast<uint4 *>(base + kWarps * S::slots * S::slot_bytes);
+  float factor[NT][2]; // what makes a column's products scores (in units of log 2, or before the cap)
+  const float to_log2 = p.call.softcap > 0.0f ? 1.0f : 1.4426950408889634f;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int row = nt * 8 + g;
+    const uint16_t *q = p.call.q + (seq.first + row / group) * p.call.q_row + (kvh * group + row % group) * p.call.q_head;
+    uint32_t fragment[Q4 ? NB * 4 : MT * 2];
+    float unscale = 1.0f;
+    if constexpr (Q4) {
+      uint4 raw[NB];
+      uint32_t top = 0;
+#pragma unroll
+      for (int k = 0; k < NB; ++k) {
+        raw[k] = row < rows ? *reinterpret_cast<const uint4 *>(q + 32 * k + 8 * t) : make_uint4(0, 0, 0, 0);
+        const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          top = max(top, max(w[i] & 0x7fffu, w[i] >> 16 & 0x7fffu));
+      }
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int up = top == 0 ? 0 : min(126, 14 - (static_cast<int>(top >> 7) - 127)); // q * 2^up has its largest in [2^14, 2^15)
+      const float mult = __int_as_float((up + 127) << 23);
+      unscale = __int_as_float(min(254, 24 - up + 127) << 23);
+#pragma unroll
+      for (int k = 0; k < NB; ++k) {
+        const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+        float x[8], sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          x[i] = __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16) * mult;
+          sum += x[i];
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        if (warp == 0 && t == 0)
+          reinterpret_cast<float *>(&queries_sum[nt][k][g >> 1])[g & 1] = sum * (-8.0f / 16777216.0f);
+        fragment[4 * k] = pack_f16(x[0], x[4]);
+        fragment[4 * k + 1] = pack_f16(x[1] * 0.0625f, x[5] * 0.0625f);
+        fragment[4 * k + 2] = pack_f16(x[2], x[6]);
+        fragment[4 * k + 3] = pack_f16(x[3] * 0.0625f, x[7] * 0.0625f);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < MT; ++k)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          fragment[2 * k + i] = row < rows ? *reinterpret_cast<const uint32_t *>(q + 16 * k + 8 * i + 2 * t) : 0;
+    }
+    if constexpr (kQueriesShared) {
+      if (warp == 0) {
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k)
+          queries_sm[(nt * (D / 32) + k) * 32 + lane] = make_uint4(fragment[4 * k], fragment[4 * k + 1], fragment[4 * k + 2], fragment[4 * k + 3]);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < (Q4 ? NB * 4 : MT * 2); ++k)
+        queries[nt][k] = fragment[k];
+    }
+    // a score's column is the row of lane 4 * (2 t) or 4 * (2 t + 1)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      factor[nt][i] = p.call.scale * to_log2 * __shfl_sync(0xffffffffu, unscale, (2 * t + i) * 4);
+  }
+  if (Q4 || kQueriesShared)
+    __syncthreads();
+  // four words of the fragments of dimensions 32 k .. 32 k + 31
+  auto query_words = [&](int nt, int k, uint32_t (&w)[4]) {
+    if constexpr (kQueriesShared) {
+      const uint4 v = queries_sm[(nt * (D / 32) + k) * 32 + lane];
+      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[i] = queries[nt][4 * k + i];
+    }
+  };
+
+  // ---- what the rows of this thread's columns see ----------------------------------------------------------------------------
+  int sees[NT][2];        // keys below it
+  float slope[NT][2], at[NT][2];
+  int sees_least = seq.length;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = nt * 8 + 2 * t + i;
+      const int position = seq.length - seq.count + row / group;
+      sees[nt][i] = row < rows ? min(seq.length, max(position + 1, p.call.prefix ? p.call.prefix[b] : 0)) : seq.length;
+      sees_least = min(sees_least, sees[nt][i]);
+      slope[nt][i] = p.call.slopes && row < rows ? p.call.slopes[kvh * group + row % group] * 1.4426950408889634f : 0.0f;
+      at[nt][i] = static_cast<float>(position);
+    }
+  const float cap = p.call.softcap, over_cap = cap > 0.0f ? 1.0f / cap : 0.0f;
+  const bool biased = p.call.slopes != nullptr;
+
+  float top[NT][2], sum[NT][2], out[MT][NT][4];
+  float shift = Q4 ? -29.0f : 0.0f; // maxima are kept without it; weights are 2^(score - maximum - shift)
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    top[nt][0] = top[nt][1] = -INFINITY;
+    sum[nt][0] = sum[nt][1] = 0.0f;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        out[mt][nt][i] = 0.0f;
+  }
+
+  const uint32_t ring_address = smem_u32(ring);
+  // 16-byte piece `piece` of row `row` of a slot as the swizzle placed it
+  auto piece_address = [&](int row, int piece) {
+    if constexpr (S::row_bytes == 128)
+      return row * 128 + ((piece ^ (row & 7)) << 4);
+    else if constexpr (S::row_bytes == 64)
+      return row * 64 + ((piece ^ (row >> 1 & 3)) << 4);
+    else
+      return row * 32 + ((piece ^ (row >> 2 & 1)) << 4);
+  };
+  // two scales each of rows 16 m + g + 8 h of a slot
+  auto scale_words = [&](int s, int m, int h) {
+    return reinterpret_cast<const uint32_t *>(ring + s * S::slot_bytes + S::value_bytes + m * scale_pitch + (g + 8 * h) * (D / 16));
+  };
+  const int lm_row = lane & 7, lm_matrix = lane >> 3;
+  bool ok = true;
+  for (int i = 0; i < tiles; ++i) {
+    const int j0 = first_key(i);
+    // ---- scores -------------------------------------------------------------------------------------------------------------
+    int s = (2 * i) % S::slots;
+    ok = mbar_wait(&full[warp][s], ((2 * i) / S::slots) & 1, &failed, p.spin_limit);
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok)
+      break;
+    uint32_t slot = ring_address + s * S::slot_bytes;
+    float x[M][NT][4];
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          x[m][nt][c] = 0.0f;
+      if constexpr (Q4) {
+        uint32_t sw[2][NB / 2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int k = 0; k < NB / 2; ++k)
+            sw[h][k] = scale_words(s, m, h)[k];
+#pragma unroll
+        for (int k = 0; k < NB; k += 2) {
+          uint32_t w[4]; // block k: rows g, g + 8; block k + 1 the same
+          ldmatrix4(w, slot + piece_address(m * 16 + (lm_matrix & 1) * 8 + lm_row, k + (lm_matrix >> 1)));
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const uint32_t lo = w[2 * u], hi = w[2 * u + 1], lo8 = lo >> 8, hi8 = hi >> 8;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              uint32_t q[4];
+              query_words(nt, k + u, q);
+              const float2 start = queries_sum[nt][k + u][t];
+              float acc[4] = {start.x, start.y, start.x, start.y};
+              mma16816<true>(acc, lo & 0x000f000fu, hi & 0x000f000fu, lo & 0x00f000f0u, hi & 0x00f000f0u, q[0], q[1]);
+              mma16816<true>(acc, lo8 & 0x000f000fu, hi8 & 0x000f000fu, lo8 & 0x00f000f0u, hi8 & 0x00f000f0u, q[2], q[3]);
+              const float d0 = f16_at(sw[0][(k + u) / 2], u), d1 = f16_at(sw[1][(k + u) / 2], u);
+              x[m][nt][0] = __fmaf_rn(acc[0], d0, x[m][nt][0]);
+              x[m][nt][1] = __fmaf_rn(acc[1], d0, x[m][nt][1]);
+              x[m][nt][2] = __fmaf_rn(acc[2], d1, x[m][nt][2]);
+              x[m][nt][3] = __fmaf_rn(acc[3], d1, x[m][nt][3]);
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < MT; k += 2) {
+          uint32_t q[NT][4];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            query_words(nt, k / 2, q[nt]);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            uint32_t a[4];
+            const int piece = 2 * (k + u) + (lm_matrix >> 1);
+            ldmatrix4(a, slot + (piece >> 3) * (KT * 128) + piece_address(m * 16 + (lm_matrix & 1) * 8 + lm_row, piece & 7));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma16816<false>(x[m][nt], a[0], a[1], a[2], a[3], q[nt][2 * u], q[nt][2 * u + 1]);
+          }
+        }
+      }
+    }
+    __syncwarp();
+    issue();
+    // ---- weights ------------------------------------------------------------------------------------------------------------
+    s = (2 * i + 1) % S::slots;
+    ok = mbar_wait(&full[warp][s], ((2 * i + 1) / S::slots) & 1, &failed, p.spin_limit);
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok)
+      break;
+    slot = ring_address + s * S::slot_bytes;
+    const bool tail = j0 + KT > seq.length; // rows of the tile past the sequence: whatever they hold
+    const float shift_before = shift;
+    if constexpr (Q4) { // the largest value scale so far, as a power of two above it: weights times scales stay below 2^15
+      uint32_t largest = 0;
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int k = 0; k < NB / 2; ++k)
+            if (!tail || j0 + m * 16 + g + h * 8 < seq.length)
+              largest = __vmaxu2(largest, scale_words(s, m, h)[k]);
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1)
+        largest = __vmaxu2(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+      shift = fmaxf(shift, static_cast<float>(static_cast<int>(max(largest & 0xffffu, largest >> 16) >> 10) - 29));
+    }
+    const bool masked = j0 + KT > sees_least; // some row of this thread does not see some key of the tile
+    float moved[NT][2];
+    bool any_moved = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float best[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int j = j0 + m * 16 + g + (c >> 1) * 8, col = c & 1;
+          float v = x[m][nt][c] * factor[nt][col];
+          if (cap > 0.0f)
+            v = capped_log2(v, cap, over_cap);
+          if (biased)
+            v -= slope[nt][col] * fabsf(at[nt][col] - static_cast<float>(j));
+          if (masked && j >= sees[nt][col])
+            v = -INFINITY;
+          x[m][nt][c] = v;
+          best[col] = fmaxf(best[col], v);
+        }
+#pragma unroll
+      for (int col = 0; col < 2; ++col) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1)
+          best[col] = fmaxf(best[col], __shfl_xor_sync(0xffffffffu, best[col], o));
+        const float higher = fmaxf(top[nt][col], best[col]);
+        any_moved |= higher + shift != top[nt][col] + shift_before;
+        moved[nt][col] = higher == -INFINITY ? 1.0f : exp2_approx((top[nt][col] + shift_before) - (higher + shift));
+        top[nt][col] = higher;
+      }
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) // a row that has seen nothing: 2^(-inf - 0)
+          x[m][nt][c] = exp2_approx(x[m][nt][c] - (top[nt][c & 1] == -INFINITY ? 0.0f : top[nt][c & 1] + shift));
+    }
+    if (__any_sync(0xffffffffu, any_moved)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        sum[nt][0] *= moved[nt][0];
+        sum[nt][1] *= moved[nt][1];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            out[mt][nt][c] *= moved[nt][c & 1];
+      }
+    }
+    if constexpr (!Q4) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            sum[nt][c & 1] += x[m][nt][c];
+    }
+    // ---- values -------------------------------------------------------------------------------------------------------------
+    if (!Q4 && tail) {
+      for (int u = lane; u < KT * 8 * S::slabs; u += 32) {
+        const int row = u / 8 % KT;
+        if (j0 + row >= seq.length)
+          *reinterpret_cast<uint4 *>(ring + s * S::slot_bytes + u * 16) = make_uint4(0, 0, 0, 0);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+    }
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      if constexpr (Q4) {
+        uint32_t sw[2][NB / 2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int k = 0; k < NB / 2; ++k) {
+            sw[h][k] = scale_words(s, m, h)[k];
+            if (tail && j0 + m * 16 + g + h * 8 >= seq.length)
+              sw[h][k] = 0;
+          }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            sum[nt][c & 1] += x[m][nt][c];
+#pragma unroll
+        for (int k = 0; k < NB; k += 2) {
+          uint32_t w[4]; // block k: keys 0-7, 8-15; block k + 1 the same
+          ldmatrix4_trans(w, slot + piece_address(m * 16 + (lm_matrix & 1) * 8 + lm_row, k + (lm_matrix >> 1)));
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const uint32_t lo = w[2 * u], hi = w[2 * u + 1], lo8 = lo >> 8, hi8 = hi >> 8;
+            const float d0 = f16_at(sw[0][(k + u) / 2], u), d1 = f16_at(sw[1][(k + u) / 2], u);
+            uint32_t a[8] = {lo & 0x000f000fu, lo & 0x00f000f0u, hi & 0x000f000fu, hi & 0x00f000f0u,
+                             lo8 & 0x000f000fu, lo8 & 0x00f000f0u, hi8 & 0x000f000fu, hi8 & 0x00f000f0u};
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+              a[n] = sub_f16(a[n], n & 1 ? 0x00800080u : 0x00080008u);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const uint32_t b0 = transpose8x8(pack_f16(x[m][nt][0] * d0, x[m][nt][1] * d0));
+              const uint32_t b1 = transpose8x8(pack_f16(x[m][nt][2] * d1, x[m][nt][3] * d1));
+              mma16816<true>(out[2 * (k + u)][nt], a[0], a[1], a[2], a[3], b0, b1);
+              mma16816<true>(out[2 * (k + u) + 1][nt], a[4], a[5], a[6], a[7], b0, b1);
+            }
+          }
+        }
+      } else {
+        uint32_t high[NT][2], rest[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float p0 = x[m][nt][2 * h], p1 = x[m][nt][2 * h + 1];
+            const uint32_t w = f32x2_to_bf16x2_hw(p0, p1);
+            high[nt][h] = transpose8x8(w);
+            rest[nt][h] = transpose8x8(f32x2_to_bf16x2_hw(p0 - __uint_as_float(w << 16), p1 - __uint_as_float(w & 0xffff0000u)));
+          }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          uint32_t a[4];
+          const int piece = 2 * mt + (lm_matrix & 1);
+          ldmatrix4_trans(a, slot + (piece >> 3) * (KT * 128) + piece_address(m * 16 + (lm_matrix >> 1) * 8 + lm_row, piece & 7));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma16816<false>(out[mt][nt], a[0], a[1], a[2], a[3], high[nt][0], high[nt][1]);
+            mma16816<false>(out[mt][nt], a[0], a[1], a[2], a[3], rest[nt][0], rest[nt][1]);
+          }
+        }
+      }
+    }
+    __syncwarp();
+    issue();
+  }
+  if (!ok) // copies already requested still write into this CTA's shared memory
+    for (int n = max(0, issued - S::slots); n < issued; ++n)
+      mbar_wait_quiet(&full[warp][n % S::slots], (n / S::slots) & 1, p.spin_limit);
+
+  // ---- the warps' parts joined --------------------------------------------------------------------------------------------------
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (Q4)
+        top[nt][i] += shift; // of the weights as they were summed
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1)
+        sum[nt][i] += __shfl_xor_sync(0xffffffffu, sum[nt][i], o);
+      if (g == 0) {
+        warp_max[warp][nt * 8 + 2 * t + i] = top[nt][i];
+        warp_sum[warp][nt * 8 + 2 * t + i] = sum[nt][i];
+      }
+    }
+  __syncthreads();
+  if (failed) {
+    if (tid == 0 && status)
+      atomicOr(status, kStatusWaitRanOut);
+    return;
+  }
+  float joined[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float all = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w)
+        all = fmaxf(all, warp_max[w][nt * 8 + 2 * t + i]);
+      joined[nt][i] = top[nt][i] == -INFINITY ? 0.0f : exp2_approx(top[nt][i] - all);
+    }
+  // row-major [warp][row][D + 4], over the rings (all copies have landed); the pad keeps the writes off each other's banks
+  constexpr int kPitch = D + 4;
+  float *parts = reinterpret_cast<float *>(base);
+  float *mine = parts + warp * (NT * 8 * kPitch);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float v = out[mt][nt][c];
+        int d;
+        if constexpr (Q4) {
+          // dims 32 k + 4 g + 2 j + (c >> 1) of m-tile 2 k + j; odd nibbles are 16 times their code
+          d = (mt / 2) * 32 + 4 * g + 2 * (mt & 1) + (c >> 1);
+          v *= c >> 1 ? 1048576.0f : 16777216.0f;
+        } else {
+          d = mt * 16 + g + (c >> 1) * 8;
+        }
+        mine[(nt * 8 + 2 * t + (c & 1)) * kPitch + d] = v * joined[nt][c & 1];
+      }
+  __syncthreads();
+  const int head0 = kvh * group;
+  for (int u = tid; u < rows * (D / 4); u += 32 * kWarps) {
+    const int row = u / (D / 4), d = u % (D / 4) * 4;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float all = -INFINITY, total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float4 v = *reinterpret_cast<const float4 *>(parts + (w * NT * 8 + row) * kPitch + d);
+      acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+      all = fmaxf(all, warp_max[w][row]);
+    }
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w)
+      total += warp_max[w][row] == -INFINITY ? 0.0f : warp_sum[w][row] * exp2_approx(warp_max[w][row] - all);
+    const int token = seq.first + row / group, head = head0 + row % group;
+    if (p.chunks == 1)
+      paged_store_out<D>(p.call, token, head, d, acc, total);
+    else
+      paged_store_part<D>(p.call, p.batch.tokens, p.chunks, chunk_index, token, head, d, acc, all, total);
+  }
+}
+
+template <int D, bool Q4, int NT>
+cudaError_t launch(const PagedKv &kv, const PagedBatch &batch, const PagedAttention &call, const PagedSplit &split, int *status, cudaStream_t stream) {
+  using S = Shape<D, Q4>;
+  Rows p;
+  p.kv = kv, p.batch = batch, p.call = call;
+  p.chunk = split.chunk, p.chunks = split.chunks;
+  p.box_rows = S::keys < (1 << kv.page_shift) ? S::keys : 1 << kv.page_shift;
+  const int64_t rows = kv.num_pages * 2 * kv.kv_heads << kv.page_shift;
+  p.out_of_range = static_cast<int>(rows);
+  p.spin_limit = kSpinLimit<true>;
+  CUtensorMap values, scales;
+  if (!paged_value_map(&values, kv, rows, p.box_rows) || (Q4 && !paged_scale_map(&scales, kv, rows, p.box_rows)))
+    return cudaErrorNotSupported;
+  if (!Q4)
+    scales = values;
+  constexpr size_t ring = kWarps * S::slots * S::slot_bytes + (NT * D > 256 ? NT * D * 16 : 0);
+  constexpr size_t parts = sizeof(float) * kWarps * NT * 8 * (D + 4);
+  constexpr size_t smem = 1024 + (ring > parts ? ring : parts);
+  const auto kernel = paged_rows_kernel<D, Q4, NT>;
+  if (cudaError_t e = opt_in_shared_memory(reinterpret_cast<const void *>(kernel), smem); e != cudaSuccess)
+    return e;
+  return launch_chained(kernel, dim3(split.chunks, kv.kv_heads, batch.sequences), dim3(32 * kWarps), smem, stream, values, scales, p, status);
+}
+
+template <int D, bool Q4>
+cudaError_t launch(const PagedKv &kv, const PagedBatch &batch, const PagedAttention &call, const PagedSplit &split, int *status, cudaStream_t stream) {
+  return static_cast<int64_t>(batch.max_q) * (call.heads / kv.kv_heads) <= 8 ? launch<D, Q4, 1>(kv, batch, call, split, status, stream)
+                                                                             : launch<D, Q4, 2>(kv, batch, call, split, status, stream);
+}
+
+} // namespace
+
+int paged_rows_tile(const PagedKv &kv) { return kWarps * (kv.scales ? (kv.head_dim == 256 ? 32 : 64) : 4096 / kv.head_dim); }
+
+cudaError_t launch_paged_rows(const PagedKv &kv, const PagedBatch &batch, const PagedAttention &call, const PagedSplit &split, int *status,
+                              cudaStream_t stream) {
+  switch (kv.head_dim) {
+  case 64:
+    return kv.scales ? launch<64, true>(kv, batch, call, split, status, stream) : launch<64, false>(kv, batch, call, split, status, stream);
+  case 128:
+    return kv.scales ? launch<128, true>(kv, batch, call, split, status, stream) : launch<128, false>(kv, batch, call, split, status, stream);
+  case 256:
+    return kv.scales ? launch<256, true>(kv, batch, call, split, status, stream) : launch<256, false>(kv, batch, call, split, status, stream);
+  default:
+    return cudaErrorInvalidValue;
+  }
+}
+
+} // namespace llmcp_b200

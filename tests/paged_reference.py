@@ -68,11 +68,12 @@ def sequence_rows(values, table, b, which, total):
 
 
 def attention(q, values, q_start, kv_len, table, scale, softcap=0.0, slopes=None, prefix=None, gate=None, rows=None):
-    """(out, weight, reach) in float64: out as defined, weight = sum p |v| * gate (what a relative error of the weights moves
-    out by at most), reach = the largest sum |q k scale| among the seen keys, per [row, head]."""
+    """(out, weight, (reach, span)) in float64: out as defined, weight = sum p |v| * gate (what a relative error of the weights
+    moves out by at most); per [row, head] reach = the largest sum |q k scale| among the seen keys, and span = their number
+    times the largest |v| among them (what an absolute error of the weights moves out by)."""
     tokens, heads, dim = q.shape
     out, weight = torch.zeros(tokens, heads, dim, dtype=torch.float64), torch.zeros(tokens, heads, dim, dtype=torch.float64)
-    reach = torch.zeros(tokens, heads, 1, dtype=torch.float64)
+    reach, span = torch.zeros(tokens, heads, 1, dtype=torch.float64), torch.zeros(tokens, heads, 1, dtype=torch.float64)
     for b in range(len(kv_len)):
         first, end, total = int(q_start[b]), int(q_start[b + 1]), int(kv_len[b])
         if end == first or total == 0:
@@ -95,17 +96,25 @@ def attention(q, values, q_start, kv_len, table, scale, softcap=0.0, slopes=None
             p = torch.nan_to_num(torch.softmax(x, -1), nan=0.0)
             out[first:end, h], weight[first:end, h] = p @ v[:, g], p @ v[:, g].abs()
             reach[first:end, h, 0] = (far * seen).amax(-1)
+            span[first:end, h, 0] = seen.sum(-1) * v[:, g].abs().max()
     if gate is not None:
         s = torch.sigmoid(gate.double())
         out, weight = out * s, weight * s
-    return out, weight, reach
+    return out, weight, (reach, span)
 
 
-def attention_bound(out, weight, reach, bits, softcap=0.0):
+def attention_bound(out, weight, extent, bits, softcap=0.0):
     """How far a kernel may be from attention()'s out.  Half a step of bf16 (2^-8) for the result.  Weights: rounded to bf16
     (2^-8) over bf16 pages, to f16 (2^-11) over 4-bit pages; there the values' and keys' f16 forms too (2^-11 each, the
     keys' as a change of the score, which moves a weight and the sum by its size: twice).  f32 sums: 2^-20 of what is
-    added up; exp, tanh and the score's scaling 2^-18 beside them, and 2^-20 of the cap."""
+    added up; exp, tanh and the score's scaling 2^-18 beside them, and 2^-20 of the cap.
+
+    Over 4-bit pages a weight has f16's range too: below 2^-14 its steps are 2^-24, so it is off by up to 2^-25 there.  With
+    the row's largest weight held at 2^7 or more (times the largest value scale, which goes into the weights or stays with
+    the values), that is 2^-32 of the largest weight for each key, and as much of the largest value for the result, which
+    the sum of the weights (at least the largest) divides.  It shows where a heavy key's value is 0 and only weights below
+    2^-21 of the largest are left."""
+    reach, span = extent
     relative = 2.0 ** -8 if bits == 16 else 2.0 ** -10
     score = reach * (2.0 ** -20 + (0 if bits == 16 else 2.0 ** -11)) + softcap * 2.0 ** -20
-    return 2.0 ** -8 * out.abs() + weight * (relative + 2 * score + 2.0 ** -17) * (1 + 2.0 ** -7) + 1e-30
+    return 2.0 ** -8 * out.abs() + weight * (relative + 2 * score + 2.0 ** -17) * (1 + 2.0 ** -7) + (0 if bits == 16 else span * 2.0 ** -32) + 1e-30

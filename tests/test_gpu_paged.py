@@ -434,10 +434,10 @@ def test_layer_equals_the_frameworks_attention(S, position):
     values = torch.zeros(count, 2, nkv, size, hd)
     at = torch.arange(total)
     values[table[0, at // size].long(), :, :, at % size] = after[:, :, :total].permute(2, 0, 1, 3).float()
-    _, weight, reach = R.attention(q.cpu(), values, q_start, kv_len, table, hd ** -0.5, gate=split[:, :, 1].cpu())
+    _, weight, (reach, span) = R.attention(q.cpu(), values, q_start, kv_len, table, hd ** -0.5, gate=split[:, :, 1].cpu())
     # beside the kernel's own bound: half a step of the other result, and scores that a step of a key or query (2^-7 in
     # 2^-7 * reach each, and hardly ever) may have moved
-    assert ((out - want).abs() <= R.attention_bound(out, weight, reach, 16) + 2.0 ** -8 * want.abs() + weight * reach * 2.0 ** -11).all()
+    assert ((out - want).abs() <= R.attention_bound(out, weight, (reach, span), 16) + 2.0 ** -8 * want.abs() + weight * reach * 2.0 ** -11).all()
 
 
 def test_other_devices_streams_and_types_are_refused():
