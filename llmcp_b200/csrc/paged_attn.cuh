@@ -13,9 +13,15 @@ struct PagedSplit {
 };
 constexpr int kMaxChunks = 512;
 
-PagedSplit paged_rows_split(const PagedKv &kv, const PagedBatch &batch, int sms);
-int paged_rows_tile(const PagedKv &kv); // keys that a CTA of the few-rows kernel takes at a time
+PagedSplit paged_rows_split(const PagedKv &kv, const PagedBatch &batch, int rows, int sms);
+int paged_rows_tile(const PagedKv &kv, int rows); // keys that a CTA of the few-rows kernel takes at a time
 cudaError_t launch_paged_rows(const PagedKv &kv, const PagedBatch &batch, const PagedAttention &call, const PagedSplit &split, int *status,
+                              cudaStream_t stream);
+
+// The kernel for many rows; its workspace holds the parts and, for a 4-bit cache, its rows of 16 bits.
+PagedSplit paged_tile_split(const PagedKv &kv, const PagedBatch &batch, int heads, int sms);
+size_t paged_tile_workspace(const PagedKv &kv, const PagedBatch &batch, int heads, const PagedSplit &split);
+cudaError_t launch_paged_tile(const PagedKv &kv, const PagedBatch &batch, const PagedAttention &call, const PagedSplit &split, int *status,
                               cudaStream_t stream);
 
 // Joins the chunks of every row.  Workspace of a call: [row][chunk][head_dim] f32 sums, then [row][chunk] (maximum in

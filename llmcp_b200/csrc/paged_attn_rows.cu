@@ -18,12 +18,12 @@
 // does not show.
 // 4-bit pages: codes + 8, 0 to 15, are used as f16 bit patterns in place: the four bits of an even nibble are the
 // subnormal value code * 2^-24, those of an odd one 16 times that, so one mask makes two operands and the factors go
-// into q (exactly: powers of two) or into the end.  For the keys the 8 is taken off through the accumulator (a block's score
-// starts at -8 sum q); for the values before the product, since a dimension in which a row's heavy key is 0 would
+// into q (exactly: powers of two) or into the end.  For the keys the 8 is taken off the sum, for the values before the product, since a dimension in which a row's heavy key is 0 would
 // otherwise be the difference of two large sums.  q is scaled by a power of two per row so that its largest element lies
 // in [2^14, 2^15): f16 holds every bf16 value that matters beside it.  A block's score is multiplied by its key scale in
-// f32; the value scale goes into the weight, p' = f16(p d 2^k), k such that the largest d so far keeps p' just below
-// 2^15 (it moves as the running maximum does): relative rounding 2^-11 for weights down to 2^-29 of the largest.
+// f32 (the part of the 8s is one more product, scales times -8 sum q in two f16 pieces); the value scale goes into the
+// weight, p' = f16(f16(p 2^k) d): k = 15, or less where the largest d so far would take p' past 2^15 (it moves as the
+// running maximum does), so that weights down to 2^-29 of the largest keep f16's relative rounding, 2^-11 twice.
 
 #include "common.cuh"
 #include "paged.h"
@@ -37,9 +37,12 @@ namespace {
 using namespace tc;
 
 constexpr int kWarps = 4;
+// A row's weights are 2^(score - reference): the reference is a score that none has outgrown by more than 2^8, so that sums
+// and outputs are hardly ever rescaled.
+constexpr float kHeadroom = 8.0f;
 
-template <int D, bool Q4> struct Shape {
-  static constexpr int keys = Q4 ? (D == 256 ? 32 : 64) : 4096 / D; // keys per tile of a warp: 8 KB of bf16, 4 or 2 of codes
+template <int D, bool Q4, int NT> struct Shape {
+  static constexpr int keys = Q4 ? (D == 256 || NT == 2 ? 32 : 64) : 4096 / D; // keys per tile of a warp: 8 KB of bf16, 1 to 4 of codes
   static constexpr int row_bytes = Q4 ? D / 2 : 128;                // shared-memory row: the swizzle's span
   static constexpr int slabs = Q4 ? 1 : D / 64;                     // a bf16 row lies in slabs of 64 dimensions
   static constexpr int value_bytes = keys * row_bytes * slabs;
@@ -57,28 +60,55 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addre
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 template <bool F16> __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t a0, const uint32_t a1, const uint32_t a2, const uint32_t a3, const uint32_t b0, const uint32_t b1) {
   if constexpr (F16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The first product of a sum: nothing to add to.
+__device__ __forceinline__ void mma16816_f16_first(float (&d)[4], const uint32_t a0, const uint32_t a1, const uint32_t a2, const uint32_t a3, const uint32_t b0, const uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ __forceinline__ uint32_t mul_f16(uint32_t x, uint32_t y) {
+  uint32_t z;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(z) : "r"(x), "r"(y));
+  return z;
 }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-__device__ __forceinline__ float f16_at(uint32_t word, int high) { return f16_bits_to_f32(static_cast<uint16_t>(high ? word >> 16 : word)); }
+__device__ __forceinline__ float2 f16_pair(uint32_t word) {
+  float2 v;
+  asm("{ .reg .b16 l, h; mov.b32 {l, h}, %2; cvt.f32.f16 %0, l; cvt.f32.f16 %1, h; }" : "=f"(v.x), "=f"(v.y) : "r"(word));
+  return v;
+}
 
 __device__ __forceinline__ uint32_t sub_f16(uint32_t x, uint32_t y) {
   uint32_t z;
   asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(z) : "r"(x), "r"(y));
   return z;
+}
+
+// N neighbouring words of shared memory.
+template <int N> __device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint32_t *p) {
+  if constexpr (N == 4) {
+    const uint4 v = *reinterpret_cast<const uint4 *>(p);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2 *>(p);
+    w[0] = v.x, w[1] = v.y;
+  } else {
+    w[0] = *p;
+  }
 }
 
 struct Rows {
@@ -91,16 +121,18 @@ struct Rows {
 };
 
 template <int D, bool Q4, int NT>
-__global__ void __launch_bounds__(32 * kWarps, NT == 1 && Q4 ? 3 : 2)
+__global__ void __launch_bounds__(32 * kWarps, Q4 ? (NT * D <= 256 ? 3 : 2) : 2)
 paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_constant__ CUtensorMap map_scales,
                   const __grid_constant__ Rows p, int *__restrict__ status) {
-  using S = Shape<D, Q4>;
+  using S = Shape<D, Q4, NT>;
   constexpr int KT = S::keys, M = KT / 16, NB = S::blocks, MT = D / 16;
-  constexpr bool kQueriesShared = NT * D > 256; // the queries' fragments in shared memory: no registers left for them
+  constexpr bool kQueriesShared = Q4 || NT * D > 256; // the queries' fragments in shared memory: registers are for warps
   extern __shared__ uint8_t raw_smem[];
   __shared__ uint64_t full[kWarps][S::slots];
-  __shared__ float2 queries_sum[Q4 ? NT : 1][NB][4]; // -8 sum q of a block, two rows
   __shared__ float warp_max[kWarps][NT * 8], warp_sum[kWarps][NT * 8];
+  __shared__ int sees[NT * 8];                       // keys below it
+  __shared__ float slope[NT * 8], at[NT * 8], unscales[NT * 8];
+  __shared__ uint2 offsets_sm[Q4 ? NT : 1][32];
   __shared__ int failed;
   uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -167,16 +199,17 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
   // ---- the queries: row 8 nt + g is token row / group, head kvh * group + row % group --------------------------------------
   uint32_t queries[kQueriesShared ? 1 : NT][Q4 ? NB * 4 : MT * 2];
   uint4 *queries_sm = reinterpret_cast<uint4 *>(base + kWarps * S::slots * S::slot_bytes);
-  float factor[NT][2]; // what makes a column's products scores (in units of log 2, or before the cap)
-  const float to_log2 = p.call.softcap > 0.0f ? 1.0f : 1.4426950408889634f;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
+    if (kQueriesShared && warp != nt)
+      continue;
     const int row = nt * 8 + g;
     const uint16_t *q = p.call.q + (seq.first + row / group) * p.call.q_row + (kvh * group + row % group) * p.call.q_head;
     uint32_t fragment[Q4 ? NB * 4 : MT * 2];
     float unscale = 1.0f;
     if constexpr (Q4) {
       uint4 raw[NB];
+      float sums[NB];
       uint32_t top = 0;
 #pragma unroll
       for (int k = 0; k < NB; ++k) {
@@ -202,12 +235,23 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
         }
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        if (warp == 0 && t == 0)
-          reinterpret_cast<float *>(&queries_sum[nt][k][g >> 1])[g & 1] = sum * (-8.0f / 16777216.0f);
+        sums[k] = sum * (-8.0f / 16777216.0f);
         fragment[4 * k] = pack_f16(x[0], x[4]);
         fragment[4 * k + 1] = pack_f16(x[1] * 0.0625f, x[5] * 0.0625f);
         fragment[4 * k + 2] = pack_f16(x[2], x[6]);
         fragment[4 * k + 3] = pack_f16(x[3] * 0.0625f, x[7] * 0.0625f);
+      }
+      // place kk of the 16 belongs to block kk % NB: its sum rounded, then what that leaves, then nothing
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float v[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int kk = 0; kk < 16; ++kk)
+          if (kk / 2 == t + 4 * h && kk < 2 * NB) {
+            const float high = f16_pair(pack_f16(sums[kk % NB], 0.0f)).x;
+            v[kk & 1] = kk < NB ? high : sums[kk % NB] - high;
+          }
+        reinterpret_cast<uint32_t *>(&offsets_sm[nt][lane])[h] = pack_f16(v[0], v[1]);
       }
     } else {
 #pragma unroll
@@ -217,23 +261,37 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
           fragment[2 * k + i] = row < rows ? *reinterpret_cast<const uint32_t *>(q + 16 * k + 8 * i + 2 * t) : 0;
     }
     if constexpr (kQueriesShared) {
-      if (warp == 0) {
 #pragma unroll
-        for (int k = 0; k < D / 32; ++k)
-          queries_sm[(nt * (D / 32) + k) * 32 + lane] = make_uint4(fragment[4 * k], fragment[4 * k + 1], fragment[4 * k + 2], fragment[4 * k + 3]);
-      }
+      for (int k = 0; k < D / 32; ++k)
+        queries_sm[(nt * (D / 32) + k) * 32 + lane] = make_uint4(fragment[4 * k], fragment[4 * k + 1], fragment[4 * k + 2], fragment[4 * k + 3]);
     } else {
 #pragma unroll
       for (int k = 0; k < (Q4 ? NB * 4 : MT * 2); ++k)
         queries[nt][k] = fragment[k];
     }
-    // a score's column is the row of lane 4 * (2 t) or 4 * (2 t + 1)
+    if (Q4 && t == 0)
+      unscales[row] = unscale;
+  }
+  // what each row sees, and its bias
+  if (tid < NT * 8) {
+    const int position = seq.length - seq.count + tid / group;
+    sees[tid] = tid < rows ? min(seq.length, max(position + 1, p.call.prefix ? p.call.prefix[b] : 0)) : seq.length;
+    slope[tid] = p.call.slopes && tid < rows ? p.call.slopes[kvh * group + tid % group] * 1.4426950408889634f : 0.0f;
+    at[tid] = static_cast<float>(position);
+  }
+  __syncthreads();
+  uint32_t offsets[NT][2]; // 4 bits: what a block's scale is multiplied by to take the 8 off its codes, as f16 and its rest
+  float factor[NT][2];     // what makes a column's products scores (in units of log 2, or before the cap)
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    if constexpr (Q4) {
+      offsets[nt][0] = offsets_sm[nt][lane].x;
+      offsets[nt][1] = offsets_sm[nt][lane].y;
+    }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      factor[nt][i] = p.call.scale * to_log2 * __shfl_sync(0xffffffffu, unscale, (2 * t + i) * 4);
+      factor[nt][i] = p.call.scale * (p.call.softcap > 0.0f ? 1.0f : 1.4426950408889634f) * (Q4 ? unscales[nt * 8 + 2 * t + i] : 1.0f);
   }
-  if (Q4 || kQueriesShared)
-    __syncthreads();
   // four words of the fragments of dimensions 32 k .. 32 k + 31
   auto query_words = [&](int nt, int k, uint32_t (&w)[4]) {
     if constexpr (kQueriesShared) {
@@ -246,26 +304,12 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
     }
   };
 
-  // ---- what the rows of this thread's columns see ----------------------------------------------------------------------------
-  int sees[NT][2];        // keys below it
-  float slope[NT][2], at[NT][2];
-  int sees_least = seq.length;
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int row = nt * 8 + 2 * t + i;
-      const int position = seq.length - seq.count + row / group;
-      sees[nt][i] = row < rows ? min(seq.length, max(position + 1, p.call.prefix ? p.call.prefix[b] : 0)) : seq.length;
-      sees_least = min(sees_least, sees[nt][i]);
-      slope[nt][i] = p.call.slopes && row < rows ? p.call.slopes[kvh * group + row % group] * 1.4426950408889634f : 0.0f;
-      at[nt][i] = static_cast<float>(position);
-    }
+  const int sees_least = min(seq.length, max(seq.length - seq.count + 1, p.call.prefix ? p.call.prefix[b] : 0)); // the first row
   const float cap = p.call.softcap, over_cap = cap > 0.0f ? 1.0f / cap : 0.0f;
   const bool biased = p.call.slopes != nullptr;
 
   float top[NT][2], sum[NT][2], out[MT][NT][4];
-  float shift = Q4 ? -29.0f : 0.0f; // maxima are kept without it; weights are 2^(score - maximum - shift)
+  float shift = Q4 ? kHeadroom - 15.0f : 0.0f; // references are kept without it; weights are 2^(score - maximum - shift)
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     top[nt][0] = top[nt][1] = -INFINITY;
@@ -278,8 +322,9 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
   }
 
   const uint32_t ring_address = smem_u32(ring);
-  // 16-byte piece `piece` of row `row` of a slot as the swizzle placed it
-  auto piece_address = [&](int row, int piece) {
+  // where a lane reads for ldmatrix: row `row` of 16, 16-byte piece `piece` as the swizzle placed it; another even piece is
+  // an exclusive or with it (rows and slots are aligned to the swizzle's span), another 16 rows an addition
+  auto piece_offset = [&](int row, int piece) {
     if constexpr (S::row_bytes == 128)
       return row * 128 + ((piece ^ (row & 7)) << 4);
     else if constexpr (S::row_bytes == 64)
@@ -287,11 +332,13 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
     else
       return row * 32 + ((piece ^ (row >> 2 & 1)) << 4);
   };
-  // two scales each of rows 16 m + g + 8 h of a slot
-  auto scale_words = [&](int s, int m, int h) {
-    return reinterpret_cast<const uint32_t *>(ring + s * S::slot_bytes + S::value_bytes + m * scale_pitch + (g + 8 * h) * (D / 16));
+  // a row's scales in a slot, two to a word
+  auto scale_words = [&](int s, int row) {
+    return reinterpret_cast<const uint32_t *>(ring + s * S::slot_bytes + S::value_bytes + (row >> 4) * scale_pitch + (row & 15) * (D / 16));
   };
   const int lm_row = lane & 7, lm_matrix = lane >> 3;
+  const int rows_first = piece_offset((lm_matrix & 1) * 8 + lm_row, lm_matrix >> 1);   // matrices: rows, then pieces
+  const int pieces_first = piece_offset((lm_matrix >> 1) * 8 + lm_row, lm_matrix & 1); // pieces, then rows
   bool ok = true;
   for (int i = 0; i < tiles; ++i) {
     const int j0 = first_key(i);
@@ -311,28 +358,31 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
         for (int c = 0; c < 4; ++c)
           x[m][nt][c] = 0.0f;
       if constexpr (Q4) {
+        const uint32_t pair0 = scale_words(s, m * 16 + g)[t % (NB / 2)], pair1 = scale_words(s, m * 16 + g + 8)[t % (NB / 2)];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          mma16816_f16_first(x[m][nt], pair0, pair1, pair0, pair1, offsets[nt][0], offsets[nt][1]);
         uint32_t sw[2][NB / 2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int k = 0; k < NB / 2; ++k)
-            sw[h][k] = scale_words(s, m, h)[k];
+        load_words(sw[0], scale_words(s, m * 16 + g));
+        load_words(sw[1], scale_words(s, m * 16 + g + 8));
 #pragma unroll
         for (int k = 0; k < NB; k += 2) {
           uint32_t w[4]; // block k: rows g, g + 8; block k + 1 the same
-          ldmatrix4(w, slot + piece_address(m * 16 + (lm_matrix & 1) * 8 + lm_row, k + (lm_matrix >> 1)));
+          ldmatrix4(w, (slot + rows_first ^ k << 4) + m * 16 * S::row_bytes);
+          const float2 scale0 = f16_pair(sw[0][k / 2]), scale1 = f16_pair(sw[1][k / 2]);
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const uint32_t lo = w[2 * u], hi = w[2 * u + 1], lo8 = lo >> 8, hi8 = hi >> 8;
+            const uint32_t a[8] = {lo & 0x000f000fu, hi & 0x000f000fu, lo & 0x00f000f0u, hi & 0x00f000f0u,
+                                   lo8 & 0x000f000fu, hi8 & 0x000f000fu, lo8 & 0x00f000f0u, hi8 & 0x00f000f0u};
+            const float d0 = u ? scale0.y : scale0.x, d1 = u ? scale1.y : scale1.x;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               uint32_t q[4];
               query_words(nt, k + u, q);
-              const float2 start = queries_sum[nt][k + u][t];
-              float acc[4] = {start.x, start.y, start.x, start.y};
-              mma16816<true>(acc, lo & 0x000f000fu, hi & 0x000f000fu, lo & 0x00f000f0u, hi & 0x00f000f0u, q[0], q[1]);
-              mma16816<true>(acc, lo8 & 0x000f000fu, hi8 & 0x000f000fu, lo8 & 0x00f000f0u, hi8 & 0x00f000f0u, q[2], q[3]);
-              const float d0 = f16_at(sw[0][(k + u) / 2], u), d1 = f16_at(sw[1][(k + u) / 2], u);
+              float acc[4];
+              mma16816_f16_first(acc, a[0], a[1], a[2], a[3], q[0], q[1]);
+              mma16816<true>(acc, a[4], a[5], a[6], a[7], q[2], q[3]);
               x[m][nt][0] = __fmaf_rn(acc[0], d0, x[m][nt][0]);
               x[m][nt][1] = __fmaf_rn(acc[1], d0, x[m][nt][1]);
               x[m][nt][2] = __fmaf_rn(acc[2], d1, x[m][nt][2]);
@@ -350,8 +400,8 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             uint32_t a[4];
-            const int piece = 2 * (k + u) + (lm_matrix >> 1);
-            ldmatrix4(a, slot + (piece >> 3) * (KT * 128) + piece_address(m * 16 + (lm_matrix & 1) * 8 + lm_row, piece & 7));
+            const int piece = 2 * (k + u);
+            ldmatrix4(a, (slot + rows_first ^ (piece & 7) << 4) + (piece >> 3) * (KT * 128) + m * 16 * S::row_bytes);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
               mma16816<false>(x[m][nt], a[0], a[1], a[2], a[3], q[nt][2 * u], q[nt][2 * u + 1]);
@@ -369,23 +419,35 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
       break;
     slot = ring_address + s * S::slot_bytes;
     const bool tail = j0 + KT > seq.length; // rows of the tile past the sequence: whatever they hold
+    if (tail) { // their weights are 0, and so are their values (bf16) or scales now
+      if constexpr (Q4) {
+        for (int row = lane; row < KT; row += 32)
+          if (j0 + row >= seq.length)
+            for (int k = 0; k < NB / 2; ++k)
+              const_cast<uint32_t *>(scale_words(s, row))[k] = 0;
+      } else {
+        for (int u = lane; u < KT * 8 * S::slabs; u += 32)
+          if (j0 + u / 8 % KT >= seq.length)
+            *reinterpret_cast<uint4 *>(ring + s * S::slot_bytes + u * 16) = make_uint4(0, 0, 0, 0);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // before the slot's next copy
+      __syncwarp();
+    }
     const float shift_before = shift;
-    if constexpr (Q4) { // the largest value scale so far, as a power of two above it: weights times scales stay below 2^15
+    if constexpr (Q4) {
+      // the largest value scale so far as a power of two above it: weights stay at 2^15 or below, and times a scale too
       uint32_t largest = 0;
 #pragma unroll
-      for (int m = 0; m < M; ++m)
+      for (int n = 0; n < KT / 32; ++n)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int k = 0; k < NB / 2; ++k)
+          largest = __vmaxu2(largest, scale_words(s, n * 32 + lane)[k]);
 #pragma unroll
-          for (int k = 0; k < NB / 2; ++k)
-            if (!tail || j0 + m * 16 + g + h * 8 < seq.length)
-              largest = __vmaxu2(largest, scale_words(s, m, h)[k]);
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1)
+      for (int o = 1; o < 32; o <<= 1)
         largest = __vmaxu2(largest, __shfl_xor_sync(0xffffffffu, largest, o));
-      shift = fmaxf(shift, static_cast<float>(static_cast<int>(max(largest & 0xffffu, largest >> 16) >> 10) - 29));
+      shift = fmaxf(shift, static_cast<float>(static_cast<int>(max(largest & 0xffffu, largest >> 16) >> 10) - 29) + kHeadroom);
     }
-    const bool masked = j0 + KT > sees_least; // some row of this thread does not see some key of the tile
+    const bool masked = j0 + KT > sees_least; // some row does not see some key of the tile
     float moved[NT][2];
     bool any_moved = false;
 #pragma unroll
@@ -394,24 +456,36 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
 #pragma unroll
       for (int m = 0; m < M; ++m)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int j = j0 + m * 16 + g + (c >> 1) * 8, col = c & 1;
-          float v = x[m][nt][c] * factor[nt][col];
-          if (cap > 0.0f)
-            v = capped_log2(v, cap, over_cap);
-          if (biased)
-            v -= slope[nt][col] * fabsf(at[nt][col] - static_cast<float>(j));
-          if (masked && j >= sees[nt][col])
-            v = -INFINITY;
-          x[m][nt][c] = v;
-          best[col] = fmaxf(best[col], v);
-        }
+        for (int c = 0; c < 4; ++c)
+          x[m][nt][c] *= factor[nt][c & 1];
+      if (cap > 0.0f) {
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            x[m][nt][c] = capped_log2(x[m][nt][c], cap, over_cap);
+      }
+      if (biased || masked) {
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int j = j0 + m * 16 + g + (c >> 1) * 8, row = nt * 8 + 2 * t + (c & 1);
+            x[m][nt][c] = j < sees[row] ? x[m][nt][c] - slope[row] * fabsf(at[row] - static_cast<float>(j)) : -INFINITY;
+          }
+      }
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          best[c & 1] = fmaxf(best[c & 1], x[m][nt][c]);
 #pragma unroll
       for (int col = 0; col < 2; ++col) {
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1)
           best[col] = fmaxf(best[col], __shfl_xor_sync(0xffffffffu, best[col], o));
-        const float higher = fmaxf(top[nt][col], best[col]);
+        // the reference moves only where a score has outgrown it by 2^8
+        const float higher = best[col] > top[nt][col] + kHeadroom ? best[col] : top[nt][col];
         any_moved |= higher + shift != top[nt][col] + shift_before;
         moved[nt][col] = higher == -INFINITY ? 1.0f : exp2_approx((top[nt][col] + shift_before) - (higher + shift));
         top[nt][col] = higher;
@@ -444,49 +518,39 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
             sum[nt][c & 1] += x[m][nt][c];
     }
     // ---- values -------------------------------------------------------------------------------------------------------------
-    if (!Q4 && tail) {
-      for (int u = lane; u < KT * 8 * S::slabs; u += 32) {
-        const int row = u / 8 % KT;
-        if (j0 + row >= seq.length)
-          *reinterpret_cast<uint4 *>(ring + s * S::slot_bytes + u * 16) = make_uint4(0, 0, 0, 0);
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-    }
 #pragma unroll
     for (int m = 0; m < M; ++m) {
       if constexpr (Q4) {
-        uint32_t sw[2][NB / 2];
+        uint32_t weights[NT][2]; // of keys 2 t, 2 t + 1 and 2 t + 8, 2 t + 9 in row g
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int k = 0; k < NB / 2; ++k) {
-            sw[h][k] = scale_words(s, m, h)[k];
-            if (tail && j0 + m * 16 + g + h * 8 >= seq.length)
-              sw[h][k] = 0;
-          }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
           for (int c = 0; c < 4; ++c)
             sum[nt][c & 1] += x[m][nt][c];
+          weights[nt][0] = transpose8x8(pack_f16(x[m][nt][0], x[m][nt][1]));
+          weights[nt][1] = transpose8x8(pack_f16(x[m][nt][2], x[m][nt][3]));
+        }
+        uint32_t sw[4][NB / 2];
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+          load_words(sw[n], scale_words(s, m * 16 + 2 * t + (n & 1) + (n >> 1) * 8));
 #pragma unroll
         for (int k = 0; k < NB; k += 2) {
           uint32_t w[4]; // block k: keys 0-7, 8-15; block k + 1 the same
-          ldmatrix4_trans(w, slot + piece_address(m * 16 + (lm_matrix & 1) * 8 + lm_row, k + (lm_matrix >> 1)));
+          ldmatrix4_trans(w, (slot + rows_first ^ k << 4) + m * 16 * S::row_bytes);
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const uint32_t lo = w[2 * u], hi = w[2 * u + 1], lo8 = lo >> 8, hi8 = hi >> 8;
-            const float d0 = f16_at(sw[0][(k + u) / 2], u), d1 = f16_at(sw[1][(k + u) / 2], u);
             uint32_t a[8] = {lo & 0x000f000fu, lo & 0x00f000f0u, hi & 0x000f000fu, hi & 0x00f000f0u,
                              lo8 & 0x000f000fu, lo8 & 0x00f000f0u, hi8 & 0x000f000fu, hi8 & 0x00f000f0u};
 #pragma unroll
             for (int n = 0; n < 8; ++n)
               a[n] = sub_f16(a[n], n & 1 ? 0x00800080u : 0x00080008u);
+            const uint32_t d0 = __byte_perm(sw[0][k / 2], sw[1][k / 2], u ? 0x7632 : 0x5410);
+            const uint32_t d1 = __byte_perm(sw[2][k / 2], sw[3][k / 2], u ? 0x7632 : 0x5410);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              const uint32_t b0 = transpose8x8(pack_f16(x[m][nt][0] * d0, x[m][nt][1] * d0));
-              const uint32_t b1 = transpose8x8(pack_f16(x[m][nt][2] * d1, x[m][nt][3] * d1));
+              const uint32_t b0 = mul_f16(weights[nt][0], d0), b1 = mul_f16(weights[nt][1], d1);
               mma16816<true>(out[2 * (k + u)][nt], a[0], a[1], a[2], a[3], b0, b1);
               mma16816<true>(out[2 * (k + u) + 1][nt], a[4], a[5], a[6], a[7], b0, b1);
             }
@@ -506,8 +570,8 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
           uint32_t a[4];
-          const int piece = 2 * mt + (lm_matrix & 1);
-          ldmatrix4_trans(a, slot + (piece >> 3) * (KT * 128) + piece_address(m * 16 + (lm_matrix >> 1) * 8 + lm_row, piece & 7));
+          const int piece = 2 * mt;
+          ldmatrix4_trans(a, (slot + pieces_first ^ (piece & 7) << 4) + (piece >> 3) * (KT * 128) + m * 16 * S::row_bytes);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             mma16816<false>(out[mt][nt], a[0], a[1], a[2], a[3], high[nt][0], high[nt][1]);
@@ -601,7 +665,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
 
 template <int D, bool Q4, int NT>
 cudaError_t launch(const PagedKv &kv, const PagedBatch &batch, const PagedAttention &call, const PagedSplit &split, int *status, cudaStream_t stream) {
-  using S = Shape<D, Q4>;
+  using S = Shape<D, Q4, NT>;
   Rows p;
   p.kv = kv, p.batch = batch, p.call = call;
   p.chunk = split.chunk, p.chunks = split.chunks;
@@ -614,7 +678,7 @@ cudaError_t launch(const PagedKv &kv, const PagedBatch &batch, const PagedAttent
     return cudaErrorNotSupported;
   if (!Q4)
     scales = values;
-  constexpr size_t ring = kWarps * S::slots * S::slot_bytes + (NT * D > 256 ? NT * D * 16 : 0);
+  constexpr size_t ring = kWarps * S::slots * S::slot_bytes + (Q4 || NT * D > 256 ? NT * D * 16 : 0);
   constexpr size_t parts = sizeof(float) * kWarps * NT * 8 * (D + 4);
   constexpr size_t smem = 1024 + (ring > parts ? ring : parts);
   const auto kernel = paged_rows_kernel<D, Q4, NT>;
@@ -631,7 +695,9 @@ cudaError_t launch(const PagedKv &kv, const PagedBatch &batch, const PagedAttent
 
 } // namespace
 
-int paged_rows_tile(const PagedKv &kv) { return kWarps * (kv.scales ? (kv.head_dim == 256 ? 32 : 64) : 4096 / kv.head_dim); }
+int paged_rows_tile(const PagedKv &kv, int rows) {
+  return kWarps * (kv.scales ? (kv.head_dim == 256 || rows > 8 ? 32 : 64) : 4096 / kv.head_dim);
+}
 
 cudaError_t launch_paged_rows(const PagedKv &kv, const PagedBatch &batch, const PagedAttention &call, const PagedSplit &split, int *status,
                               cudaStream_t stream) {
