@@ -10,14 +10,14 @@ namespace llmcp_b200 {
 
 namespace {
 
-// One CTA per (row, head): groups of head_dim / 4 threads take the chunks in turn.
+// One CTA per (row, head): groups of head_dim / 8 threads take the chunks in turn.
 template <int D>
 __global__ void __launch_bounds__(256)
 paged_merge_kernel(PagedKv kv, PagedBatch batch, PagedAttention call, PagedSplit split) {
-  constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
+  constexpr int kLanes = D / 8, kGroups = 256 / kLanes;
   __shared__ float weights[kMaxChunks];
   __shared__ float tops[8], totals[8];
-  __shared__ float4 parts[kGroups][kLanes];
+  __shared__ float4 parts[kGroups][kLanes][2];
   const int token = blockIdx.x, head = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   grid_dependency_sync();
   const int b = paged_owner(batch, token);
@@ -60,27 +60,32 @@ paged_merge_kernel(PagedKv kv, PagedBatch batch, PagedAttention call, PagedSplit
   if (lane == 0)
     totals[warp] = total;
   __syncthreads();
-  const int d = tid % kLanes * 4;
+  const int d = tid % kLanes * 8;
   const float *src = static_cast<const float *>(call.workspace) + row * D + d;
-  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f), y = x;
+  auto add = [](float4 &to, const float4 &v, float w) {
+    to.x = __fmaf_rn(v.x, w, to.x), to.y = __fmaf_rn(v.y, w, to.y), to.z = __fmaf_rn(v.z, w, to.z), to.w = __fmaf_rn(v.w, w, to.w);
+  };
 #pragma unroll 4
   for (int c = tid / kLanes; c < used; c += kGroups) {
-    const float4 v = *reinterpret_cast<const float4 *>(src + static_cast<int64_t>(c) * D);
-    const float w = weights[c];
-    acc.x = __fmaf_rn(v.x, w, acc.x), acc.y = __fmaf_rn(v.y, w, acc.y);
-    acc.z = __fmaf_rn(v.z, w, acc.z), acc.w = __fmaf_rn(v.w, w, acc.w);
+    const float4 *part = reinterpret_cast<const float4 *>(src + static_cast<int64_t>(c) * D);
+    add(x, part[0], weights[c]);
+    add(y, part[1], weights[c]);
   }
-  parts[tid / kLanes][tid % kLanes] = acc;
+  parts[tid / kLanes][tid % kLanes][0] = x;
+  parts[tid / kLanes][tid % kLanes][1] = y;
   __syncthreads();
   if (tid < kLanes) {
     for (int i = 1; i < kGroups; ++i) {
-      const float4 v = parts[i][tid];
-      acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+      add(x, parts[i][tid][0], 1.0f);
+      add(y, parts[i][tid][1], 1.0f);
     }
     total = 0.0f;
     for (int w = 0; w < 8; ++w)
       total += totals[w];
-    paged_store_out<D>(call, token, head, d, acc, total);
+    const float inv = total == 0.0f ? 0.0f : __fdiv_rn(1.0f, total);
+    paged_store_row<D>(call, token, head, d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv), make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv),
+                       call.gate ? paged_gate<D>(call, token, head, d) : make_uint4(0, 0, 0, 0));
   }
 }
 

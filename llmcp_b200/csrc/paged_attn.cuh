@@ -77,36 +77,43 @@ __device__ __forceinline__ float capped_log2(float x, float cap, float over_cap)
   return cap * kLog2e * __fmaf_rn(-2.0f, r, 1.0f);
 }
 
-// Four dimensions of a finished row: the sum over its weights' total (0 where there are none), the gate, bf16.
-template <int D>
-__device__ __forceinline__ void paged_store_out(const PagedAttention &call, int token, int head, int d, float4 acc, float total) {
-  const float inv = total == 0.0f ? 0.0f : __fdiv_rn(1.0f, total);
-  float v[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+// The gate of eight dimensions.
+template <int D> __device__ __forceinline__ uint4 paged_gate(const PagedAttention &call, int token, int head, int d) {
+  return *reinterpret_cast<const uint4 *>(call.gate + token * call.gate_row + head * call.gate_head + d);
+}
+
+// Eight dimensions of a finished row: times their gate, where there is one, as bf16.
+template <int D> __device__ __forceinline__ void paged_store_row(const PagedAttention &call, int token, int head, int d, float4 x, float4 y, uint4 gate8) {
+  float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
   if (call.gate) {
-    const uint2 raw = *reinterpret_cast<const uint2 *>(call.gate + token * call.gate_row + head * call.gate_head + d);
-    const float gate[4] = {__uint_as_float(raw.x << 16), __uint_as_float(raw.x & 0xffff0000u), __uint_as_float(raw.y << 16),
-                           __uint_as_float(raw.y & 0xffff0000u)};
+    const uint32_t w[4] = {gate8.x, gate8.y, gate8.z, gate8.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      v[i] = __fdividef(v[i], 1.0f + __expf(-fmaxf(gate[i], -80.0f))); // below -80 the gate is 0 to every bit of a bf16 sum
+    for (int i = 0; i < 8; ++i) {
+      const float gate = __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+      v[i] = __fdividef(v[i], 1.0f + __expf(-fmaxf(gate, -80.0f))); // below -80 the product is 0 beside any other value of a row
+    }
   }
-  uint2 words;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(words.x) : "f"(v[1]), "f"(v[0]));
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(words.y) : "f"(v[3]), "f"(v[2]));
-  *reinterpret_cast<uint2 *>(call.out + (static_cast<int64_t>(token) * call.heads + head) * D + d) = words;
+  uint32_t words[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(words[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
+  *reinterpret_cast<uint4 *>(call.out + (static_cast<int64_t>(token) * call.heads + head) * D + d) = make_uint4(words[0], words[1], words[2], words[3]);
 }
 
 __device__ __forceinline__ float2 *paged_part_sums(const PagedAttention &call, int tokens, int chunks, int head_dim) {
   return reinterpret_cast<float2 *>(static_cast<float *>(call.workspace) + static_cast<int64_t>(tokens) * call.heads * chunks * head_dim);
 }
 
+// A chunk's part of a row: eight dimensions of its sum, and (once) its reference and the sum of its weights.
 template <int D>
-__device__ __forceinline__ void paged_store_part(const PagedAttention &call, int tokens, int chunks, int chunk, int token, int head, int d, float4 acc,
-                                                 float top, float total) {
-  const int64_t row = (static_cast<int64_t>(token) * call.heads + head) * chunks + chunk;
-  *reinterpret_cast<float4 *>(static_cast<float *>(call.workspace) + row * D + d) = acc;
-  if (d == 0)
-    paged_part_sums(call, tokens, chunks, D)[row] = make_float2(top, total);
+__device__ __forceinline__ void paged_store_part(const PagedAttention &call, int chunks, int chunk, int token, int head, int d, float4 x, float4 y) {
+  float4 *to = reinterpret_cast<float4 *>(static_cast<float *>(call.workspace) + ((static_cast<int64_t>(token) * call.heads + head) * chunks + chunk) * D + d);
+  to[0] = x;
+  to[1] = y;
+}
+template <int D>
+__device__ __forceinline__ void paged_store_sums(const PagedAttention &call, int tokens, int chunks, int chunk, int token, int head, float top, float total) {
+  paged_part_sums(call, tokens, chunks, D)[(static_cast<int64_t>(token) * call.heads + head) * chunks + chunk] = make_float2(top, total);
 }
 #endif
 

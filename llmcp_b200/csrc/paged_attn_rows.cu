@@ -642,24 +642,34 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
       }
   __syncthreads();
   const int head0 = kvh * group;
-  for (int u = tid; u < rows * (D / 4); u += 32 * kWarps) {
-    const int row = u / (D / 4), d = u % (D / 4) * 4;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int u = tid; u < rows * (D / 8); u += 32 * kWarps) {
+    const int row = u / (D / 8), d = u % (D / 8) * 8;
+    float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
     float all = -INFINITY, total = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float4 v = *reinterpret_cast<const float4 *>(parts + (w * NT * 8 + row) * kPitch + d);
-      acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+      const float *part = parts + (w * NT * 8 + row) * kPitch + d;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        v[i] += part[i];
       all = fmaxf(all, warp_max[w][row]);
     }
 #pragma unroll
     for (int w = 0; w < kWarps; ++w)
       total += warp_max[w][row] == -INFINITY ? 0.0f : warp_sum[w][row] * exp2_approx(warp_max[w][row] - all);
     const int token = seq.first + row / group, head = head0 + row % group;
-    if (p.chunks == 1)
-      paged_store_out<D>(p.call, token, head, d, acc, total);
-    else
-      paged_store_part<D>(p.call, p.batch.tokens, p.chunks, chunk_index, token, head, d, acc, all, total);
+    if (p.chunks == 1) {
+      const float inv = total == 0.0f ? 0.0f : __fdiv_rn(1.0f, total);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        v[i] *= inv;
+      paged_store_row<D>(p.call, token, head, d, make_float4(v[0], v[1], v[2], v[3]), make_float4(v[4], v[5], v[6], v[7]),
+                         p.call.gate ? paged_gate<D>(p.call, token, head, d) : make_uint4(0, 0, 0, 0));
+    } else {
+      paged_store_part<D>(p.call, p.chunks, chunk_index, token, head, d, make_float4(v[0], v[1], v[2], v[3]), make_float4(v[4], v[5], v[6], v[7]));
+      if (d == 0)
+        paged_store_sums<D>(p.call, p.batch.tokens, p.chunks, chunk_index, token, head, all, total);
+    }
   }
 }
 

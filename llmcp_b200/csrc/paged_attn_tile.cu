@@ -6,15 +6,16 @@
 // f16 rows (paged_expand_kernel), value = code * scale / 8 rounded to f16 (2^-11; the 8 keeps the largest below f16's
 // end and goes into the factors), because every tile of rows would otherwise unpack the same keys again.
 //
-// One CTA, 320 threads:
+// One CTA, 384 threads (warp 11 only hands over its registers):
 //   warps 0-7  softmax, a thread per row: warps 0-3 take the even key tiles, 4-7 the odd ones.  A thread reads its scores
 //              from tensor memory, writes P over them and, when its row's reference moves, rescales its row of O there.
 //              The reference (a score that none has outgrown by more than 2^8) passes from tile to tile, between the two
 //              warps that share 32 rows, through shared memory; the exponentials of two tiles run side by side.
-//   warp 8     issues the MMAs: Q and P from tensor memory, K (K-major) and V (MN-major: rows are keys) from shared memory,
-//              both with the 128-byte swizzle.  Scores of tile i + 1 are issued before P V of tile i.
-//   warp 9     issues the TMA loads into a ring of tiles, in the order in which the MMAs take them: K0 K1 V0 K2 V1 ...
-// Tensor memory: two score buffers, O, Q; Q is written there from registers, so queries may have any strides.
+//   warp 8     one thread issues the MMAs: Q and P from tensor memory, K (K-major) and V (MN-major: rows are keys) from shared memory,
+//              both with the 128-byte swizzle.  Scores are issued two or three tiles ahead of P V.
+//   warp 9     issues the TMA loads into a ring of tiles, in the order in which the MMAs take them: K0 K1 K2 V0 K3 V1 ...
+//   warp 10    zeroes the rows of the last value tile that lie past the sequence: 0 times whatever they hold is not 0.
+// Q is written to tensor (or shared) memory from registers, so queries may have any strides.
 //
 // Every wait on a barrier is bounded; one that runs out raises a flag that all roles observe, the loader waits (bounded)
 // for its copies in flight, tensor memory is released and the status bit is set.
@@ -31,18 +32,26 @@ namespace {
 using namespace tc;
 
 constexpr int kRows = 128;
-constexpr int kSoftmaxWarps = 8, kMmaWarp = 8, kLoadWarp = 9, kThreads = 320;
+constexpr int kSoftmaxWarps = 8, kMmaWarp = 8, kLoadWarp = 9, kThreads = 384;
+// Registers a thread: 168 at launch (all there are for 12 warps), then 208 for the two softmax warpgroups, 88 for the third.
+constexpr int kSoftmaxRegisters = 208, kOtherRegisters = 88;
+static_assert(2 * kSoftmaxRegisters + kOtherRegisters == 3 * 168, "registers of the block");
 constexpr float kHeadroom = 8.0f;
 
 template <int D> struct Shape {
   static constexpr int keys = D == 256 ? 64 : 128; // per tile
   static constexpr int slabs = D / 64;
   static constexpr int slot_bytes = keys * D * 2;
-  static constexpr int slots = 6 * 32768 / slot_bytes; // 192 KB: one CTA on an SM, as tensor memory is one CTA's
-  // tensor memory, in columns
-  static constexpr int o_column = 2 * keys, q_column = o_column + D;
-  static_assert(q_column + D / 2 <= 512, "tensor memory");
-  static constexpr size_t smem = 1024 + static_cast<size_t>(slots) * slot_bytes;
+  // Tensor memory: score buffers, O, Q.  Three buffers let a warpgroup begin its next tile before the product of its last
+  // one is done; with 256 dimensions there is room for two only, with 128 Q goes to shared memory for the third's sake.
+  static constexpr int buffers = D == 256 ? 2 : 3;
+  static constexpr bool q_shared = D == 128;
+  static constexpr int o_column = buffers * keys, q_column = o_column + D;
+  static_assert(q_column + (q_shared ? 0 : D / 2) <= 512, "tensor memory");
+  static constexpr int q_bytes = q_shared ? kRows * D * 2 : 0;
+  static constexpr int slots = (6 * 32768 - q_bytes) / slot_bytes; // 192 KB: one CTA on an SM, as tensor memory is one CTA's
+  static constexpr int q_slot = slots - kRows * D * 2 / slot_bytes; // where Q waits on its way to tensor memory
+  static constexpr size_t smem = 1024 + q_bytes + static_cast<size_t>(slots) * slot_bytes;
 };
 
 struct Tile {
@@ -60,12 +69,19 @@ struct Tile {
 template <bool F16, int N, bool MN> constexpr uint32_t kInstruction =
     (1u << 4) | (F16 ? 0u : (1u << 7) | (1u << 10)) | (MN ? 1u << 16 : 0u) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(kRows >> 4) << 24);
 
-// A from tensor memory, B from shared memory.
+// A from tensor memory or shared memory, B from shared memory.
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t instruction, uint32_t accumulate) {
   asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0;\n"
-               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p; }"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }"
                :
-               : "r"(d), "r"(a), "l"(b), "r"(instruction), "r"(accumulate), "r"(0u)
+               : "r"(d), "r"(a), "l"(b), "r"(instruction), "r"(accumulate)
+               : "memory");
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t instruction, uint32_t accumulate) {
+  asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0;\n"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }"
+               :
+               : "r"(d), "l"(a), "l"(b), "r"(instruction), "r"(accumulate)
                : "memory");
 }
 
@@ -107,10 +123,34 @@ template <bool F16> __device__ __forceinline__ uint32_t pack16(float lo, float h
   return r;
 }
 
+// Two f32 values in one register pair.
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 halves(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 template <int SLOTS> struct Barriers {
   uint64_t full[SLOTS], empty[SLOTS]; // a tile of keys or values
-  uint64_t s_full[2];                 // scores of a tile are in tensor memory
-  uint64_t p_full[2];                 // its weights are
+  uint64_t s_full[3];                 // [buffer]: scores of a tile are in tensor memory
+  uint64_t p_full[3];                 // its weights are
+  uint64_t o_full;                    // every tile's P V has been added
+  uint64_t tail_here, tail_ready;     // the last tile of a sequence's values has landed; its rows past the end are zeros
   uint64_t q_full;                    // the queries are
   uint64_t o_done[2];                 // [tile & 1]: P V of a tile has been added
   uint64_t reference[2][4];           // [tile & 1][32 rows]: the reference after a tile
@@ -126,7 +166,8 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
   extern __shared__ uint8_t raw_smem[];
   __shared__ Barriers<S::slots> bars;
   __shared__ float references[kRows], last_reference[2][kRows], sums[2][kRows];
-  uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
+  uint8_t *q_sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
+  uint8_t *ring = q_sm + S::q_bytes;
   volatile int *abort_flag = &bars.abort_flag;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int kvh = blockIdx.x % p.kv.kv_heads, b = blockIdx.y, chunk_index = blockIdx.z;
@@ -137,9 +178,14 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
       mbar_init(&bars.full[i], 1);
       mbar_init(&bars.empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 3; ++i) {
       mbar_init(&bars.s_full[i], 1);
       mbar_init(&bars.p_full[i], 4);
+    }
+    mbar_init(&bars.o_full, 1);
+    mbar_init(&bars.tail_here, 1);
+    mbar_init(&bars.tail_ready, 1);
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.o_done[i], 1);
       for (int w = 0; w < 4; ++w)
         mbar_init(&bars.reference[i][w], 1);
@@ -150,7 +196,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
   }
   grid_dependency_sync();
   const PagedSequence seq = paged_sequence(p.batch, p.kv.page_shift, b, tid == 0 && blockIdx.x == 0 && chunk_index == 0 ? status : nullptr);
-  const int group = p.call.heads / p.kv.kv_heads;
+  const unsigned group = static_cast<unsigned>(p.call.heads) / static_cast<unsigned>(p.kv.kv_heads);
   const int token0 = q_tile * p.tokens_per_tile, tokens = min(p.tokens_per_tile, seq.count - token0);
   if (tokens <= 0)
     return;
@@ -172,19 +218,22 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
   tc_fence_after();
   const uint32_t tmem = bars.tmem_base;
 
+  if (warp >= kSoftmaxWarps) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
   if (warp == kLoadWarp) {
-    // ---- loader: item 0 is K0, then K(n+1) and V(n) in turn, the last one V(tiles - 1); a box per lane ---------------------------
+    // ---- loader: the first `ahead` tiles of keys, then values and keys in turn, as the MMAs take them; a box per lane -------------
     const int sub_boxes = KT / p.box_rows, boxes = S::slabs * sub_boxes;
     const int slab = lane / sub_boxes, sub = lane % sub_boxes;
     const int32_t *table = p.batch.page_table + b * p.batch.table_stride;
     const int head_rows = p.kv.kv_heads << p.kv.page_shift;
-    int issued = 0;
+    const int ahead = min(S::buffers, tiles);
+    int issued = 0, keys_issued = 0, values_issued = 0;
     bool ok = true;
     const int items = 2 * tiles;
     for (int n = 0; n < items && ok; ++n) {
-      // items 1, 2, 3, 4 ...: K1 V0 K2 V1 ...; with one tile only, item 1 is V0
-      const int which = n == 0 ? 0 : n == items - 1 ? 1 : (n & 1) ? 0 : 1;
-      const int i = n == 0 ? 0 : n == items - 1 ? tiles - 1 : (n & 1) ? (n + 1) / 2 : n / 2 - 1;
+      // K0 K1 (K2) V0 K.. V1 K.. ...: keys while fewer than `ahead` tiles lie between them and the values, and while there are any
+      const int which = keys_issued < tiles && keys_issued - values_issued < ahead ? 0 : 1;
+      const int i = which ? values_issued++ : keys_issued++;
       const int key = key0 + i * KT + sub * p.box_rows;
       int row = p.out_of_range;
       if (lane < boxes && key < seq.length) {
@@ -199,8 +248,10 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
         }
       }
       const int s = n % S::slots;
-      if (n >= S::slots)
-        ok = __all_sync(0xffffffffu, mbar_wait(&bars.empty[s], (n / S::slots - 1) & 1, abort_flag, p.spin_limit));
+      if (!S::q_shared && n == S::q_slot)
+        ok = __all_sync(0xffffffffu, mbar_wait<false>(&bars.q_full, 0, abort_flag, p.spin_limit));
+      if (ok && n >= S::slots)
+        ok = __all_sync(0xffffffffu, mbar_wait<false>(&bars.empty[s], (n / S::slots - 1) & 1, abort_flag, p.spin_limit));
       if (!ok)
         break;
       if (lane == 0)
@@ -212,131 +263,186 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
     }
     if (*abort_flag) // copies already requested still write into this CTA's shared memory
       for (int n = max(0, issued - S::slots); n < issued; ++n)
-        mbar_wait_quiet(&bars.full[n % S::slots], (n / S::slots) & 1, p.spin_limit);
+        mbar_wait_quiet<false>(&bars.full[n % S::slots], (n / S::slots) & 1, p.spin_limit);
   } else if (warp == kMmaWarp) {
-    // ---- MMA issue ---------------------------------------------------------------------------------------------------------------
-    auto all_wait = [&](uint64_t *bar, int parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.spin_limit)); };
-    const uint32_t ring_address = smem_u32(ring);
-    int taken = 0; // items of the ring
-    bool ok = tiles > 0 && all_wait(&bars.q_full, 0);
-    auto scores = [&](int i) {
-      const int s = taken % S::slots;
-      if (!all_wait(&bars.full[s], (taken / S::slots) & 1))
-        return false;
-      tc_fence_after();
-      if (lane == 0) {
-        const uint32_t k = ring_address + s * S::slot_bytes;
+    // ---- MMA issue: one thread ---------------------------------------------------------------------------------------------------
+    if (elect_one()) {
+      auto wait = [&](uint64_t *bar, int parity) { return mbar_wait<false>(bar, parity, abort_flag, p.spin_limit); };
+      const uint32_t ring_address = smem_u32(ring);
+      const uint64_t q_descriptor = operand_descriptor(smem_u32(q_sm)); // addresses in descriptors count in units of 16 bytes
+      int slot = 0, phase = 0, s_buffer = 0;
+      auto next_slot = [&]() {
+        if (++slot == S::slots) {
+          slot = 0;
+          phase ^= 1;
+        }
+      };
+      auto scores = [&]() {
+        if (!wait(&bars.full[slot], phase))
+          return false;
+        tc_fence_after();
+        const uint64_t k = operand_descriptor(ring_address + slot * S::slot_bytes);
+        const uint32_t to = tmem + s_buffer * KT;
 #pragma unroll
-        for (int n = 0; n < D / 16; ++n)
-          mma_ts(tmem + (i & 1) * KT, tmem + S::q_column + n * 8, operand_descriptor(k + (n / 4) * (KT * 128) + (n % 4) * 32), kInstruction<F16, KT, false>, n != 0);
-        mma_commit(&bars.empty[s]);
-        mma_commit(&bars.s_full[i & 1]);
+        for (int n = 0; n < D / 16; ++n) {
+          if constexpr (S::q_shared)
+            mma_ss(to, q_descriptor + ((n / 4) * (kRows * 128) + (n % 4) * 32) / 16, k + ((n / 4) * (KT * 128) + (n % 4) * 32) / 16, kInstruction<F16, KT, false>, n != 0);
+          else
+            mma_ts(to, tmem + S::q_column + n * 8, k + ((n / 4) * (KT * 128) + (n % 4) * 32) / 16, kInstruction<F16, KT, false>, n != 0);
+        }
+        mma_commit(&bars.s_full[s_buffer]);
+        mma_commit(&bars.empty[slot]);
+        next_slot();
+        s_buffer = s_buffer + 1 == S::buffers ? 0 : s_buffer + 1;
+        return true;
+      };
+      bool ok = tiles > 0 && wait(&bars.q_full, 0);
+      int scored = 0;
+      for (; ok && scored < min(S::buffers, tiles); ++scored) {
+        tc_fence_after();
+        ok = scores();
       }
-      __syncwarp();
-      ++taken;
-      return true;
-    };
-    ok = ok && scores(0);
-    for (int i = 0; i < tiles && ok; ++i) {
-      if (i + 1 < tiles)
-        ok = scores(i + 1);
-      const int s = taken % S::slots;
-      ok = ok && all_wait(&bars.full[s], (taken / S::slots) & 1);
-      if (!ok)
-        break;
-      const int past = seq.length - key0 - i * KT; // rows from here on are past the sequence: whatever they hold
-      if (past < KT) {
-        for (int u = lane; u < KT * 8 * S::slabs; u += 32)
-          if (u / 8 % KT >= past)
-            *reinterpret_cast<uint4 *>(ring + s * S::slot_bytes + u * 16) = make_uint4(0, 0, 0, 0);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-      }
-      ok = all_wait(&bars.p_full[i & 1], (i >> 1) & 1);
-      if (!ok)
-        break;
-      tc_fence_after();
-      if (lane == 0) {
-        const uint32_t v = ring_address + s * S::slot_bytes;
+      int p_buffer = 0, p_phase = 0;
+      for (int i = 0; i < tiles && ok; ++i) {
+        ok = wait(&bars.full[slot], phase);
+        if (ok && i == tiles - 1 && seq.length - key0 - i * KT < KT) { // rows past the sequence: whatever they hold
+          mbar_arrive(&bars.tail_here);
+          ok = wait(&bars.tail_ready, 0);
+        }
+        ok = ok && wait(&bars.p_full[p_buffer], p_phase);
+        if (!ok)
+          break;
+        tc_fence_after();
+        const uint64_t v = mn_descriptor(ring_address + slot * S::slot_bytes, KT * 128);
 #pragma unroll
         for (int n = 0; n < KT / 16; ++n)
-          mma_ts(tmem + S::o_column, tmem + (i & 1) * KT + n * 8, mn_descriptor(v + n * 2048, KT * 128), kInstruction<F16, D, true>, i != 0 || n != 0);
-        mma_commit(&bars.empty[s]);
+          mma_ts(tmem + S::o_column, tmem + p_buffer * KT + n * 8, v + n * (2048 / 16), kInstruction<F16, D, true>, i != 0 || n != 0);
         mma_commit(&bars.o_done[i & 1]);
+        mma_commit(&bars.empty[slot]);
+        next_slot();
+        if (++p_buffer == S::buffers) {
+          p_buffer = 0;
+          p_phase ^= 1;
+        }
+        if (scored < tiles) { // into the buffer that this tile's weights leave: products run in the order of their issue
+          ok = scores();
+          ++scored;
+        }
       }
-      __syncwarp();
-      ++taken;
+      if (ok)
+        mma_commit(&bars.o_full);
     }
+    __syncwarp();
+  } else if (warp == kMmaWarp + 2 && tiles > 0) {
+    // ---- values of the last tile past the sequence ----------------------------------------------------------------------------------
+    const int past = seq.length - key0 - (tiles - 1) * KT;
+    if (past < KT && __all_sync(0xffffffffu, mbar_wait(&bars.tail_here, 0, abort_flag, p.spin_limit))) {
+      uint8_t *tile = ring + (2 * tiles - 1) % S::slots * S::slot_bytes;
+      for (int u = lane; u < KT * 8 * S::slabs; u += 32)
+        if (u / 8 % KT >= past)
+          *reinterpret_cast<uint4 *>(tile + u * 16) = make_uint4(0, 0, 0, 0);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0)
+        mbar_arrive(&bars.tail_ready);
+    }
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
     // ---- softmax: a thread per row -----------------------------------------------------------------------------------------------
     const int half = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-    const bool valid = row < tokens * group;
-    const int token = seq.first + token0 + (valid ? row / group : 0), head = kvh * group + (valid ? row % group : 0);
-    const uint16_t *q = p.call.q + token * p.call.q_row + head * p.call.q_head;
+    const bool valid = row < static_cast<int>(tokens * group);
+    const int head0 = kvh * static_cast<int>(group), token_first = seq.first + token0;
     float factor = p.call.scale * (p.call.softcap > 0.0f ? 1.0f : 1.4426950408889634f);
     const bool negative = factor < 0.0f; // goes into the queries: the largest product is the largest score
-    const bool flat = factor == 0.0f; // every score is 0: so are the queries, and the factor stays usable beside -infinity
+    const bool flat = factor == 0.0f;    // every score is 0: so are the queries, and the factor stays usable beside -infinity
     factor = flat ? 1.0f : fabsf(factor);
-    uint32_t mult_bits = 0x3f800000u;
-    if constexpr (F16) { // a power of two per row takes the largest |q| into [2^14, 2^15); keys are 1 / 8 of themselves
-      uint32_t top = 0;
-      for (int k = 0; k < D / 8; ++k) {
-        const uint4 v = valid ? reinterpret_cast<const uint4 *>(q)[k] : make_uint4(0, 0, 0, 0);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    // Rows come in whole, a lane 16 bytes of one; they go to shared memory as the swizzle has them, K-major slabs of 64
+    // dimensions: where the MMAs read them, or in the ring's last slots for the threads that take them to tensor memory.
+    constexpr int kLanes = D / 8, kSide = 32 / kLanes;
+    uint8_t *staged = S::q_shared ? q_sm : ring + S::q_slot * S::slot_bytes;
+    constexpr int kStep = kSoftmaxWarps * kSide, kMine = kRows / kStep; // rows of a lane: all requested at once
+    const int piece = lane % kLanes, first_row = warp * kSide + lane / kLanes;
+    uint4 pieces[kMine];
+#pragma unroll
+    for (int n = 0; n < kMine; ++n) {
+      const unsigned r = first_row + n * kStep;
+      pieces[n] = make_uint4(0, 0, 0, 0);
+      if (r < static_cast<unsigned>(tokens * group) && !flat)
+        pieces[n] = *reinterpret_cast<const uint4 *>(p.call.q + (token_first + r / group) * p.call.q_row + (head0 + r % group) * p.call.q_head + piece * 8);
+    }
+#pragma unroll
+    for (int n = 0; n < kMine; ++n) {
+      const int r = first_row + n * kStep;
+      const uint4 v = pieces[n];
+      uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      if constexpr (F16) { // a power of two per row takes the largest |q| into [2^14, 2^15); keys are 1 / 8 of themselves
+        uint32_t top2 = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          top = max(top, max(w[i] & 0x7fffu, w[i] >> 16 & 0x7fffu));
+          top2 = __vmaxu2(top2, w[i] & 0x7fff7fffu);
+#pragma unroll
+        for (int o = 1; o < kLanes; o <<= 1)
+          top2 = __vmaxu2(top2, __shfl_xor_sync(0xffffffffu, top2, o));
+        const uint32_t top = max(top2 & 0xffffu, top2 >> 16);
+        const int up = top == 0 ? 0 : min(126, 14 - (static_cast<int>(top >> 7) - 127));
+        const float mult = __uint_as_float(static_cast<uint32_t>(up + 127) << 23 | (negative ? 0x80000000u : 0u));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          w[i] = pack16<true>(__uint_as_float(w[i] << 16) * mult, __uint_as_float(w[i] & 0xffff0000u) * mult);
+        if (piece == 0)
+          references[r] = __int_as_float(min(254, 3 - up + 127) << 23);
+      } else if (negative) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          w[i] ^= 0x80008000u;
       }
-      const int up = top == 0 ? 0 : min(126, 14 - (static_cast<int>(top >> 7) - 127));
-      mult_bits = static_cast<uint32_t>(up + 127) << 23;
-      factor *= __int_as_float(min(254, 3 - up + 127) << 23);
+      *reinterpret_cast<uint4 *>(staged + (piece / 8) * (kRows * 128) + r * 128 + ((piece % 8 ^ r & 7) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    const float mult = __uint_as_float(mult_bits | (negative ? 0x80000000u : 0u));
-#pragma unroll 1
-    for (int c = 0; c < D / 2 / 32; ++c) { // 32 dimensions = 16 columns at a time; this half's
-      const int d = half * (D / 2) + c * 32;
-      uint32_t w[16];
+    if constexpr (S::q_shared)
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    asm volatile("bar.sync 1, 256;" ::: "memory"); // the softmax warps
+    if constexpr (F16)
+      factor *= references[row];
+    if constexpr (!S::q_shared) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint4 v = valid ? *reinterpret_cast<const uint4 *>(q + d + 8 * k) : make_uint4(0, 0, 0, 0);
-        w[4 * k] = v.x, w[4 * k + 1] = v.y, w[4 * k + 2] = v.z, w[4 * k + 3] = v.w;
-      }
-      if (flat) {
+      for (int c = 0; c < D / 2 / 32; ++c) { // 32 dimensions = 16 columns at a time; half of them each
+        const int d = half * (D / 2) + c * 32;
+        uint32_t w[16];
 #pragma unroll
-        for (int k = 0; k < 16; ++k)
-          w[k] = 0;
+        for (int k = 0; k < 4; ++k) {
+          const uint4 v = *reinterpret_cast<const uint4 *>(staged + (d / 64) * (kRows * 128) + row * 128 + ((d % 64 / 8 + k ^ row & 7) << 4));
+          w[4 * k] = v.x, w[4 * k + 1] = v.y, w[4 * k + 2] = v.z, w[4 * k + 3] = v.w;
+        }
+        tmem_store16(lanes + S::q_column + d / 2, w);
       }
-#pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        if constexpr (F16)
-          w[k] = pack16<true>(__uint_as_float(w[k] << 16) * mult, __uint_as_float(w[k] & 0xffff0000u) * mult);
-        else
-          w[k] ^= negative ? 0x80008000u : 0u;
-      }
-      tmem_store16(lanes + S::q_column + d / 2, w);
+      tmem_wait_stores();
+      tc_fence_before();
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // the loader's copies into these slots come after
     }
-    tmem_wait_stores();
-    tc_fence_before();
     __syncwarp();
     if (lane == 0)
       mbar_arrive(&bars.q_full);
+    if constexpr (F16)
+      asm volatile("bar.sync 1, 256;" ::: "memory"); // the factors have been read: their place is the references' now
 
-    const int position = seq.length - seq.count + token0 + row / group;
+    const int position = seq.length - seq.count + token0 + static_cast<int>(row / group);
     const int sees = valid ? max(0, min(seq.length, max(position + 1, prefix))) : 0;
     const float cap = p.call.softcap, over_cap = cap > 0.0f ? 1.0f / cap : 0.0f;
     const bool biased = p.call.slopes != nullptr;
-    const float slope = biased && valid ? p.call.slopes[head] * 1.4426950408889634f : 0.0f, at = static_cast<float>(position);
+    const float slope = biased && valid ? p.call.slopes[head0 + row % group] * 1.4426950408889634f : 0.0f, at = static_cast<float>(position);
     float reference = -INFINITY, sum = 0.0f;
-    auto o_wait = [&](int i) { return __all_sync(0xffffffffu, mbar_wait(&bars.o_done[i & 1], (i >> 1) & 1, abort_flag, p.spin_limit)); };
+    auto o_wait = [&](int i) { return __all_sync(0xffffffffu, mbar_wait<false>(&bars.o_done[i & 1], (i >> 1) & 1, abort_flag, p.spin_limit)); };
     bool ok = true;
+    int buffer = half, buffer_phase = 0; // tile i is in buffer i % buffers
     for (int i = half; i < tiles; i += 2) {
       const int j0 = key0 + i * KT;
-      ok = __all_sync(0xffffffffu, mbar_wait(&bars.s_full[half], (i >> 1) & 1, abort_flag, p.spin_limit));
+      ok = __all_sync(0xffffffffu, mbar_wait<false>(&bars.s_full[buffer], buffer_phase, abort_flag, p.spin_limit));
       if (!ok)
         break;
       tc_fence_after();
-      const uint32_t s_at = lanes + half * KT;
+      const uint32_t s_at = lanes + buffer * KT;
       uint32_t x[KT / 32][32];
 #pragma unroll
       for (int c = 0; c < KT / 32; ++c)
@@ -369,17 +475,21 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
             if (j0 + c * 32 + u >= sees)
               x[c][u] = 0xff800000u;
       }
-      float best = -INFINITY;
+      float most[8]; // side by side: one chain of maxima would take as long as everything else
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        most[u] = -INFINITY;
 #pragma unroll
       for (int c = 0; c < KT / 32; ++c)
 #pragma unroll
         for (int u = 0; u < 32; ++u)
-          best = fmaxf(best, __uint_as_float(x[c][u]));
+          most[u & 7] = fmaxf(most[u & 7], __uint_as_float(x[c][u]));
+      float best = fmaxf(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])), fmaxf(fmaxf(most[4], most[5]), fmaxf(most[6], most[7])));
       best = best == -INFINITY ? best : best * scaled;
       // the reference after the tile in front
       float before = -INFINITY;
       if (i > 0) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&bars.reference[half ^ 1][quarter], ((i - 1) >> 1) & 1, abort_flag, p.spin_limit));
+        ok = __all_sync(0xffffffffu, mbar_wait<false>(&bars.reference[half ^ 1][quarter], ((i - 1) >> 1) & 1, abort_flag, p.spin_limit));
         if (!ok)
           break;
         before = references[row];
@@ -395,7 +505,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
       }
       if (__any_sync(0xffffffffu, now != before) && i > 0) {
         // O holds every tile up to i - 1 once the product of that one is done.  (A wait by parity tells a phase from its
-        // neighbours only: the barrier's one before, tile i - 3, is done, or these scores would not be there.)
+        // neighbours only: the one before, tile i - 3, is done, or the scores of this one would not be there.)
         ok = o_wait(i - 1);
         if (!ok)
           break;
@@ -414,32 +524,47 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
       }
       // f16 weights lie between 2^7 (a row's largest, at least) and 2^15, and keep their precision down to 2^-14
       const float minus = (now == -INFINITY ? 0.0f : -now) + (F16 ? 15.0f - kHeadroom : 0.0f);
+      uint64_t added[4] = {0, 0, 0, 0}; // pairs of sums
+      const uint64_t scaled2 = pair(scaled, scaled), minus2 = pair(minus, minus);
 #pragma unroll
       for (int c = 0; c < KT / 32; ++c) {
         uint32_t w[16];
 #pragma unroll
         for (int u = 0; u < 32; u += 2) {
-          const float p0 = exp2_approx(__fmaf_rn(__uint_as_float(x[c][u]), scaled, minus));
-          const float p1 = exp2_approx(__fmaf_rn(__uint_as_float(x[c][u + 1]), scaled, minus));
-          sum += p0 + p1;
+          const float2 y = halves(fma2(pair(__uint_as_float(x[c][u]), __uint_as_float(x[c][u + 1])), scaled2, minus2));
+          const float p0 = exp2_approx(y.x), p1 = exp2_approx(y.y);
+          added[u >> 1 & 3] = add2(added[u >> 1 & 3], pair(p0, p1));
           w[u >> 1] = pack16<F16>(p0, p1);
         }
         tmem_store16(s_at + c * 16, w);
       }
+      const float2 added2 = halves(add2(add2(added[0], added[1]), add2(added[2], added[3])));
+      sum += added2.x + added2.y;
       tmem_wait_stores();
       tc_fence_before();
       __syncwarp();
       if (lane == 0)
-        mbar_arrive(&bars.p_full[half]);
+        mbar_arrive(&bars.p_full[buffer]);
+      buffer += 2;
+      if (buffer >= S::buffers) {
+        buffer -= S::buffers;
+        buffer_phase ^= 1;
+      }
     }
     // ---- epilogue: the two halves' sums, then half of the dimensions each -----------------------------------------------------------
     last_reference[half][row] = reference;
     sums[half][row] = sum;
     asm volatile("bar.sync 1, 256;" ::: "memory"); // the softmax warps
-    if (ok && tiles > 1) // for the sake of the parity of the next wait
-      ok = o_wait(tiles - 2);
+    if (p.call.gate && p.chunks == 1) { // on their way while the last products run
+#pragma unroll
+      for (int n = 0; n < kMine; ++n) {
+        const unsigned r = first_row + n * kStep;
+        if (r < static_cast<unsigned>(tokens * group))
+          pieces[n] = paged_gate<D>(p.call, token_first + r / group, head0 + r % group, piece * 8);
+      }
+    }
     if (ok && tiles > 0)
-      ok = o_wait(tiles - 1);
+      ok = __all_sync(0xffffffffu, mbar_wait<false>(&bars.o_full, 0, abort_flag, p.spin_limit));
     if (ok) {
       tc_fence_after();
       const float final_reference = tiles > 0 ? references[row] : -INFINITY;
@@ -447,26 +572,43 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         total += last_reference[h][row] == -INFINITY ? 0.0f : sums[h][row] * exp2_approx(last_reference[h][row] - final_reference);
-      constexpr float kUnscale = F16 ? 8.0f : 1.0f; // values are 1 / 8 of themselves
+      // rows of O by thread into shared memory (the ring is done with), then whole rows out
+      constexpr int kPitch = D + 4;
+      float *rows_out = reinterpret_cast<float *>(ring);
+      // values are 1 / 8 of themselves in f16; where a row has seen nothing O may hold anything
+      const float unscale = (F16 ? 8.0f : 1.0f) * (total == 0.0f ? 0.0f : p.chunks == 1 ? __fdiv_rn(1.0f, total) : 1.0f);
 #pragma unroll 1
       for (int c = 0; c < D / 2 / 32; ++c) {
         const int d = half * (D / 2) + c * 32;
         uint32_t o[32];
         __syncwarp();
         tmem_load32(lanes + S::o_column + d, o);
-        if (!valid)
-          continue;
 #pragma unroll
         for (int u = 0; u < 32; u += 4) {
-          float4 acc = make_float4(__uint_as_float(o[u]) * kUnscale, __uint_as_float(o[u + 1]) * kUnscale, __uint_as_float(o[u + 2]) * kUnscale,
-                                   __uint_as_float(o[u + 3]) * kUnscale);
-          if (total == 0.0f) // nothing seen: O may hold anything
-            acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          if (p.chunks == 1)
-            paged_store_out<D>(p.call, token, head, d + u, acc, total);
-          else
-            paged_store_part<D>(p.call, p.batch.tokens, p.chunks, chunk_index, token, head, d + u, acc, final_reference, total);
+          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (total != 0.0f)
+            v = make_float4(__uint_as_float(o[u]) * unscale, __uint_as_float(o[u + 1]) * unscale, __uint_as_float(o[u + 2]) * unscale,
+                            __uint_as_float(o[u + 3]) * unscale);
+          *reinterpret_cast<float4 *>(rows_out + row * kPitch + d + u) = v;
         }
+      }
+      if (p.chunks > 1 && half == 0 && valid)
+        paged_store_sums<D>(p.call, p.batch.tokens, p.chunks, chunk_index, token_first + row / group, head0 + row % group, final_reference, total);
+    }
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    if (ok) {
+      const float *rows_out = reinterpret_cast<const float *>(ring);
+#pragma unroll
+      for (int n = 0; n < kMine; ++n) {
+        const unsigned r = first_row + n * kStep;
+        if (r >= static_cast<unsigned>(tokens * group))
+          break;
+        const int d = piece * 8, token = token_first + r / group, head = head0 + r % group;
+        const float4 x = *reinterpret_cast<const float4 *>(rows_out + r * (D + 4) + d), y = *reinterpret_cast<const float4 *>(rows_out + r * (D + 4) + d + 4);
+        if (p.chunks == 1)
+          paged_store_row<D>(p.call, token, head, d, x, y, pieces[n]);
+        else
+          paged_store_part<D>(p.call, p.chunks, chunk_index, token, head, d, x, y);
       }
     }
   }
@@ -542,7 +684,7 @@ cudaError_t launch(const PagedKv &kv, const PagedBatch &batch, const PagedAttent
   p.kv = kv, p.batch = batch, p.call = call;
   p.chunk = split.chunk, p.chunks = split.chunks;
   p.tokens_per_tile = kRows / group;
-  p.spin_limit = kSpinLimit<true>;
+  p.spin_limit = kSpinLimit<false>;
   const int page = 1 << kv.page_shift;
   PagedKv source = kv;
   int64_t rows = kv.num_pages * 2 * kv.kv_heads << kv.page_shift;
