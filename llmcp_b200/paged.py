@@ -52,20 +52,19 @@ def _refuse(what):
 
 
 def _tensor(t, name, dtype, dims, device):
-    """The address of ``t``, which has to have that type and rank, lie on that device and be dense in its last dimension."""
-    if t.dtype is not dtype:
-        _refuse(f"{name} has to be {dtype}")
-    if t.ndim != dims:
-        _refuse(f"{name} has to have {dims} dimensions")
-    if t.get_device() != device.index:
-        _refuse(f"{name} has to lie on {device}")
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
-        _refuse(f"{name} has to be dense in its last dimension")
-    return t.data_ptr()
+    """The address and strides of ``t``, which has to have that type and rank, lie on that device and be dense in its last
+    dimension.  (These checks are most of a small call's time: one look at the strides, messages only where needed.)"""
+    strides = t.stride()
+    if t.dtype is not dtype or len(strides) != dims or t.get_device() != device.index or (strides[-1] != 1 and t.shape[-1] > 1):
+        _refuse(f"{name} has to be {dtype}" if t.dtype is not dtype else
+                f"{name} has to have {dims} dimensions" if len(strides) != dims else
+                f"{name} has to lie on {device}" if t.get_device() != device.index else
+                f"{name} has to be dense in its last dimension")
+    return t.data_ptr(), strides
 
 
 def _optional(t, name, dtype, dims, device):
-    return None if t is None else _tensor(t, name, dtype, dims, device)
+    return None if t is None else _tensor(t, name, dtype, dims, device)[0]
 
 
 class Cache:
@@ -103,13 +102,11 @@ class Batch:
         device = q_start.device
         if not q_start.is_cuda:
             _refuse("q_start has to lie on a CUDA device")
-        starts = _tensor(q_start, "q_start", torch.int32, 1, device)
-        lengths = _tensor(kv_len, "kv_len", torch.int32, 1, device)
-        table = _tensor(page_table, "page_table", torch.int32, 2, device)
+        starts, lengths = _tensor(q_start, "q_start", torch.int32, 1, device)[0], _tensor(kv_len, "kv_len", torch.int32, 1, device)[0]
+        table, (stride, _) = _tensor(page_table, "page_table", torch.int32, 2, device)
         sequences, width = page_table.shape
         if q_start.shape[0] != sequences + 1 or kv_len.shape[0] != sequences:
             _refuse("q_start has one entry more than kv_len and page_table have rows")
-        stride = page_table.stride(0)
         if sequences > 1 and stride < width:
             _refuse("rows of page_table overlap")
         self.q_start, self.kv_len, self.page_table, self.device, self.sequences = q_start, kv_len, page_table, device, sequences
@@ -150,21 +147,21 @@ def append(cache, batch, q, k, v, cos=None, sin=None, q_norm=None, k_norm=None, 
     in their pages and returns the queries.  Rotation: the first cos.shape[1] dimensions by rows ``position`` of cos and
     sin (float32); none without them.  ``q`` may be None (keys and values only; returns None)."""
     dev, bf, dim = cache.device, torch.bfloat16, cache.head_dim
-    kp, vp = _tensor(k, "k", bf, 3, dev), _tensor(v, "v", bf, 3, dev)
+    (kp, ks), (vp, vs) = _tensor(k, "k", bf, 3, dev), _tensor(v, "v", bf, 3, dev)
     shape = k.shape
     tokens = shape[0]
     if shape[1] != cache.kv_heads or shape[2] != dim or v.shape != shape:
         _refuse("k and v have to be [tokens, kv_heads, head_dim]")
     qp, op, strides = None, None, (0, 0, 0)
     if q is not None:
-        qp, shape = _tensor(q, "q", bf, 3, dev), q.shape
+        (qp, qs), shape = _tensor(q, "q", bf, 3, dev), q.shape
         if shape[0] != tokens or shape[2] != dim:
             _refuse("q has to be [tokens, heads, head_dim]")
         if q_out is None:
             q_out = torch.empty(shape, dtype=bf, device=dev)
         elif q_out.shape != shape or not q_out.is_contiguous():
             _refuse("q_out has to be [tokens, heads, head_dim], contiguous")
-        op, strides = _tensor(q_out, "q_out", bf, 3, dev), (q.stride(0), q.stride(1), shape[1])
+        op, strides = _tensor(q_out, "q_out", bf, 3, dev)[0], (qs[0], qs[1], shape[1])
     norms = _optional(q_norm, "q_norm", bf, 1, dev), _optional(k_norm, "k_norm", bf, 1, dev)
     if (q_norm is not None and q_norm.shape[0] != dim) or (k_norm is not None and k_norm.shape[0] != dim):
         _refuse("q_norm and k_norm have to have head_dim elements")
@@ -172,12 +169,13 @@ def append(cache, batch, q, k, v, cos=None, sin=None, q_norm=None, k_norm=None, 
         _refuse("cos and sin come together")
     tables, rows, rot = (None, None), 0, 0
     if cos is not None:
-        tables = _tensor(cos, "cos", torch.float32, 2, dev), _tensor(sin, "sin", torch.float32, 2, dev)
-        if cos.shape != sin.shape or not cos.is_contiguous() or not sin.is_contiguous():
-            _refuse("cos and sin have to be [positions, rot], contiguous")
+        (cp, cs), (sp, ss) = _tensor(cos, "cos", torch.float32, 2, dev), _tensor(sin, "sin", torch.float32, 2, dev)
         rows, rot = cos.shape
+        if cos.shape != sin.shape or (rows > 1 and (cs[0] != rot or ss[0] != rot)):
+            _refuse("cos and sin have to be [positions, rot], contiguous")
+        tables = cp, sp
     _checked(_library().llmcp_dev_paged_append(
-        cache._c, batch._c(cache, tokens), qp, *strides, kp, k.stride(0), k.stride(1), vp, v.stride(0), v.stride(1), *norms, eps, *tables,
+        cache._c, batch._c(cache, tokens), qp, *strides, kp, ks[0], ks[1], vp, vs[0], vs[1], *norms, eps, *tables,
         rows, rot, op, _optional(status, "status", torch.int32, 1, dev), _stream(cache)))
     return q_out
 
@@ -215,21 +213,20 @@ def attention(cache, batch, q, scale=None, softcap=0.0, slopes=None, prefix=None
     ``gate`` like q.  ``workspace``: a uint8 tensor of workspace_bytes() that no other call uses meanwhile; taken from
     torch's allocator where it is not given."""
     dev, bf = cache.device, torch.bfloat16
-    qp, shape = _tensor(q, "q", bf, 3, dev), q.shape
+    (qp, qs), shape = _tensor(q, "q", bf, 3, dev), q.shape
     tokens, heads, dim = shape
     if dim != cache.head_dim or heads < 1 or heads % cache.kv_heads:
         _refuse("q has to be [tokens, heads, head_dim], heads a multiple of kv_heads")
     if out is None:
         out = torch.empty(shape, dtype=bf, device=dev)
-    op = _tensor(out, "out", bf, 3, dev)
-    if out.shape != shape or not out.is_contiguous():
+    op, strides = _tensor(out, "out", bf, 3, dev)
+    if out.shape != shape or (tokens and strides != (heads * dim, dim, 1) and not out.is_contiguous()):
         _refuse("out has to be [tokens, heads, head_dim], contiguous")
-    gp, gate_strides = None, (0, 0)
+    gp, gate_strides = None, (0, 0, 1)
     if gate is not None:
-        gp = _tensor(gate, "gate", bf, 3, dev)
+        gp, gate_strides = _tensor(gate, "gate", bf, 3, dev)
         if gate.shape != shape:
             _refuse("gate has to have q's shape")
-        gate_strides = gate.stride(0), gate.stride(1)
     sp, pp = _optional(slopes, "slopes", torch.float32, 1, dev), _optional(prefix, "prefix", torch.int32, 1, dev)
     if slopes is not None and slopes.shape[0] != heads:
         _refuse("slopes has to have one value per head")
@@ -241,6 +238,6 @@ def attention(cache, batch, q, scale=None, softcap=0.0, slopes=None, prefix=None
         workspace = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     wp = _optional(workspace, "workspace", torch.uint8, 1, dev)
     _checked(_library().llmcp_dev_paged_attention(
-        cache._c, rows, qp, q.stride(0), q.stride(1), heads, dim ** -0.5 if scale is None else scale, softcap, sp, pp, gp, *gate_strides, op,
+        cache._c, rows, qp, qs[0], qs[1], heads, dim ** -0.5 if scale is None else scale, softcap, sp, pp, gp, gate_strides[0], gate_strides[1], op,
         wp, 0 if wp is None else workspace.numel(), _optional(status, "status", torch.int32, 1, dev), _stream(cache)))
     return out
