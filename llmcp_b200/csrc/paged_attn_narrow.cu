@@ -1,13 +1,13 @@
-// Attention over the paged cache for many rows (prompts), 64 and 128 dimensions: as paged_attn_tile.cu, but two tiles of 128
-// rows in a CTA, which share every tile of keys and values.
+// Attention over the paged cache for many rows (prompts), 64 and 128 dimensions: as paged_attn_tile.cu, but O leaves room in
+// tensor memory, so two CTAs share an SM: while one loads, waits or writes, the other computes.  Each has 128 rows, a
+// thread per row, two buffers of 64 scores and O in 256 columns, the queries in shared memory.  (One CTA with two tiles of
+// rows that share the keys measured the same on long prompts and 15 % longer on short ones, where its longest tile
+// decides.)
 //
-// Each tile of rows has a warpgroup, an O and two score buffers of 64 keys in tensor memory of its own (D + 128 columns, 512
-// for both at 128 dimensions), so the two depend on each other only through the ring: while one computes weights, the
-// other's products run.  A tile of keys costs 64 x 256 rows of exponentials (1024 cycles at 16 a cycle) and, at 128
-// dimensions, 1024 cycles of products.  Queries lie in shared memory.
+// A tile of 64 keys costs 512 cycles of exponentials (16 a cycle, less what the multipliers take over) and, at 128
+// dimensions, 640 cycles of products: the scores' operands both come from shared memory, 128 bytes a cycle.
 //
-//   warps 0-3, 4-7  softmax of the first and second tile of rows;  8, 9  MMA issue for them (one thread each);  10  TMA loads;
-//   11  zeroes the rows of the last value tile past the sequence.
+//   warps 0-3  softmax;  4  MMA issue (one thread);  5  TMA loads;  6  zeroes the rows of the last value tile past the sequence.
 
 #include "paged_attn_tc.cuh"
 
@@ -18,26 +18,27 @@ namespace {
 using namespace tc;
 
 constexpr int KT = 64;
-constexpr int kMmaWarp = 8, kLoadWarp = 10, kTailWarp = 11, kThreads = 384; // MMA warps 8 and 9: one for each tile of rows
+
+constexpr int kMmaWarp = 4, kLoadWarp = 5, kTailWarp = 6, kThreads = 224;
 
 template <int D> struct Shape {
   static constexpr int slabs = D / 64;
   static constexpr int slot_bytes = KT * D * 2;
-  static constexpr int q_bytes = kRows * D * 2; // of a tile of rows
-  static constexpr int slots = D == 128 ? 8 : 16;
-  static constexpr int columns = 2 * KT + D; // of a tile of rows: scores, scores, O
-  static_assert(2 * columns <= 512, "tensor memory");
+  static constexpr int q_bytes = kRows * D * 2;
+  static constexpr int slots = D == 128 ? 4 : 8; // 64 KB
+  static constexpr int o_column = 2 * KT;        // tensor memory: two score buffers, O
+  static_assert(o_column + D <= 256, "tensor memory of one of two CTAs");
   // results leave as f32 rows over the queries and the ring
-  static constexpr size_t buffers = 2 * q_bytes + slots * slot_bytes, results = 2 * kRows * (D + 4) * sizeof(float);
+  static constexpr size_t buffers = q_bytes + slots * slot_bytes, results = kRows * (D + 4) * sizeof(float);
   static constexpr size_t smem = 1024 + (buffers > results ? buffers : results);
 };
 
 template <int SLOTS> struct Barriers {
   uint64_t full[SLOTS], empty[SLOTS]; // a tile of keys or values
   uint64_t q_full;                    // the queries are in shared memory
-  uint64_t s_full[2][2];              // [tile of rows][key tile & 1]: scores are in tensor memory
-  uint64_t p_full[2][2];              // their weights are
-  uint64_t o_done[2][2];              // P V has been added
+  uint64_t s_full[2];                 // [key tile & 1]: scores are in tensor memory
+  uint64_t p_full[2];                 // their weights are
+  uint64_t o_done[2];                 // P V has been added
   uint64_t o_full;                    // all of it
   uint64_t tail_here, tail_ready;     // the last tile of a sequence's values has landed; its rows past the end are zeros
   uint32_t tmem_base;
@@ -45,14 +46,14 @@ template <int SLOTS> struct Barriers {
 };
 
 template <int D, bool F16>
-__global__ void __launch_bounds__(kThreads, 1)
-paged_pair_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_constant__ Tile p, int *__restrict__ status) {
+__global__ void __launch_bounds__(kThreads, 2)
+paged_narrow_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_constant__ Tile p, int *__restrict__ status) {
   using S = Shape<D>;
   extern __shared__ uint8_t raw_smem[];
   __shared__ Barriers<S::slots> bars;
-  __shared__ float unscales[2][kRows];
+  __shared__ float unscales[kRows];
   uint8_t *q_sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
-  uint8_t *ring = q_sm + 2 * S::q_bytes;
+  uint8_t *ring = q_sm + S::q_bytes;
   volatile int *abort_flag = &bars.abort_flag;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int kvh = blockIdx.x % p.kv.kv_heads, b = blockIdx.y, chunk_index = blockIdx.z;
@@ -61,17 +62,16 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
   if (tid == 0) {
     for (int i = 0; i < S::slots; ++i) {
       mbar_init(&bars.full[i], 1);
-      mbar_init(&bars.empty[i], 2);
+      mbar_init(&bars.empty[i], 1);
     }
-    for (int h = 0; h < 2; ++h)
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(&bars.s_full[h][i], 1);
-        mbar_init(&bars.p_full[h][i], 4);
-        mbar_init(&bars.o_done[h][i], 1);
-      }
-    mbar_init(&bars.q_full, 8);
-    mbar_init(&bars.o_full, 2);
-    mbar_init(&bars.tail_here, 2);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.s_full[i], 1);
+      mbar_init(&bars.p_full[i], 4);
+      mbar_init(&bars.o_done[i], 1);
+    }
+    mbar_init(&bars.q_full, 4);
+    mbar_init(&bars.o_full, 1);
+    mbar_init(&bars.tail_here, 1);
     mbar_init(&bars.tail_ready, 1);
     bars.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -79,26 +79,19 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
   grid_dependency_sync();
   const PagedSequence seq = paged_sequence(p.batch, p.kv.page_shift, b, tid == 0 && blockIdx.x == 0 && chunk_index == 0 ? status : nullptr);
   const unsigned group = static_cast<unsigned>(p.call.heads) / static_cast<unsigned>(p.kv.kv_heads);
-  const int token0 = q_tile * 2 * p.tokens_per_tile;
-  if (token0 >= seq.count)
+  const int token0 = q_tile * p.tokens_per_tile, tokens = min(p.tokens_per_tile, seq.count - token0);
+  if (tokens <= 0)
     return;
-  const int prefix = p.call.prefix ? p.call.prefix[b] : 0, key0 = chunk_index * p.chunk;
-  // keys below these are seen by a tile's first and last token; tiles of keys of each tile of rows
-  int tokens[2], sees_least[2], tiles_of[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int first = token0 + h * p.tokens_per_tile;
-    tokens[h] = max(0, min(p.tokens_per_tile, seq.count - first));
-    sees_least[h] = max(0, min(seq.length, max(seq.length - seq.count + first + 1, prefix)));
-    const int sees_most = max(0, min(seq.length, max(seq.length - seq.count + first + tokens[h], prefix)));
-    tiles_of[h] = tokens[h] > 0 ? max(0, min(sees_most, key0 + p.chunk) - key0 + KT - 1) / KT : 0;
-  }
-  const int tiles = max(tiles_of[0], tiles_of[1]);
+  const int prefix = p.call.prefix ? p.call.prefix[b] : 0;
+  // keys below these are seen by the tile's first and last token
+  const int sees_least = max(0, min(seq.length, max(seq.length - seq.count + token0 + 1, prefix)));
+  const int sees_most = max(0, min(seq.length, max(seq.length - seq.count + token0 + tokens, prefix)));
+  const int key0 = chunk_index * p.chunk, tiles = max(0, min(sees_most, key0 + p.chunk) - key0 + KT - 1) / KT;
   if (tiles == 0 && chunk_index > 0)
     return;
 
   if (warp == kMmaWarp) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem_base)), "r"(512) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem_base)), "r"(256) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
@@ -133,20 +126,15 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
     if (*abort_flag) // copies already requested still write into this CTA's shared memory
       for (int n = max(0, issued - S::slots); n < issued; ++n)
         mbar_wait_quiet<false>(&bars.full[n % S::slots], (n / S::slots) & 1, p.spin_limit);
-  } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
-    // ---- MMA issue: one thread for each tile of rows ----------------------------------------------------------------------------------
+  } else if (warp == kMmaWarp) {
+    // ---- MMA issue: one thread ---------------------------------------------------------------------------------------------------
     if (elect_one()) {
-      const int h = warp - kMmaWarp, mine = h ? tiles_of[1] : tiles_of[0];
       auto wait = [&](uint64_t *bar, int parity) { return mbar_wait<false>(bar, parity, abort_flag, p.spin_limit); };
       const uint64_t k0 = operand_descriptor(smem_u32(ring)), v0 = mn_descriptor(smem_u32(ring), KT * 128); // addresses in descriptors
-      const uint64_t q_descriptor = operand_descriptor(smem_u32(q_sm + h * S::q_bytes));                    // count in units of 16 bytes
-      const uint32_t own = tmem + h * S::columns;
+      const uint64_t q_descriptor = operand_descriptor(smem_u32(q_sm));                                     // count in units of 16 bytes
       int slot = 0, phase = 0;
-      auto next = [&](bool used) { // the ring's item is done with, by this thread
-        if (used)
-          mma_commit(&bars.empty[slot]);
-        else
-          mbar_arrive(&bars.empty[slot]);
+      auto next_slot = [&]() {
+        mma_commit(&bars.empty[slot]);
         if (++slot == S::slots) {
           slot = 0;
           phase ^= 1;
@@ -155,16 +143,14 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
       auto scores = [&](int i) {
         if (!wait(&bars.full[slot], phase))
           return false;
-        if (i < mine) {
-          tc_fence_after();
-          const uint64_t k = k0 + static_cast<uint32_t>(slot) * (S::slot_bytes / 16);
+        tc_fence_after();
+        const uint64_t k = k0 + static_cast<uint32_t>(slot) * (S::slot_bytes / 16);
 #pragma unroll
-          for (int n = 0; n < D / 16; ++n)
-            mma_ss(own + (i & 1) * KT, q_descriptor + ((n / 4) * (kRows * 128) + (n % 4) * 32) / 16, k + ((n / 4) * (KT * 128) + (n % 4) * 32) / 16,
-                   kInstruction<F16, KT, false>, n != 0);
-          mma_commit(&bars.s_full[h][i & 1]);
-        }
-        next(i < mine);
+        for (int n = 0; n < D / 16; ++n)
+          mma_ss(tmem + (i & 1) * KT, q_descriptor + ((n / 4) * (kRows * 128) + (n % 4) * 32) / 16, k + ((n / 4) * (KT * 128) + (n % 4) * 32) / 16,
+                 kInstruction<F16, KT, false>, n != 0);
+        mma_commit(&bars.s_full[i & 1]);
+        next_slot();
         return true;
       };
       bool ok = tiles > 0 && wait(&bars.q_full, 0);
@@ -176,26 +162,21 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
           mbar_arrive(&bars.tail_here);
           ok = wait(&bars.tail_ready, 0);
         }
-        if (ok && i < mine) {
-          ok = wait(&bars.p_full[h][i & 1], (i >> 1) & 1);
-          if (!ok)
-            break;
-          tc_fence_after();
-          const uint64_t v = v0 + static_cast<uint32_t>(slot) * (S::slot_bytes / 16);
+        ok = ok && wait(&bars.p_full[i & 1], (i >> 1) & 1);
+        if (!ok)
+          break;
+        tc_fence_after();
+        const uint64_t v = v0 + static_cast<uint32_t>(slot) * (S::slot_bytes / 16);
 #pragma unroll
-          for (int n = 0; n < KT / 16; ++n)
-            mma_ts(own + 2 * KT, own + (i & 1) * KT + n * 8, v + n * (2048 / 16), kInstruction<F16, D, true>, i != 0 || n != 0);
-          mma_commit(&bars.o_done[h][i & 1]);
-        }
-        if (ok)
-          next(i < mine);
-        if (ok && i + 2 < tiles) // into the buffer that these weights leave: products run in the order of their issue
+        for (int n = 0; n < KT / 16; ++n)
+          mma_ts(tmem + S::o_column, tmem + (i & 1) * KT + n * 8, v + n * (2048 / 16), kInstruction<F16, D, true>, i != 0 || n != 0);
+        mma_commit(&bars.o_done[i & 1]);
+        next_slot();
+        if (i + 2 < tiles) // into the buffer that these weights leave: products run in the order of their issue
           ok = scores(i + 2);
       }
-      if (ok && mine > 0)
+      if (ok)
         mma_commit(&bars.o_full);
-      else
-        mbar_arrive(&bars.o_full);
     }
     __syncwarp();
   } else if (warp == kTailWarp) {
@@ -207,48 +188,41 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
     }
   } else {
     // ---- softmax: a thread per row -----------------------------------------------------------------------------------------------
-    const int h = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
-    const uint32_t own = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + h * S::columns;
-    const unsigned rows = (h ? tokens[1] : tokens[0]) * group;
+    const int row = warp * 32 + lane;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+    const unsigned rows = tokens * group;
     const bool valid = row < static_cast<int>(rows);
-    const int head0 = kvh * static_cast<int>(group), token_tile = token0 + h * p.tokens_per_tile, token_first = seq.first + token_tile;
-    auto together = [&]() { // the four warps of this tile of rows
-      if (h == 0)
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-      else
-        asm volatile("bar.sync 2, 128;" ::: "memory");
-    };
+    const int head0 = kvh * static_cast<int>(group), token_first = seq.first + token0;
     RowScores r;
     r.factor = p.call.scale * (p.call.softcap > 0.0f ? 1.0f : 1.4426950408889634f);
     const bool negative = r.factor < 0.0f; // goes into the queries: the largest product is the largest score
     const bool flat = r.factor == 0.0f;    // every score is 0: so are the queries, and the factor stays usable beside -infinity
     r.factor = flat ? 1.0f : fabsf(r.factor);
-    WholeRows<D, 4> whole(quarter, lane);
+    WholeRows<D, 4> whole(warp, lane);
     whole.load_queries(p.call, flat ? 0 : rows, group, token_first, head0);
-    whole.template stage_queries<F16>(q_sm + h * S::q_bytes, negative, unscales[h]);
+    whole.template stage_queries<F16>(q_sm, negative, unscales);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // visible to the tensor core's reads
     __syncwarp();
     if (lane == 0)
       mbar_arrive(&bars.q_full);
     if constexpr (F16) {
-      together();
-      r.factor *= unscales[h][row];
+      asm volatile("bar.sync 1, 128;" ::: "memory"); // the softmax warps
+      r.factor *= unscales[row];
     }
-    const int position = seq.length - seq.count + token_tile + static_cast<int>(row / group);
+    const int position = seq.length - seq.count + token0 + static_cast<int>(row / group);
     r.cap = p.call.softcap, r.over_cap = r.cap > 0.0f ? 1.0f / r.cap : 0.0f;
     r.biased = p.call.slopes != nullptr;
     r.slope = r.biased && valid ? p.call.slopes[head0 + row % group] * 1.4426950408889634f : 0.0f, r.at = static_cast<float>(position);
-    r.sees = valid ? max(0, min(seq.length, max(position + 1, prefix))) : 0, r.sees_least = h ? sees_least[1] : sees_least[0];
+    r.sees = valid ? max(0, min(seq.length, max(position + 1, prefix))) : 0, r.sees_least = sees_least;
     float reference = -INFINITY, sum = 0.0f;
     bool ok = true;
     auto all_wait = [&](uint64_t *bar, int parity) { return __all_sync(0xffffffffu, mbar_wait<false>(bar, parity, abort_flag, p.spin_limit)); };
-    const int mine = h ? tiles_of[1] : tiles_of[0];
-    for (int i = 0; i < mine; ++i) {
-      ok = all_wait(&bars.s_full[h][i & 1], (i >> 1) & 1);
+    for (int i = 0; i < tiles; ++i) {
+      ok = all_wait(&bars.s_full[i & 1], (i >> 1) & 1);
       if (!ok)
         break;
       tc_fence_after();
-      const uint32_t s_at = own + (i & 1) * KT;
+      const uint32_t s_at = lanes + (i & 1) * KT;
       uint32_t x[KT / 32][32];
       load_scores<KT>(x, s_at);
       const float scaled = shape_scores<KT>(x, r, key0 + i * KT);
@@ -260,35 +234,35 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
         if (i > 0) {
           // O holds every tile up to i - 1 once the product of that one is done.  (A wait by parity tells a phase from its
           // neighbours only: the one before, tile i - 3, is done, or the scores of this one would not be there.)
-          ok = all_wait(&bars.o_done[h][(i - 1) & 1], ((i - 1) >> 1) & 1);
+          ok = all_wait(&bars.o_done[(i - 1) & 1], ((i - 1) >> 1) & 1);
           if (!ok)
             break;
           tc_fence_after();
-          rescale_row<D>(own + 2 * KT, moved);
+          rescale_row<D>(lanes + S::o_column, moved);
         }
         reference = now;
       }
       // a masked score is -infinity, whose weight has to be 0
-      sum += key0 + i * KT + KT > r.sees_least ? store_weights<KT, F16, 0>(x, s_at, scaled, reference) : store_weights<KT, F16, 3>(x, s_at, scaled, reference);
+      sum += key0 + i * KT + KT > r.sees_least ? store_weights<KT, F16, 0>(x, s_at, scaled, reference) : store_weights<KT, F16, 2>(x, s_at, scaled, reference);
       tc_fence_before();
       __syncwarp();
       if (lane == 0)
-        mbar_arrive(&bars.p_full[h][i & 1]);
+        mbar_arrive(&bars.p_full[i & 1]);
     }
     // ---- epilogue -------------------------------------------------------------------------------------------------------------------
     whole.load_gates(p.call, p.call.gate && p.chunks == 1, rows, group, token_first, head0); // on their way while the last products run
     if (ok && tiles > 0)
       ok = all_wait(&bars.o_full, 0);
-    float *rows_out = reinterpret_cast<float *>(q_sm) + h * (kRows * (D + 4)); // queries and ring are done with
+    float *rows_out = reinterpret_cast<float *>(q_sm); // queries and ring are done with
     if (ok) {
       tc_fence_after();
       // f16 values are 1 / 8 of themselves; where a row has seen nothing O may hold anything
       const float scale = (F16 ? 8.0f : 1.0f) * (p.chunks == 1 && sum != 0.0f ? __fdiv_rn(1.0f, sum) : 1.0f);
-      unload_row<D, D>(rows_out + row * (D + 4), own + 2 * KT, 0, scale, sum == 0.0f);
+      unload_row<D, D>(rows_out + row * (D + 4), lanes + S::o_column, 0, scale, sum == 0.0f);
       if (p.chunks > 1 && valid)
         paged_store_sums<D>(p.call, p.batch.tokens, p.chunks, chunk_index, token_first + row / group, head0 + row % group, reference, sum);
     }
-    together();
+    asm volatile("bar.sync 1, 128;" ::: "memory"); // the softmax warps
     if (ok)
       whole.store(p, rows_out, rows, group, token_first, head0, chunk_index);
   }
@@ -297,14 +271,14 @@ paged_pair_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
   __syncthreads();
   if (warp == kMmaWarp) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256) : "memory");
   }
   if (tid == 0 && bars.abort_flag && status)
     atomicOr(status, kStatusWaitRanOut);
 }
 
 template <int D, bool F16> cudaError_t launch(const CUtensorMap &values, const Tile &p, unsigned q_tiles, int *status, cudaStream_t stream) {
-  const auto kernel = paged_pair_kernel<D, F16>;
+  const auto kernel = paged_narrow_kernel<D, F16>;
   if (cudaError_t e = opt_in_shared_memory(reinterpret_cast<const void *>(kernel), Shape<D>::smem); e != cudaSuccess)
     return e;
   return launch_chained(kernel, dim3(p.kv.kv_heads * q_tiles, p.batch.sequences, p.chunks), dim3(kThreads), Shape<D>::smem, stream, values, p, status);
@@ -312,7 +286,7 @@ template <int D, bool F16> cudaError_t launch(const CUtensorMap &values, const T
 
 } // namespace
 
-cudaError_t launch_paged_pair(int head_dim, bool f16, const CUtensorMap &values, const Tile &p, unsigned q_tiles, int *status, cudaStream_t stream) {
+cudaError_t launch_paged_narrow(int head_dim, bool f16, const CUtensorMap &values, const Tile &p, unsigned q_tiles, int *status, cudaStream_t stream) {
   if (head_dim == 64)
     return f16 ? launch<64, true>(values, p, q_tiles, status, stream) : launch<64, false>(values, p, q_tiles, status, stream);
   return f16 ? launch<128, true>(values, p, q_tiles, status, stream) : launch<128, false>(values, p, q_tiles, status, stream);

@@ -160,16 +160,36 @@ __device__ __forceinline__ float2 exp2_by_fma(uint64_t y) {
   return v;
 }
 
-// scale * tanh of two values of at most 1 by an odd polynomial of degree 13 (absolute error 4.4e-8, fitted likewise).
-__device__ __forceinline__ uint64_t tanh_by_fma(uint64_t y, float scale) {
+// scale * tanh of two values by an odd polynomial, fitted likewise: of at most 1 by degree 13 (absolute error 4.4e-8), of at
+// most 1/2 by degree 9 (6.3e-9).
+template <bool HALF> __device__ __forceinline__ uint64_t tanh_by_fma(uint64_t y, float scale) {
   const uint64_t u = mul2(y, y);
-  uint64_t r = fma2(u, pair(0.0010531353245070575f, 0.0010531353245070575f), pair(-0.006239815943848765f, -0.006239815943848765f));
-  r = fma2(r, u, pair(0.020331109759454728f, 0.020331109759454728f));
-  r = fma2(r, u, pair(-0.05347844709285361f, -0.05347844709285361f));
-  r = fma2(r, u, pair(0.1332570887576237f, 0.1332570887576237f));
-  r = fma2(r, u, pair(-0.33332882758746407f, -0.33332882758746407f));
-  r = fma2(r, u, pair(0.9999999563685537f, 0.9999999563685537f));
+  uint64_t r;
+  if constexpr (HALF) {
+    r = fma2(u, pair(0.017151297808556672f, 0.017151297808556672f), pair(-0.05299423135979913f, -0.05299423135979913f));
+    r = fma2(r, u, pair(0.13324906986917054f, 0.13324906986917054f));
+    r = fma2(r, u, pair(-0.333330757952904f, -0.333330757952904f));
+    r = fma2(r, u, pair(0.9999999873746263f, 0.9999999873746263f));
+  } else {
+    r = fma2(u, pair(0.0010531353245070575f, 0.0010531353245070575f), pair(-0.006239815943848765f, -0.006239815943848765f));
+    r = fma2(r, u, pair(0.020331109759454728f, 0.020331109759454728f));
+    r = fma2(r, u, pair(-0.05347844709285361f, -0.05347844709285361f));
+    r = fma2(r, u, pair(0.1332570887576237f, 0.1332570887576237f));
+    r = fma2(r, u, pair(-0.33332882758746407f, -0.33332882758746407f));
+    r = fma2(r, u, pair(0.9999999563685537f, 0.9999999563685537f));
+  }
   return mul2(mul2(y, pair(scale, scale)), r);
+}
+
+template <int KT, bool HALF> __device__ __forceinline__ void cap_scores(uint32_t (&x)[KT / 32][32], float into, float scale) {
+#pragma unroll
+  for (int c = 0; c < KT / 32; ++c)
+#pragma unroll
+    for (int u = 0; u < 32; u += 2) {
+      const float2 v = halves(tanh_by_fma<HALF>(mul2(pair(__uint_as_float(x[c][u]), __uint_as_float(x[c][u + 1])), pair(into, into)), scale));
+      x[c][u] = __float_as_uint(v.x);
+      x[c][u + 1] = __float_as_uint(v.y);
+    }
 }
 
 // Products to scores (up to the returned factor), capped, biased and masked.
@@ -182,32 +202,28 @@ template <int KT> __device__ __forceinline__ float shape_scores(uint32_t (&x)[KT
 #pragma unroll
       for (int u = 0; u < 32; u += 2)
         most[u >> 1 & 3] = max3(most[u >> 1 & 3], fabsf(__uint_as_float(x[c][u])), fabsf(__uint_as_float(x[c][u + 1])));
+    const float into = r.factor * r.over_cap, far = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * into, scale = r.cap * 1.4426950408889634f;
     // the hardware's exp and reciprocal are few; scores within the cap, which is the rule, do without
-    if (__any_sync(0xffffffffu, !(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * (r.factor * r.over_cap) <= 1.0f))) {
+    if (!__any_sync(0xffffffffu, !(far <= 0.5f))) {
+      cap_scores<KT, true>(x, into, scale);
+    } else if (!__any_sync(0xffffffffu, !(far <= 1.0f))) {
+      cap_scores<KT, false>(x, into, scale);
+    } else {
 #pragma unroll
       for (int c = 0; c < KT / 32; ++c)
 #pragma unroll
         for (int u = 0; u < 32; ++u)
           x[c][u] = __float_as_uint(capped_log2(__uint_as_float(x[c][u]) * r.factor, r.cap, r.over_cap));
-    } else {
-      const uint64_t into = pair(r.factor * r.over_cap, r.factor * r.over_cap);
-#pragma unroll
-      for (int c = 0; c < KT / 32; ++c)
-#pragma unroll
-        for (int u = 0; u < 32; u += 2) {
-          const float2 v = halves(tanh_by_fma(mul2(pair(__uint_as_float(x[c][u]), __uint_as_float(x[c][u + 1])), into), r.cap * 1.4426950408889634f));
-          x[c][u] = __float_as_uint(v.x);
-          x[c][u + 1] = __float_as_uint(v.y);
-        }
     }
     scaled = 1.0f;
   }
   if (r.biased) {
+    const float from = r.at - static_cast<float>(j0); // whole numbers: exact to 2^24
 #pragma unroll
     for (int c = 0; c < KT / 32; ++c)
 #pragma unroll
       for (int u = 0; u < 32; ++u)
-        x[c][u] = __float_as_uint(__uint_as_float(x[c][u]) * scaled - r.slope * fabsf(r.at - static_cast<float>(j0 + c * 32 + u)));
+        x[c][u] = __float_as_uint(__fmaf_rn(-r.slope, fabsf(from - static_cast<float>(c * 32 + u)), __uint_as_float(x[c][u]) * scaled));
     scaled = 1.0f;
   }
   if (j0 + KT > r.sees_least) {
@@ -398,6 +414,6 @@ template <int KT, int SLABS> __device__ __forceinline__ void zero_tail(uint8_t *
 
 } // namespace tc
 
-cudaError_t launch_paged_pair(int head_dim, bool f16, const CUtensorMap &values, const tc::Tile &p, unsigned q_tiles, int *status, cudaStream_t stream);
+cudaError_t launch_paged_narrow(int head_dim, bool f16, const CUtensorMap &values, const tc::Tile &p, unsigned q_tiles, int *status, cudaStream_t stream);
 
 } // namespace llmcp_b200

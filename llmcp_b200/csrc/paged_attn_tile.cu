@@ -1,5 +1,5 @@
 // Attention over the paged cache for many rows (prompts), 256 dimensions: both products on tcgen05.  (64 and 128 dimensions:
-// paged_attn_pair.cu, launched from here.)
+// paged_attn_narrow.cu, launched from here.)
 //
 //   S = Q K^T,  P = 2^(S scale log2 e - m),  O = sum P V / sum P,   128 rows (tokens x the query heads of one key head) a CTA
 //
@@ -391,9 +391,6 @@ template <bool F16> cudaError_t launch_wide(const CUtensorMap &values, const Til
   return launch_chained(kernel, dim3(p.kv.kv_heads * q_tiles, p.batch.sequences, p.chunks), dim3(kThreads), kSmem, stream, values, p, status);
 }
 
-// Tokens of a CTA: 128 rows with 256 dimensions, twice that else.
-int tokens_per_cta(const PagedKv &kv, int heads) { return kRows / (heads / kv.kv_heads) * (kv.head_dim == D ? 1 : 2); }
-
 } // namespace
 
 size_t paged_tile_workspace(const PagedKv &kv, const PagedBatch &batch, int heads, const PagedSplit &split) {
@@ -401,7 +398,7 @@ size_t paged_tile_workspace(const PagedKv &kv, const PagedBatch &batch, int head
 }
 
 PagedSplit paged_tile_split(const PagedKv &kv, const PagedBatch &batch, int heads, int sms) {
-  const int per_cta = tokens_per_cta(kv, heads);
+  const int per_cta = kRows / (heads / kv.kv_heads);
   const int64_t ctas = static_cast<int64_t>((batch.max_q + per_cta - 1) / per_cta) * kv.kv_heads * batch.sequences;
   const int64_t tiles = (batch.max_kv + KT - 1) / KT;
   // pieces of at least eight tiles, as many as fill the SMs once
@@ -443,10 +440,9 @@ cudaError_t launch_paged_tile(const PagedKv &kv, const PagedBatch &batch, const 
   CUtensorMap values;
   if (!paged_value_map(&values, source, rows, p.box_rows))
     return cudaErrorNotSupported;
-  const int per_cta = tokens_per_cta(kv, call.heads);
-  const unsigned q_tiles = static_cast<unsigned>((batch.max_q + per_cta - 1) / per_cta);
+  const unsigned q_tiles = static_cast<unsigned>((batch.max_q + p.tokens_per_tile - 1) / p.tokens_per_tile);
   if (kv.head_dim != D)
-    return launch_paged_pair(kv.head_dim, f16, values, p, q_tiles, status, stream);
+    return launch_paged_narrow(kv.head_dim, f16, values, p, q_tiles, status, stream);
   return f16 ? launch_wide<true>(values, p, q_tiles, status, stream) : launch_wide<false>(values, p, q_tiles, status, stream);
 }
 
