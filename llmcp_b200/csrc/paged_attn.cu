@@ -84,8 +84,8 @@ paged_merge_kernel(PagedKv kv, PagedBatch batch, PagedAttention call, PagedSplit
     for (int w = 0; w < 8; ++w)
       total += totals[w];
     const float inv = total == 0.0f ? 0.0f : __fdiv_rn(1.0f, total);
-    paged_store_row<D>(call, token, head, d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv), make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv),
-                       call.gate ? paged_gate<D>(call, token, head, d) : make_uint4(0, 0, 0, 0));
+    paged_store_row(call.out + paged_out_at<D>(call, token, head, d), make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv),
+                    make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv), paged_gate(call, token, head, d), call.gate != nullptr);
   }
 }
 

@@ -77,27 +77,30 @@ __device__ __forceinline__ float capped_log2(float x, float cap, float over_cap)
   return cap * kLog2e * __fmaf_rn(-2.0f, r, 1.0f);
 }
 
-// The gate of eight dimensions.
-template <int D> __device__ __forceinline__ uint4 paged_gate(const PagedAttention &call, int token, int head, int d) {
-  return *reinterpret_cast<const uint4 *>(call.gate + token * call.gate_row + head * call.gate_head + d);
-}
-
 // Eight dimensions of a finished row: times their gate, where there is one, as bf16.
-template <int D> __device__ __forceinline__ void paged_store_row(const PagedAttention &call, int token, int head, int d, float4 x, float4 y, uint4 gate8) {
+__device__ __forceinline__ void paged_store_row(uint16_t *to, float4 x, float4 y, uint4 gate8, bool gated) {
   float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-  if (call.gate) {
+  if (gated) {
     const uint32_t w[4] = {gate8.x, gate8.y, gate8.z, gate8.w};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float gate = __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
-      v[i] = __fdividef(v[i], 1.0f + __expf(-fmaxf(gate, -80.0f))); // below -80 the product is 0 beside any other value of a row
+      // below -80 the product is 0 beside any other value of a row
+      v[i] = __fdividef(v[i], 1.0f + exp2_approx(fminf(gate * -1.4426950408889634f, 115.0f)));
     }
   }
   uint32_t words[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(words[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
-  *reinterpret_cast<uint4 *>(call.out + (static_cast<int64_t>(token) * call.heads + head) * D + d) = make_uint4(words[0], words[1], words[2], words[3]);
+  *reinterpret_cast<uint4 *>(to) = make_uint4(words[0], words[1], words[2], words[3]);
+}
+// Where a row's eight dimensions from d lie in out, and its gate.
+template <int D> __device__ __forceinline__ int64_t paged_out_at(const PagedAttention &call, int token, int head, int d) {
+  return (static_cast<int64_t>(token) * call.heads + head) * D + d;
+}
+__device__ __forceinline__ uint4 paged_gate(const PagedAttention &call, int token, int head, int d) {
+  return call.gate ? *reinterpret_cast<const uint4 *>(call.gate + token * call.gate_row + head * call.gate_head + d) : make_uint4(0, 0, 0, 0);
 }
 
 __device__ __forceinline__ float2 *paged_part_sums(const PagedAttention &call, int tokens, int chunks, int head_dim) {
@@ -105,11 +108,9 @@ __device__ __forceinline__ float2 *paged_part_sums(const PagedAttention &call, i
 }
 
 // A chunk's part of a row: eight dimensions of its sum, and (once) its reference and the sum of its weights.
-template <int D>
-__device__ __forceinline__ void paged_store_part(const PagedAttention &call, int chunks, int chunk, int token, int head, int d, float4 x, float4 y) {
-  float4 *to = reinterpret_cast<float4 *>(static_cast<float *>(call.workspace) + ((static_cast<int64_t>(token) * call.heads + head) * chunks + chunk) * D + d);
-  to[0] = x;
-  to[1] = y;
+__device__ __forceinline__ void paged_store_part(float *to, float4 x, float4 y) {
+  reinterpret_cast<float4 *>(to)[0] = x;
+  reinterpret_cast<float4 *>(to)[1] = y;
 }
 template <int D>
 __device__ __forceinline__ void paged_store_sums(const PagedAttention &call, int tokens, int chunks, int chunk, int token, int head, float top, float total) {

@@ -78,7 +78,7 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap map_values, const __grid
   }
   grid_dependency_sync();
   const PagedSequence seq = paged_sequence(p.batch, p.kv.page_shift, b, tid == 0 && blockIdx.x == 0 && chunk_index == 0 ? status : nullptr);
-  const unsigned group = static_cast<unsigned>(p.call.heads) / static_cast<unsigned>(p.kv.kv_heads);
+  const unsigned group = p.group;
   const int token0 = q_tile * p.tokens_per_tile, tokens = min(p.tokens_per_tile, seq.count - token0);
   if (tokens <= 0)
     return;
@@ -141,8 +141,6 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap map_values, const __grid
         }
       };
       auto scores = [&](int i) {
-        if (!wait(&bars.full[slot], phase))
-          return false;
         tc_fence_after();
         const uint64_t k = k0 + static_cast<uint32_t>(slot) * (S::slot_bytes / 16);
 #pragma unroll
@@ -151,18 +149,19 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap map_values, const __grid
                  kInstruction<F16, KT, false>, n != 0);
         mma_commit(&bars.s_full[i & 1]);
         next_slot();
-        return true;
       };
       bool ok = tiles > 0 && wait(&bars.q_full, 0);
-      for (int i = 0; i < min(2, tiles) && ok; ++i)
-        ok = scores(i);
-      for (int i = 0; i < tiles && ok; ++i) {
+      for (int i = 0; i < min(2, tiles) && ok; ++i) {
         ok = wait(&bars.full[slot], phase);
+        if (ok)
+          scores(i);
+      }
+      for (int i = 0; i < tiles && ok; ++i) {
+        ok = wait_for_both(&bars.full[slot], phase, &bars.p_full[i & 1], (i >> 1) & 1, abort_flag, p.spin_limit);
         if (ok && i == tiles - 1 && seq.length - key0 - i * KT < KT) { // rows past the sequence: whatever they hold
           mbar_arrive(&bars.tail_here);
           ok = wait(&bars.tail_ready, 0);
         }
-        ok = ok && wait(&bars.p_full[i & 1], (i >> 1) & 1);
         if (!ok)
           break;
         tc_fence_after();
@@ -172,8 +171,11 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap map_values, const __grid
           mma_ts(tmem + S::o_column, tmem + (i & 1) * KT + n * 8, v + n * (2048 / 16), kInstruction<F16, D, true>, i != 0 || n != 0);
         mma_commit(&bars.o_done[i & 1]);
         next_slot();
-        if (i + 2 < tiles) // into the buffer that these weights leave: products run in the order of their issue
-          ok = scores(i + 2);
+        if (i + 2 < tiles) { // into the buffer that these weights leave: products run in the order of their issue
+          ok = wait(&bars.full[slot], phase);
+          if (ok)
+            scores(i + 2);
+        }
       }
       if (ok)
         mma_commit(&bars.o_full);
@@ -198,8 +200,8 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap map_values, const __grid
     const bool negative = r.factor < 0.0f; // goes into the queries: the largest product is the largest score
     const bool flat = r.factor == 0.0f;    // every score is 0: so are the queries, and the factor stays usable beside -infinity
     r.factor = flat ? 1.0f : fabsf(r.factor);
-    WholeRows<D, 4> whole(warp, lane);
-    whole.load_queries(p.call, flat ? 0 : rows, group, token_first, head0);
+    WholeRows<D, 4> whole(p, warp, lane, rows, token_first, head0);
+    whole.load(p.call.q, p.call.q_row, p.call.q_head, !flat);
     whole.template stage_queries<F16>(q_sm, negative, unscales);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // visible to the tensor core's reads
     __syncwarp();
@@ -250,7 +252,7 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap map_values, const __grid
         mbar_arrive(&bars.p_full[i & 1]);
     }
     // ---- epilogue -------------------------------------------------------------------------------------------------------------------
-    whole.load_gates(p.call, p.call.gate && p.chunks == 1, rows, group, token_first, head0); // on their way while the last products run
+    whole.load(p.call.gate, p.call.gate_row, p.call.gate_head, p.call.gate && p.chunks == 1); // on their way while the last products run
     if (ok && tiles > 0)
       ok = all_wait(&bars.o_full, 0);
     float *rows_out = reinterpret_cast<float *>(q_sm); // queries and ring are done with
@@ -264,7 +266,7 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap map_values, const __grid
     }
     asm volatile("bar.sync 1, 128;" ::: "memory"); // the softmax warps
     if (ok)
-      whole.store(p, rows_out, rows, group, token_first, head0, chunk_index);
+      whole.store(p, rows_out, chunk_index);
   }
 
   tc_fence_before();

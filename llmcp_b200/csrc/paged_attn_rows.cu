@@ -663,10 +663,11 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         v[i] *= inv;
-      paged_store_row<D>(p.call, token, head, d, make_float4(v[0], v[1], v[2], v[3]), make_float4(v[4], v[5], v[6], v[7]),
-                         p.call.gate ? paged_gate<D>(p.call, token, head, d) : make_uint4(0, 0, 0, 0));
+      paged_store_row(p.call.out + paged_out_at<D>(p.call, token, head, d), make_float4(v[0], v[1], v[2], v[3]), make_float4(v[4], v[5], v[6], v[7]),
+                      paged_gate(p.call, token, head, d), p.call.gate != nullptr);
     } else {
-      paged_store_part<D>(p.call, p.chunks, chunk_index, token, head, d, make_float4(v[0], v[1], v[2], v[3]), make_float4(v[4], v[5], v[6], v[7]));
+      paged_store_part(static_cast<float *>(p.call.workspace) + paged_out_at<D>(p.call, token, head, 0) * p.chunks + chunk_index * D + d,
+                       make_float4(v[0], v[1], v[2], v[3]), make_float4(v[4], v[5], v[6], v[7]));
       if (d == 0)
         paged_store_sums<D>(p.call, p.batch.tokens, p.chunks, chunk_index, token, head, all, total);
     }

@@ -27,6 +27,7 @@ struct Tile {
   PagedAttention call;
   int chunk, chunks, box_rows;
   int tokens_per_tile;   // of 128 rows
+  unsigned group, one_over_group; // query heads that share a key head; 2^16 / group rounded up
   int64_t expanded_rows; // rows of a sequence's keys in the expanded cache; 0: pages
   int out_of_range;      // a row coordinate past the last row: reads as zeros
   uint32_t spin_limit;
@@ -122,6 +123,20 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
+
+// Two barriers awaited together: a look at one takes some 150 cycles, and looks at both overlap.
+__device__ __forceinline__ bool wait_for_both(uint64_t *a, uint32_t pa, uint64_t *b, uint32_t pb, volatile int *abort_flag, uint32_t limit) {
+  const uint32_t aa = smem_u32(a), ab = smem_u32(b);
+  for (uint32_t spin = 0; spin < limit; ++spin) {
+    const bool ra = mbar_poll<false>(aa, pa), rb = mbar_poll<false>(ab, pb);
+    if (ra && rb)
+      return true;
+    if ((spin & 63) == 63 && *abort_flag)
+      return false;
+  }
+  *abort_flag = 1;
+  return false;
+}
 
 // The scores of a row in a tile, from tensor memory.
 template <int KT> __device__ __forceinline__ void load_scores(uint32_t (&x)[KT / 32][32], uint32_t address) {
@@ -301,16 +316,25 @@ template <int D, int WARPS> struct WholeRows {
   static constexpr int kLanes = D / 8, kSide = 32 / kLanes, kStep = WARPS * kSide, kMine = kRows / kStep;
   uint4 pieces[kMine];
   int piece, first; // 16-byte piece of a row, first row
+  unsigned rows, group, one_over_group;
+  int token0, head0;
 
-  __device__ __forceinline__ WholeRows(int warp, int lane) : piece(lane % kLanes), first(warp * kSide + lane / kLanes) {}
+  __device__ __forceinline__ WholeRows(const Tile &p, int warp, int lane, unsigned rows, int token0, int head0)
+      : piece(lane % kLanes), first(warp * kSide + lane / kLanes), rows(rows), group(p.group), one_over_group(p.one_over_group), token0(token0), head0(head0) {}
 
-  __device__ __forceinline__ void load_queries(const PagedAttention &call, unsigned rows, unsigned group, int token0, int head0) {
+  // Row r is token r / group, head r % group.  (r below 128 and group at most 128: the product is exact enough.)
+  __device__ __forceinline__ int64_t at(unsigned r, int64_t token_stride, int64_t head_stride) const {
+    const unsigned token = r * one_over_group >> 16;
+    return static_cast<int64_t>(token0 + token) * token_stride + static_cast<int64_t>(head0 + (r - token * group)) * head_stride + piece * 8;
+  }
+
+  __device__ __forceinline__ void load(const uint16_t *from, int64_t token_stride, int64_t head_stride, bool wanted) {
 #pragma unroll
     for (int n = 0; n < kMine; ++n) {
       const unsigned r = first + n * kStep;
       pieces[n] = make_uint4(0, 0, 0, 0);
-      if (r < rows)
-        pieces[n] = *reinterpret_cast<const uint4 *>(call.q + (token0 + r / group) * call.q_row + (head0 + r % group) * call.q_head + piece * 8);
+      if (wanted && r < rows)
+        pieces[n] = *reinterpret_cast<const uint4 *>(from + at(r, token_stride, head_stride));
     }
   }
 
@@ -346,29 +370,19 @@ template <int D, int WARPS> struct WholeRows {
     }
   }
 
-  __device__ __forceinline__ void load_gates(const PagedAttention &call, bool wanted, unsigned rows, unsigned group, int token0, int head0) {
-#pragma unroll
-    for (int n = 0; n < kMine; ++n) {
-      const unsigned r = first + n * kStep;
-      pieces[n] = make_uint4(0, 0, 0, 0);
-      if (wanted && r < rows)
-        pieces[n] = paged_gate<D>(call, token0 + r / group, head0 + r % group, piece * 8);
-    }
-  }
-
-  // From f32 rows D + 4 apart.
-  __device__ __forceinline__ void store(const Tile &p, const float *from, unsigned rows, unsigned group, int token0, int head0, int chunk) {
+  // From f32 rows D + 4 apart; `pieces` are the gates.
+  __device__ __forceinline__ void store(const Tile &p, const float *from, int chunk) const {
 #pragma unroll
     for (int n = 0; n < kMine; ++n) {
       const unsigned r = first + n * kStep;
       if (r >= rows)
         break;
-      const int d = piece * 8, token = token0 + r / group, head = head0 + r % group;
-      const float4 x = *reinterpret_cast<const float4 *>(from + r * (D + 4) + d), y = *reinterpret_cast<const float4 *>(from + r * (D + 4) + d + 4);
+      const float4 *v = reinterpret_cast<const float4 *>(from + r * (D + 4) + piece * 8);
+      const int64_t to = at(r, static_cast<int64_t>(p.call.heads) * D, D);
       if (p.chunks == 1)
-        paged_store_row<D>(p.call, token, head, d, x, y, pieces[n]);
+        paged_store_row(p.call.out + to, v[0], v[1], pieces[n], p.call.gate != nullptr);
       else
-        paged_store_part<D>(p.call, p.chunks, chunk, token, head, d, x, y);
+        paged_store_part(static_cast<float *>(p.call.workspace) + (to - piece * 8) * p.chunks + chunk * D + piece * 8, v[0], v[1]);
     }
   }
 };

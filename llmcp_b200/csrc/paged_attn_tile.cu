@@ -85,7 +85,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
   }
   grid_dependency_sync();
   const PagedSequence seq = paged_sequence(p.batch, p.kv.page_shift, b, tid == 0 && blockIdx.x == 0 && chunk_index == 0 ? status : nullptr);
-  const unsigned group = static_cast<unsigned>(p.call.heads) / static_cast<unsigned>(p.kv.kv_heads);
+  const unsigned group = p.group;
   const int token0 = q_tile * p.tokens_per_tile, tokens = min(p.tokens_per_tile, seq.count - token0);
   if (tokens <= 0)
     return;
@@ -149,8 +149,6 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
         }
       };
       auto scores = [&]() {
-        if (!wait(&bars.full[slot], phase))
-          return false;
         tc_fence_after();
         const uint64_t k = operand_descriptor(ring_address + slot * kSlotBytes); // addresses count in units of 16 bytes
 #pragma unroll
@@ -160,20 +158,19 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
         mma_commit(&bars.empty[slot]);
         next_slot();
         ++scored;
-        return true;
       };
       bool ok = tiles > 0 && wait(&bars.q_full, 0);
       while (ok && scored < min(2, tiles)) {
-        tc_fence_after();
-        ok = scores();
+        ok = wait(&bars.full[slot], phase);
+        if (ok)
+          scores();
       }
       for (int i = 0; i < tiles && ok; ++i) {
-        ok = wait(&bars.full[slot], phase);
+        ok = wait_for_both(&bars.full[slot], phase, &bars.p_full[i & 1], (i >> 1) & 1, abort_flag, p.spin_limit);
         if (ok && i == tiles - 1 && seq.length - key0 - i * KT < KT) { // rows past the sequence: whatever they hold
           mbar_arrive(&bars.tail_here);
           ok = wait(&bars.tail_ready, 0);
         }
-        ok = ok && wait(&bars.p_full[i & 1], (i >> 1) & 1);
         if (!ok)
           break;
         tc_fence_after();
@@ -184,8 +181,11 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
         mma_commit(&bars.o_done[i & 1]);
         mma_commit(&bars.empty[slot]);
         next_slot();
-        if (scored < tiles) // into the buffer that this tile's weights leave: products run in the order of their issue
-          ok = scores();
+        if (scored < tiles) { // into the buffer that this tile's weights leave: products run in the order of their issue
+          ok = wait(&bars.full[slot], phase);
+          if (ok)
+            scores();
+        }
       }
       if (ok)
         mma_commit(&bars.o_full);
@@ -209,8 +209,8 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
     const bool negative = factor < 0.0f; // goes into the queries: the largest product is the largest score
     const bool flat = factor == 0.0f;    // every score is 0: so are the queries, and the factor stays usable beside -infinity
     factor = flat ? 1.0f : fabsf(factor);
-    WholeRows<D, kSoftmaxWarps> whole(warp, lane);
-    whole.load_queries(p.call, flat ? 0 : rows, group, token_first, head0);
+    WholeRows<D, kSoftmaxWarps> whole(p, warp, lane, rows, token_first, head0);
+    whole.load(p.call.q, p.call.q_row, p.call.q_head, !flat);
     uint8_t *staged = ring + kQSlot * kSlotBytes; // the loader leaves these slots until the queries have gone on
     whole.stage_queries<F16>(staged, negative, references);
     asm volatile("bar.sync 1, 256;" ::: "memory"); // the softmax warps
@@ -291,7 +291,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
     last_reference[half][row] = reference;
     sums[half][row] = sum;
     asm volatile("bar.sync 1, 256;" ::: "memory");
-    whole.load_gates(p.call, p.call.gate && p.chunks == 1, rows, group, token_first, head0); // on their way while the last products run
+    whole.load(p.call.gate, p.call.gate_row, p.call.gate_head, p.call.gate && p.chunks == 1); // on their way while the last products run
     if (ok && tiles > 0)
       ok = all_wait(&bars.o_full, 0);
     float *rows_out = reinterpret_cast<float *>(ring); // the ring is done with
@@ -310,7 +310,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
     }
     asm volatile("bar.sync 1, 256;" ::: "memory");
     if (ok)
-      whole.store(p, rows_out, rows, group, token_first, head0, chunk_index);
+      whole.store(p, rows_out, chunk_index);
   }
 
   tc_fence_before();
@@ -417,7 +417,8 @@ cudaError_t launch_paged_tile(const PagedKv &kv, const PagedBatch &batch, const 
   Tile p;
   p.kv = kv, p.batch = batch, p.call = call;
   p.chunk = split.chunk, p.chunks = split.chunks;
-  p.tokens_per_tile = kRows / (call.heads / kv.kv_heads);
+  p.group = call.heads / kv.kv_heads, p.one_over_group = (65536 + p.group - 1) / p.group;
+  p.tokens_per_tile = kRows / p.group;
   p.spin_limit = kSpinLimit<false>;
   p.expanded_rows = 0;
   p.box_rows = KT < 1 << kv.page_shift ? KT : 1 << kv.page_shift;
