@@ -77,17 +77,19 @@ __device__ __forceinline__ float capped_log2(float x, float cap, float over_cap)
   return cap * kLog2e * __fmaf_rn(-2.0f, r, 1.0f);
 }
 
+// x sigmoid(gate); below -80 the product is 0 beside any other value of a row.
+__device__ __forceinline__ float times_sigmoid(float x, float gate) {
+  return __fdividef(x, 1.0f + exp2_approx(fminf(gate * -1.4426950408889634f, 115.0f)));
+}
+
 // Eight dimensions of a finished row: times their gate, where there is one, as bf16.
 __device__ __forceinline__ void paged_store_row(uint16_t *to, float4 x, float4 y, uint4 gate8, bool gated) {
   float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
   if (gated) {
     const uint32_t w[4] = {gate8.x, gate8.y, gate8.z, gate8.w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float gate = __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
-      // below -80 the product is 0 beside any other value of a row
-      v[i] = __fdividef(v[i], 1.0f + exp2_approx(fminf(gate * -1.4426950408889634f, 115.0f)));
-    }
+    for (int i = 0; i < 8; ++i)
+      v[i] = times_sigmoid(v[i], __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16));
   }
   uint32_t words[4];
 #pragma unroll

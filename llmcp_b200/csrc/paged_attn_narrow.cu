@@ -28,9 +28,7 @@ template <int D> struct Shape {
   static constexpr int slots = D == 128 ? 4 : 8; // 64 KB
   static constexpr int o_column = 2 * KT;        // tensor memory: two score buffers, O
   static_assert(o_column + D <= 256, "tensor memory of one of two CTAs");
-  // results leave as f32 rows over the queries and the ring
-  static constexpr size_t buffers = q_bytes + slots * slot_bytes, results = kRows * (D + 4) * sizeof(float);
-  static constexpr size_t smem = 1024 + (buffers > results ? buffers : results);
+  static constexpr size_t smem = 1024 + q_bytes + slots * slot_bytes;
 };
 
 template <int SLOTS> struct Barriers {
@@ -51,7 +49,6 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap map_values, const __grid
   using S = Shape<D>;
   extern __shared__ uint8_t raw_smem[];
   __shared__ Barriers<S::slots> bars;
-  __shared__ float unscales[kRows];
   uint8_t *q_sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
   uint8_t *ring = q_sm + S::q_bytes;
   volatile int *abort_flag = &bars.abort_flag;
@@ -200,17 +197,27 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap map_values, const __grid
     const bool negative = r.factor < 0.0f; // goes into the queries: the largest product is the largest score
     const bool flat = r.factor == 0.0f;    // every score is 0: so are the queries, and the factor stays usable beside -infinity
     r.factor = flat ? 1.0f : fabsf(r.factor);
-    WholeRows<D, 4> whole(p, warp, lane, rows, token_first, head0);
-    whole.load(p.call.q, p.call.q_row, p.call.q_head, !flat);
-    whole.template stage_queries<F16>(q_sm, negative, unscales);
+    const TileRows whole{flat ? 0 : rows, group, p.one_over_group, token_first, head0};
+    copy_rows_in<D, 4>(smem_u32(q_sm), p.call.q, p.call.q_row, p.call.q_head, whole, warp, lane);
+    copies_done();
+    if (F16 || negative) { // in place, a row per thread
+      asm volatile("bar.sync 1, 128;" ::: "memory"); // the softmax warps
+      float multiplier = 1.0f, unscale = 1.0f;
+      if constexpr (F16)
+        multiplier = query_multiplier<D>(q_sm, row, negative, &unscale);
+      r.factor *= unscale;
+#pragma unroll 2
+      for (int piece = 0; piece < D / 8; ++piece) {
+        uint4 *at = reinterpret_cast<uint4 *>(q_sm + piece_at(row, piece));
+        const uint4 v = *at;
+        *at = make_uint4(query_pair<F16>(v.x, multiplier, negative), query_pair<F16>(v.y, multiplier, negative),
+                         query_pair<F16>(v.z, multiplier, negative), query_pair<F16>(v.w, multiplier, negative));
+      }
+    }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // visible to the tensor core's reads
     __syncwarp();
     if (lane == 0)
       mbar_arrive(&bars.q_full);
-    if constexpr (F16) {
-      asm volatile("bar.sync 1, 128;" ::: "memory"); // the softmax warps
-      r.factor *= unscales[row];
-    }
     const int position = seq.length - seq.count + token0 + static_cast<int>(row / group);
     r.cap = p.call.softcap, r.over_cap = r.cap > 0.0f ? 1.0f / r.cap : 0.0f;
     r.biased = p.call.slopes != nullptr;
@@ -252,21 +259,33 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap map_values, const __grid
         mbar_arrive(&bars.p_full[i & 1]);
     }
     // ---- epilogue -------------------------------------------------------------------------------------------------------------------
-    whole.load(p.call.gate, p.call.gate_row, p.call.gate_head, p.call.gate && p.chunks == 1); // on their way while the last products run
+    // Gates, then results, lie in the queries' place: the last scores that this warp has seen were their last product.  (All
+    // four warps have to have seen them.)
+    const TileRows mine{rows, group, p.one_over_group, token_first, head0};
+    const bool gated = p.call.gate && p.chunks == 1;
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    if (ok && gated)
+      copy_rows_in<D, 4>(smem_u32(q_sm), p.call.gate, p.call.gate_row, p.call.gate_head, mine, warp, lane);
     if (ok && tiles > 0)
       ok = all_wait(&bars.o_full, 0);
-    float *rows_out = reinterpret_cast<float *>(q_sm); // queries and ring are done with
+    copies_done();
+    asm volatile("bar.sync 1, 128;" ::: "memory");
     if (ok) {
       tc_fence_after();
       // f16 values are 1 / 8 of themselves; where a row has seen nothing O may hold anything
       const float scale = (F16 ? 8.0f : 1.0f) * (p.chunks == 1 && sum != 0.0f ? __fdiv_rn(1.0f, sum) : 1.0f);
-      unload_row<D, D>(rows_out + row * (D + 4), lanes + S::o_column, 0, scale, sum == 0.0f);
-      if (p.chunks > 1 && valid)
-        paged_store_sums<D>(p.call, p.batch.tokens, p.chunks, chunk_index, token_first + row / group, head0 + row % group, reference, sum);
+      if (p.chunks == 1) {
+        unload_row<D>(q_sm, row, lanes + S::o_column, scale, sum == 0.0f, gated);
+      } else {
+        const int64_t part = (mine.at(row, p.call.heads, 1) * p.chunks + chunk_index) * D;
+        unload_part<D>(static_cast<float *>(p.call.workspace) + (valid ? part : 0), lanes + S::o_column, scale, sum == 0.0f, valid);
+        if (valid)
+          paged_store_sums<D>(p.call, p.batch.tokens, p.chunks, chunk_index, token_first + row / group, head0 + row % group, reference, sum);
+      }
     }
-    asm volatile("bar.sync 1, 128;" ::: "memory"); // the softmax warps
-    if (ok)
-      whole.store(p, rows_out, chunk_index);
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    if (ok && p.chunks == 1)
+      copy_rows_out<D, 4>(p.call.out, static_cast<int64_t>(p.call.heads) * D, D, q_sm, mine, warp, lane);
   }
 
   tc_fence_before();

@@ -311,95 +311,110 @@ template <int D> __device__ __forceinline__ void rescale_row(uint32_t address, f
   tmem_wait_stores();
 }
 
-// 128 rows, read and written whole by WARPS warps: a lane takes 16 bytes of a row, and all its rows at once.
-template <int D, int WARPS> struct WholeRows {
-  static constexpr int kLanes = D / 8, kSide = 32 / kLanes, kStep = WARPS * kSide, kMine = kRows / kStep;
-  uint4 pieces[kMine];
-  int piece, first; // 16-byte piece of a row, first row
+// Rows of queries, gates and results lie in shared memory as K-major slabs of 64 dimensions, 128 rows of 128 bytes each,
+// 16-byte pieces where the 128-byte swizzle has them.  Everything below is done once per CTA and written as short loops:
+// unrolled, its instructions take longer to fetch than to execute.
+__device__ __forceinline__ uint32_t piece_at(int row, int piece) { return (piece / 8) * (kRows * 128) + row * 128 + ((piece % 8 ^ row & 7) << 4); }
+
+// Which rows of global memory those are: row r is token r / group, head r % group.  (r below 128 and group at most 128: the
+// product with the reciprocal is exact enough.)
+struct TileRows {
   unsigned rows, group, one_over_group;
   int token0, head0;
-
-  __device__ __forceinline__ WholeRows(const Tile &p, int warp, int lane, unsigned rows, int token0, int head0)
-      : piece(lane % kLanes), first(warp * kSide + lane / kLanes), rows(rows), group(p.group), one_over_group(p.one_over_group), token0(token0), head0(head0) {}
-
-  // Row r is token r / group, head r % group.  (r below 128 and group at most 128: the product is exact enough.)
   __device__ __forceinline__ int64_t at(unsigned r, int64_t token_stride, int64_t head_stride) const {
     const unsigned token = r * one_over_group >> 16;
-    return static_cast<int64_t>(token0 + token) * token_stride + static_cast<int64_t>(head0 + (r - token * group)) * head_stride + piece * 8;
-  }
-
-  __device__ __forceinline__ void load(const uint16_t *from, int64_t token_stride, int64_t head_stride, bool wanted) {
-#pragma unroll
-    for (int n = 0; n < kMine; ++n) {
-      const unsigned r = first + n * kStep;
-      pieces[n] = make_uint4(0, 0, 0, 0);
-      if (wanted && r < rows)
-        pieces[n] = *reinterpret_cast<const uint4 *>(from + at(r, token_stride, head_stride));
-    }
-  }
-
-  // Into K-major slabs of 64 dimensions with the 128-byte swizzle.  f16: a power of two per row takes the largest |q| into
-  // [2^14, 2^15), and `unscale` gets what takes it back (and the keys' 8).
-  template <bool F16> __device__ __forceinline__ void stage_queries(uint8_t *to, bool negative, float *unscale) {
-#pragma unroll
-    for (int n = 0; n < kMine; ++n) {
-      const int r = first + n * kStep;
-      uint32_t w[4] = {pieces[n].x, pieces[n].y, pieces[n].z, pieces[n].w};
-      if constexpr (F16) {
-        uint32_t top2 = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          top2 = __vmaxu2(top2, w[i] & 0x7fff7fffu);
-#pragma unroll
-        for (int o = 1; o < kLanes; o <<= 1)
-          top2 = __vmaxu2(top2, __shfl_xor_sync(0xffffffffu, top2, o));
-        const uint32_t top = max(top2 & 0xffffu, top2 >> 16);
-        const int up = top == 0 ? 0 : min(126, 14 - (static_cast<int>(top >> 7) - 127));
-        const float mult = __uint_as_float(static_cast<uint32_t>(up + 127) << 23 | (negative ? 0x80000000u : 0u));
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          w[i] = pack16<true>(__uint_as_float(w[i] << 16) * mult, __uint_as_float(w[i] & 0xffff0000u) * mult);
-        if (piece == 0)
-          unscale[r] = __int_as_float(min(254, 3 - up + 127) << 23);
-      } else if (negative) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          w[i] ^= 0x80008000u;
-      }
-      *reinterpret_cast<uint4 *>(to + (piece / 8) * (kRows * 128) + r * 128 + ((piece % 8 ^ r & 7) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-  }
-
-  // From f32 rows D + 4 apart; `pieces` are the gates.
-  __device__ __forceinline__ void store(const Tile &p, const float *from, int chunk) const {
-#pragma unroll
-    for (int n = 0; n < kMine; ++n) {
-      const unsigned r = first + n * kStep;
-      if (r >= rows)
-        break;
-      const float4 *v = reinterpret_cast<const float4 *>(from + r * (D + 4) + piece * 8);
-      const int64_t to = at(r, static_cast<int64_t>(p.call.heads) * D, D);
-      if (p.chunks == 1)
-        paged_store_row(p.call.out + to, v[0], v[1], pieces[n], p.call.gate != nullptr);
-      else
-        paged_store_part(static_cast<float *>(p.call.workspace) + (to - piece * 8) * p.chunks + chunk * D + piece * 8, v[0], v[1]);
-    }
+    return static_cast<int64_t>(token0 + token) * token_stride + static_cast<int64_t>(head0 + (r - token * group)) * head_stride;
   }
 };
 
-// Columns first .. first + N of a thread's row of O into its f32 row, times `scale`; zeros where the row has no weights.
-template <int D, int N>
-__device__ __forceinline__ void unload_row(float *row, uint32_t address, int first, float scale, bool empty) {
+// DIMS dimensions of every row into shared memory, by WARPS warps (zeros where there is no row); wait with copies_done.
+template <int DIMS, int WARPS>
+__device__ __forceinline__ void copy_rows_in(uint32_t to, const uint16_t *from, int64_t token_stride, int64_t head_stride, const TileRows &t, int warp, int lane) {
+  constexpr int kLanes = DIMS / 8, kSide = 32 / kLanes;
+  const int piece = lane % kLanes;
+#pragma unroll 2
+  for (int r = warp * kSide + lane / kLanes; r < kRows; r += WARPS * kSide) {
+    const bool there = r < static_cast<int>(t.rows);
+    const uint16_t *src = from + (there ? t.at(r, token_stride, head_stride) + piece * 8 : 0);
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + piece_at(r, piece)), "l"(src), "r"(there ? 16 : 0) : "memory");
+  }
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+
+template <int DIMS, int WARPS>
+__device__ __forceinline__ void copy_rows_out(uint16_t *to, int64_t token_stride, int64_t head_stride, const uint8_t *from, const TileRows &t, int warp, int lane) {
+  constexpr int kLanes = DIMS / 8, kSide = 32 / kLanes;
+  const int piece = lane % kLanes;
+#pragma unroll 2
+  for (int r = warp * kSide + lane / kLanes; r < static_cast<int>(t.rows); r += WARPS * kSide)
+    *reinterpret_cast<uint4 *>(to + t.at(r, token_stride, head_stride) + piece * 8) = *reinterpret_cast<const uint4 *>(from + piece_at(r, piece));
+}
+
+// f16 queries: the power of two that takes a row's largest |q| into [2^14, 2^15) (1 for a row of zeros), with the sign of
+// the scale; and what takes it back, with the keys' 1 / 8.
+template <int D> __device__ __forceinline__ float query_multiplier(const uint8_t *queries, int row, bool negative, float *unscale) {
+  uint32_t top2 = 0;
+#pragma unroll 4
+  for (int piece = 0; piece < D / 8; ++piece) {
+    const uint4 v = *reinterpret_cast<const uint4 *>(queries + piece_at(row, piece));
+    top2 = __vmaxu2(__vmaxu2(top2, __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu)), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+  }
+  const uint32_t top = max(top2 & 0xffffu, top2 >> 16);
+  const int up = top == 0 ? 0 : min(126, 14 - (static_cast<int>(top >> 7) - 127));
+  *unscale = __int_as_float(min(254, 3 - up + 127) << 23);
+  return __uint_as_float(static_cast<uint32_t>(up + 127) << 23 | (negative ? 0x80000000u : 0u));
+}
+
+// Two bf16 queries as the products take them: f16 times the multiplier, or bf16 with the sign of the scale.
+template <bool F16> __device__ __forceinline__ uint32_t query_pair(uint32_t w, float multiplier, bool negative) {
+  if constexpr (F16)
+    return pack16<true>(__uint_as_float(w << 16) * multiplier, __uint_as_float(w & 0xffff0000u) * multiplier);
+  return w ^ (negative ? 0x80008000u : 0u);
+}
+
+// DIMS dimensions of a thread's row of O, times `scale` and its gate (in shared memory, where there is one), as bf16 into
+// the gate's place; zeros where the row has no weights.
+template <int DIMS> __device__ __forceinline__ void unload_row(uint8_t *to, int row, uint32_t address, float scale, bool empty, bool gated) {
 #pragma unroll 1
-  for (int c = first; c < first + N; c += 32) {
+  for (int c = 0; c < DIMS / 32; ++c) {
     uint32_t o[32];
     __syncwarp();
-    tmem_load32(address + c, o);
+    tmem_load32(address + c * 32, o);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint4 *at = reinterpret_cast<uint4 *>(to + piece_at(row, c * 4 + k));
+      const uint4 gate = gated ? *at : make_uint4(0, 0, 0, 0);
+      const uint32_t g[4] = {gate.x, gate.y, gate.z, gate.w};
+      uint32_t words[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x = empty ? 0.0f : __uint_as_float(o[8 * k + 2 * i]) * scale, y = empty ? 0.0f : __uint_as_float(o[8 * k + 2 * i + 1]) * scale;
+        if (gated) {
+          x = times_sigmoid(x, __uint_as_float(g[i] << 16));
+          y = times_sigmoid(y, __uint_as_float(g[i] & 0xffff0000u));
+        }
+        words[i] = pack16<false>(x, y);
+      }
+      *at = make_uint4(words[0], words[1], words[2], words[3]);
+    }
+  }
+}
+
+// The same as a part, f32 rows of the workspace.
+template <int DIMS> __device__ __forceinline__ void unload_part(float *to, uint32_t address, float scale, bool empty, bool valid) {
+#pragma unroll 1
+  for (int c = 0; c < DIMS / 32; ++c) {
+    uint32_t o[32];
+    __syncwarp();
+    tmem_load32(address + c * 32, o);
+    if (!valid)
+      continue;
 #pragma unroll
     for (int u = 0; u < 32; u += 4)
-      *reinterpret_cast<float4 *>(row + c + u) = empty ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
-                                                       : make_float4(__uint_as_float(o[u]) * scale, __uint_as_float(o[u + 1]) * scale,
-                                                                     __uint_as_float(o[u + 2]) * scale, __uint_as_float(o[u + 3]) * scale);
+      *reinterpret_cast<float4 *>(to + c * 32 + u) = empty ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
+                                                           : make_float4(__uint_as_float(o[u]) * scale, __uint_as_float(o[u + 1]) * scale,
+                                                                         __uint_as_float(o[u + 2]) * scale, __uint_as_float(o[u + 3]) * scale);
   }
 }
 

@@ -209,23 +209,25 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
     const bool negative = factor < 0.0f; // goes into the queries: the largest product is the largest score
     const bool flat = factor == 0.0f;    // every score is 0: so are the queries, and the factor stays usable beside -infinity
     factor = flat ? 1.0f : fabsf(factor);
-    WholeRows<D, kSoftmaxWarps> whole(p, warp, lane, rows, token_first, head0);
-    whole.load(p.call.q, p.call.q_row, p.call.q_head, !flat);
+    const TileRows whole{flat ? 0 : rows, group, p.one_over_group, token_first, head0};
     uint8_t *staged = ring + kQSlot * kSlotBytes; // the loader leaves these slots until the queries have gone on
-    whole.stage_queries<F16>(staged, negative, references);
+    copy_rows_in<D, kSoftmaxWarps>(smem_u32(staged), p.call.q, p.call.q_row, p.call.q_head, whole, warp, lane);
+    copies_done();
     asm volatile("bar.sync 1, 256;" ::: "memory"); // the softmax warps
+    float multiplier = 1.0f, unscale = 1.0f;
     if constexpr (F16)
-      factor *= references[row];
-#pragma unroll
-    for (int c = 0; c < D / 2 / 32; ++c) { // 32 dimensions = 16 columns at a time; half of them each
-      const int d = half * (D / 2) + c * 32;
+      multiplier = query_multiplier<D>(staged, row, negative, &unscale);
+    factor *= unscale;
+#pragma unroll 1
+    for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c) { // 32 dimensions = 16 columns at a time; half of them each
       uint32_t w[16];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(staged + (d / 64) * (kRows * 128) + row * 128 + ((d % 64 / 8 + k ^ row & 7) << 4));
-        w[4 * k] = v.x, w[4 * k + 1] = v.y, w[4 * k + 2] = v.z, w[4 * k + 3] = v.w;
+        const uint4 v = *reinterpret_cast<const uint4 *>(staged + piece_at(row, c * 4 + k));
+        w[4 * k] = query_pair<F16>(v.x, multiplier, negative), w[4 * k + 1] = query_pair<F16>(v.y, multiplier, negative);
+        w[4 * k + 2] = query_pair<F16>(v.z, multiplier, negative), w[4 * k + 3] = query_pair<F16>(v.w, multiplier, negative);
       }
-      tmem_store16(lanes + kQColumn + d / 2, w);
+      tmem_store16(lanes + kQColumn + c * 16, w);
     }
     tmem_wait_stores();
     tc_fence_before();
@@ -233,8 +235,6 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
     __syncwarp();
     if (lane == 0)
       mbar_arrive(&bars.q_full);
-    if constexpr (F16)
-      asm volatile("bar.sync 1, 256;" ::: "memory"); // the factors have been read: their place is the references' now
 
     RowScores r;
     const int position = seq.length - seq.count + token0 + static_cast<int>(row / group);
@@ -290,11 +290,21 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
     // ---- epilogue: the two halves' sums, then half of the dimensions each -----------------------------------------------------------
     last_reference[half][row] = reference;
     sums[half][row] = sum;
+    // Gates, then results, lie in the two slots after the ring's last item: what was in them, six items before their turn, was
+    // done with before the last scores that either half has seen.
+    const TileRows mine{rows, group, p.one_over_group, token_first, head0};
+    uint8_t *rows_out = ring + (2 * tiles + half) % kSlots * kSlotBytes;
+    const bool gated = p.call.gate && p.chunks == 1;
     asm volatile("bar.sync 1, 256;" ::: "memory");
-    whole.load(p.call.gate, p.call.gate_row, p.call.gate_head, p.call.gate && p.chunks == 1); // on their way while the last products run
+    if (ok && gated)
+      copy_rows_in<D / 2, 4>(smem_u32(rows_out), p.call.gate + half * (D / 2), p.call.gate_row, p.call.gate_head, mine, quarter, lane);
     if (ok && tiles > 0)
       ok = all_wait(&bars.o_full, 0);
-    float *rows_out = reinterpret_cast<float *>(ring); // the ring is done with
+    copies_done();
+    if (half == 0)
+      asm volatile("bar.sync 2, 128;" ::: "memory");
+    else
+      asm volatile("bar.sync 3, 128;" ::: "memory");
     if (ok) {
       tc_fence_after();
       const float final_reference = tiles > 0 ? references[row] : -INFINITY;
@@ -304,13 +314,22 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
         total += last_reference[h][row] == -INFINITY ? 0.0f : sums[h][row] * exp2_approx(last_reference[h][row] - final_reference);
       // f16 values are 1 / 8 of themselves; where a row has seen nothing O may hold anything
       const float scale = (F16 ? 8.0f : 1.0f) * (p.chunks == 1 && total != 0.0f ? __fdiv_rn(1.0f, total) : 1.0f);
-      unload_row<D, D / 2>(rows_out + row * (D + 4), lanes + kOColumn, half * (D / 2), scale, total == 0.0f);
-      if (p.chunks > 1 && half == 0 && valid)
-        paged_store_sums<D>(p.call, p.batch.tokens, p.chunks, chunk_index, token_first + row / group, head0 + row % group, final_reference, total);
+      const uint32_t o_at = lanes + kOColumn + half * (D / 2);
+      if (p.chunks == 1) {
+        unload_row<D / 2>(rows_out, row, o_at, scale, total == 0.0f, gated);
+      } else {
+        const int64_t part = (mine.at(row, p.call.heads, 1) * p.chunks + chunk_index) * D + half * (D / 2);
+        unload_part<D / 2>(static_cast<float *>(p.call.workspace) + (valid ? part : 0), o_at, scale, total == 0.0f, valid);
+        if (half == 0 && valid)
+          paged_store_sums<D>(p.call, p.batch.tokens, p.chunks, chunk_index, token_first + row / group, head0 + row % group, final_reference, total);
+      }
     }
-    asm volatile("bar.sync 1, 256;" ::: "memory");
-    if (ok)
-      whole.store(p, rows_out, chunk_index);
+    if (half == 0)
+      asm volatile("bar.sync 2, 128;" ::: "memory");
+    else
+      asm volatile("bar.sync 3, 128;" ::: "memory");
+    if (ok && p.chunks == 1)
+      copy_rows_out<D / 2, 4>(p.call.out + half * (D / 2), static_cast<int64_t>(p.call.heads) * D, D, rows_out, mine, quarter, lane);
   }
 
   tc_fence_before();
