@@ -59,6 +59,19 @@ inline bool paged_scale_map(CUtensorMap *map, const PagedKv &kv, int64_t rows, i
                 CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// [token][head][dim] rows with strides, in boxes of 64 dimensions x `group` heads x `box_tokens` tokens, swizzled.
+inline bool paged_rows_map(CUtensorMap *map, const uint16_t *base, int dim, int heads, int tokens, int64_t head_stride, int64_t token_stride, int group, int box_tokens) {
+  tc::EncodeTiled encode = tc::encode_tiled();
+  if (!encode)
+    return false;
+  // the stride of a dimension with one entry is never used, but has to be one
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(2 * (heads > 1 ? head_stride : dim)), static_cast<cuuint64_t>(2 * (tokens > 1 ? token_stride : dim))};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(group), static_cast<cuuint32_t>(box_tokens)}, elem[3] = {1, 1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<uint16_t *>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 #ifdef __CUDACC__
 // 2^x by the hardware's instruction (relative error about 2^-22; 0 for -infinity).
 __device__ __forceinline__ float exp2_approx(float x) {

@@ -33,7 +33,9 @@ template <int D> struct Shape {
 
 template <int SLOTS> struct Barriers {
   uint64_t full[SLOTS], empty[SLOTS]; // a tile of keys or values
-  uint64_t q_full;                    // the queries are in shared memory
+  uint64_t q_here;                    // the queries have landed
+  uint64_t q_full;                    // ... and are as the products take them
+  uint64_t gates_here;
   uint64_t s_full[2];                 // [key tile & 1]: scores are in tensor memory
   uint64_t p_full[2];                 // their weights are
   uint64_t o_done[2];                 // P V has been added
@@ -45,7 +47,7 @@ template <int SLOTS> struct Barriers {
 
 template <int D, bool F16>
 __global__ void __launch_bounds__(kThreads, 2)
-paged_narrow_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_constant__ Tile p, int *__restrict__ status) {
+paged_narrow_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_constant__ RowMaps maps, const __grid_constant__ Tile p, int *__restrict__ status) {
   using S = Shape<D>;
   extern __shared__ uint8_t raw_smem[];
   __shared__ Barriers<S::slots> bars;
@@ -66,7 +68,9 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap map_values, const __grid
       mbar_init(&bars.p_full[i], 4);
       mbar_init(&bars.o_done[i], 1);
     }
+    mbar_init(&bars.q_here, 1);
     mbar_init(&bars.q_full, 4);
+    mbar_init(&bars.gates_here, 1);
     mbar_init(&bars.o_full, 1);
     mbar_init(&bars.tail_here, 1);
     mbar_init(&bars.tail_ready, 1);
@@ -104,6 +108,12 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap map_values, const __grid
     const int ahead = min(2, tiles);
     int issued = 0, keys_issued = 0, values_issued = 0;
     bool ok = true;
+    const int slab_bytes = p.tokens_per_tile * p.group * 128, token_first = seq.first + token0, head0 = kvh * p.group;
+    if (lane == 0) {
+      mbar_expect_tx(&bars.q_here, S::slabs * slab_bytes);
+      for (int k = 0; k < S::slabs; ++k)
+        load_slab(q_sm + k * (kRows * 128), &maps.queries, k * 64, head0, token_first, &bars.q_here);
+    }
     for (int n = 0; n < 2 * tiles && ok; ++n) {
       const int which = keys_issued < tiles && keys_issued - values_issued < ahead ? 0 : 1;
       const int i = which ? values_issued++ : keys_issued++;
@@ -120,9 +130,25 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap map_values, const __grid
       if (slab < S::slabs)
         tma_load_2d(ring + s * S::slot_bytes + (slab * KT + sub * p.box_rows) * 128, &map_values, slab * 64, row, &bars.full[s]);
     }
-    if (*abort_flag) // copies already requested still write into this CTA's shared memory
+    // the gates take the queries' place, once the last keys' product is done (or nobody has wanted them)
+    bool gates = false;
+    if (ok && p.call.gate && p.chunks == 1) {
+      const int last = tiles == 1 ? 0 : 2 * tiles - 3; // the ring's item
+      gates = __all_sync(0xffffffffu, tiles > 0 ? mbar_wait<false>(&bars.empty[last % S::slots], (last / S::slots) & 1, abort_flag, p.spin_limit)
+                                                 : mbar_wait<false>(&bars.q_full, 0, abort_flag, p.spin_limit));
+      if (gates && lane == 0) {
+        mbar_expect_tx(&bars.gates_here, S::slabs * slab_bytes);
+        for (int k = 0; k < S::slabs; ++k)
+          load_slab(q_sm + k * (kRows * 128), &maps.gates, k * 64, head0, token_first, &bars.gates_here);
+      }
+    }
+    if (*abort_flag) { // copies already requested still write into this CTA's shared memory
+      mbar_wait_quiet<false>(&bars.q_here, 0, p.spin_limit);
+      if (gates)
+        mbar_wait_quiet<false>(&bars.gates_here, 0, p.spin_limit);
       for (int n = max(0, issued - S::slots); n < issued; ++n)
         mbar_wait_quiet<false>(&bars.full[n % S::slots], (n / S::slots) & 1, p.spin_limit);
+    }
   } else if (warp == kMmaWarp) {
     // ---- MMA issue: one thread ---------------------------------------------------------------------------------------------------
     if (elect_one()) {
@@ -197,11 +223,9 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap map_values, const __grid
     const bool negative = r.factor < 0.0f; // goes into the queries: the largest product is the largest score
     const bool flat = r.factor == 0.0f;    // every score is 0: so are the queries, and the factor stays usable beside -infinity
     r.factor = flat ? 1.0f : fabsf(r.factor);
-    const TileRows whole{flat ? 0 : rows, group, p.one_over_group, token_first, head0};
-    copy_rows_in<D, 4>(smem_u32(q_sm), p.call.q, p.call.q_row, p.call.q_head, whole, warp, lane);
-    copies_done();
-    if (F16 || negative) { // in place, a row per thread
-      asm volatile("bar.sync 1, 128;" ::: "memory"); // the softmax warps
+    auto all_wait = [&](uint64_t *bar, int parity) { return __all_sync(0xffffffffu, mbar_wait<false>(bar, parity, abort_flag, p.spin_limit)); };
+    bool ok = all_wait(&bars.q_here, 0);
+    if (F16 || negative || flat) { // in place, a row per thread
       float multiplier = 1.0f, unscale = 1.0f;
       if constexpr (F16)
         multiplier = query_multiplier<D>(q_sm, row, negative, &unscale);
@@ -209,9 +233,7 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap map_values, const __grid
 #pragma unroll 2
       for (int piece = 0; piece < D / 8; ++piece) {
         uint4 *at = reinterpret_cast<uint4 *>(q_sm + piece_at(row, piece));
-        const uint4 v = *at;
-        *at = make_uint4(query_pair<F16>(v.x, multiplier, negative), query_pair<F16>(v.y, multiplier, negative),
-                         query_pair<F16>(v.z, multiplier, negative), query_pair<F16>(v.w, multiplier, negative));
+        *at = query_piece<F16>(*at, multiplier, negative, flat);
       }
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // visible to the tensor core's reads
@@ -224,9 +246,7 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap map_values, const __grid
     r.slope = r.biased && valid ? p.call.slopes[head0 + row % group] * 1.4426950408889634f : 0.0f, r.at = static_cast<float>(position);
     r.sees = valid ? max(0, min(seq.length, max(position + 1, prefix))) : 0, r.sees_least = sees_least;
     float reference = -INFINITY, sum = 0.0f;
-    bool ok = true;
-    auto all_wait = [&](uint64_t *bar, int parity) { return __all_sync(0xffffffffu, mbar_wait<false>(bar, parity, abort_flag, p.spin_limit)); };
-    for (int i = 0; i < tiles; ++i) {
+    for (int i = 0; i < tiles && ok; ++i) {
       ok = all_wait(&bars.s_full[i & 1], (i >> 1) & 1);
       if (!ok)
         break;
@@ -259,17 +279,13 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap map_values, const __grid
         mbar_arrive(&bars.p_full[i & 1]);
     }
     // ---- epilogue -------------------------------------------------------------------------------------------------------------------
-    // Gates, then results, lie in the queries' place: the last scores that this warp has seen were their last product.  (All
-    // four warps have to have seen them.)
+    // Gates, then results, lie in the queries' place.
     const TileRows mine{rows, group, p.one_over_group, token_first, head0};
     const bool gated = p.call.gate && p.chunks == 1;
-    asm volatile("bar.sync 1, 128;" ::: "memory");
     if (ok && gated)
-      copy_rows_in<D, 4>(smem_u32(q_sm), p.call.gate, p.call.gate_row, p.call.gate_head, mine, warp, lane);
+      ok = all_wait(&bars.gates_here, 0);
     if (ok && tiles > 0)
       ok = all_wait(&bars.o_full, 0);
-    copies_done();
-    asm volatile("bar.sync 1, 128;" ::: "memory");
     if (ok) {
       tc_fence_after();
       // f16 values are 1 / 8 of themselves; where a row has seen nothing O may hold anything
@@ -298,19 +314,19 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap map_values, const __grid
     atomicOr(status, kStatusWaitRanOut);
 }
 
-template <int D, bool F16> cudaError_t launch(const CUtensorMap &values, const Tile &p, unsigned q_tiles, int *status, cudaStream_t stream) {
+template <int D, bool F16> cudaError_t launch(const CUtensorMap &values, const RowMaps &maps, const Tile &p, unsigned q_tiles, int *status, cudaStream_t stream) {
   const auto kernel = paged_narrow_kernel<D, F16>;
   if (cudaError_t e = opt_in_shared_memory(reinterpret_cast<const void *>(kernel), Shape<D>::smem); e != cudaSuccess)
     return e;
-  return launch_chained(kernel, dim3(p.kv.kv_heads * q_tiles, p.batch.sequences, p.chunks), dim3(kThreads), Shape<D>::smem, stream, values, p, status);
+  return launch_chained(kernel, dim3(p.kv.kv_heads * q_tiles, p.batch.sequences, p.chunks), dim3(kThreads), Shape<D>::smem, stream, values, maps, p, status);
 }
 
 } // namespace
 
-cudaError_t launch_paged_narrow(int head_dim, bool f16, const CUtensorMap &values, const Tile &p, unsigned q_tiles, int *status, cudaStream_t stream) {
+cudaError_t launch_paged_narrow(int head_dim, bool f16, const CUtensorMap &values, const RowMaps &maps, const Tile &p, unsigned q_tiles, int *status, cudaStream_t stream) {
   if (head_dim == 64)
-    return f16 ? launch<64, true>(values, p, q_tiles, status, stream) : launch<64, false>(values, p, q_tiles, status, stream);
-  return f16 ? launch<128, true>(values, p, q_tiles, status, stream) : launch<128, false>(values, p, q_tiles, status, stream);
+    return f16 ? launch<64, true>(values, maps, p, q_tiles, status, stream) : launch<64, false>(values, maps, p, q_tiles, status, stream);
+  return f16 ? launch<128, true>(values, maps, p, q_tiles, status, stream) : launch<128, false>(values, maps, p, q_tiles, status, stream);
 }
 
 } // namespace llmcp_b200

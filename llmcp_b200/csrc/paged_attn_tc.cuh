@@ -124,6 +124,24 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 }
 
 
+// 2^y of two finite values by multiplications: y = n + f with n an integer and |f| <= 1/2 (the range reduction of Cody and
+// Waite), 2^f by a polynomial of degree 4 (relative error 2.6e-6, fitted for the smallest largest error), n into the
+// exponent.  Below 2^-126 the result is some number about as small.
+__device__ __forceinline__ float2 exp2_by_fma(uint64_t y) {
+  constexpr float kRound = 12582912.0f; // 1.5 * 2^23: what is added to it is rounded to an integer
+  float2 v = halves(y);
+  y = pair(fmaxf(v.x, -126.0f), fmaxf(v.y, -126.0f));
+  const uint64_t t = add2(y, pair(kRound, kRound)), f = fma2(add2(t, pair(-kRound, -kRound)), pair(-1.0f, -1.0f), y);
+  uint64_t r = fma2(f, pair(0.00957010032775151f, 0.00957010032775151f), pair(0.05591786276854936f, 0.05591786276854936f));
+  r = fma2(r, f, pair(0.24024744889319694f, 0.24024744889319694f));
+  r = fma2(r, f, pair(0.693121814447754f, 0.693121814447754f));
+  r = fma2(r, f, pair(0.9999992614202372f, 0.9999992614202372f));
+  const float2 n = halves(t), e = halves(r);
+  v.x = __int_as_float(__float_as_int(e.x) + (__float_as_int(n.x) << 23));
+  v.y = __int_as_float(__float_as_int(e.y) + (__float_as_int(n.y) << 23));
+  return v;
+}
+
 // Two barriers awaited together: a look at one takes some 150 cycles, and looks at both overlap.
 __device__ __forceinline__ bool wait_for_both(uint64_t *a, uint32_t pa, uint64_t *b, uint32_t pb, volatile int *abort_flag, uint32_t limit) {
   const uint32_t aa = smem_u32(a), ab = smem_u32(b);
@@ -156,24 +174,6 @@ struct RowScores {
   int sees, sees_least; // keys below: this row, every row of its tile
   bool biased;
 };
-
-// 2^y of two finite values by multiplications: y = n + f with n an integer and |f| <= 1/2 (the range reduction of Cody and
-// Waite), 2^f by a polynomial of degree 4 (relative error 2.6e-6, fitted for the smallest largest error), n into the
-// exponent.  Below 2^-126 the result is some number about as small.
-__device__ __forceinline__ float2 exp2_by_fma(uint64_t y) {
-  constexpr float kRound = 12582912.0f; // 1.5 * 2^23: what is added to it is rounded to an integer
-  float2 v = halves(y);
-  y = pair(fmaxf(v.x, -126.0f), fmaxf(v.y, -126.0f));
-  const uint64_t t = add2(y, pair(kRound, kRound)), f = fma2(add2(t, pair(-kRound, -kRound)), pair(-1.0f, -1.0f), y);
-  uint64_t r = fma2(f, pair(0.00957010032775151f, 0.00957010032775151f), pair(0.05591786276854936f, 0.05591786276854936f));
-  r = fma2(r, f, pair(0.24024744889319694f, 0.24024744889319694f));
-  r = fma2(r, f, pair(0.693121814447754f, 0.693121814447754f));
-  r = fma2(r, f, pair(0.9999992614202372f, 0.9999992614202372f));
-  const float2 n = halves(t), e = halves(r);
-  v.x = __int_as_float(__float_as_int(e.x) + (__float_as_int(n.x) << 23));
-  v.y = __int_as_float(__float_as_int(e.y) + (__float_as_int(n.y) << 23));
-  return v;
-}
 
 // scale * tanh of two values by an odd polynomial, fitted likewise: of at most 1 by degree 13 (absolute error 4.4e-8), of at
 // most 1/2 by degree 9 (6.3e-9).
@@ -314,6 +314,13 @@ template <int D> __device__ __forceinline__ void rescale_row(uint32_t address, f
 // Rows of queries, gates and results lie in shared memory as K-major slabs of 64 dimensions, 128 rows of 128 bytes each,
 // 16-byte pieces where the 128-byte swizzle has them.  Everything below is done once per CTA and written as short loops:
 // unrolled, its instructions take longer to fetch than to execute.
+// They come in by TMA, a slab a copy: a box of 64 dimensions x group heads x tokens_per_tile tokens of a [token][head][dim]
+// tensor (rows of the next sequence among them, zeros past the tensor, and nothing in the rows past a whole number of tokens).
+__device__ __forceinline__ void load_slab(uint8_t *to, const CUtensorMap *map, int dim, int head0, int token0, uint64_t *bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(to)),
+               "l"(reinterpret_cast<uint64_t>(map)), "r"(dim), "r"(head0), "r"(token0), "r"(smem_u32(bar))
+               : "memory");
+}
 __device__ __forceinline__ uint32_t piece_at(int row, int piece) { return (piece / 8) * (kRows * 128) + row * 128 + ((piece % 8 ^ row & 7) << 4); }
 
 // Which rows of global memory those are: row r is token r / group, head r % group.  (r below 128 and group at most 128: the
@@ -326,21 +333,6 @@ struct TileRows {
     return static_cast<int64_t>(token0 + token) * token_stride + static_cast<int64_t>(head0 + (r - token * group)) * head_stride;
   }
 };
-
-// DIMS dimensions of every row into shared memory, by WARPS warps (zeros where there is no row); wait with copies_done.
-template <int DIMS, int WARPS>
-__device__ __forceinline__ void copy_rows_in(uint32_t to, const uint16_t *from, int64_t token_stride, int64_t head_stride, const TileRows &t, int warp, int lane) {
-  constexpr int kLanes = DIMS / 8, kSide = 32 / kLanes;
-  const int piece = lane % kLanes;
-#pragma unroll 2
-  for (int r = warp * kSide + lane / kLanes; r < kRows; r += WARPS * kSide) {
-    const bool there = r < static_cast<int>(t.rows);
-    const uint16_t *src = from + (there ? t.at(r, token_stride, head_stride) + piece * 8 : 0);
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + piece_at(r, piece)), "l"(src), "r"(there ? 16 : 0) : "memory");
-  }
-  asm volatile("cp.async.commit_group;" ::: "memory");
-}
-__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 
 template <int DIMS, int WARPS>
 __device__ __forceinline__ void copy_rows_out(uint16_t *to, int64_t token_stride, int64_t head_stride, const uint8_t *from, const TileRows &t, int warp, int lane) {
@@ -366,11 +358,18 @@ template <int D> __device__ __forceinline__ float query_multiplier(const uint8_t
   return __uint_as_float(static_cast<uint32_t>(up + 127) << 23 | (negative ? 0x80000000u : 0u));
 }
 
-// Two bf16 queries as the products take them: f16 times the multiplier, or bf16 with the sign of the scale.
-template <bool F16> __device__ __forceinline__ uint32_t query_pair(uint32_t w, float multiplier, bool negative) {
+// Two bf16 queries as the products take them: f16 times the multiplier, or bf16 with the sign of the scale; zeros where the
+// scale is 0.
+template <bool F16> __device__ __forceinline__ uint32_t query_pair(uint32_t w, float multiplier, bool negative, bool flat) {
   if constexpr (F16)
-    return pack16<true>(__uint_as_float(w << 16) * multiplier, __uint_as_float(w & 0xffff0000u) * multiplier);
-  return w ^ (negative ? 0x80008000u : 0u);
+    w = pack16<true>(__uint_as_float(w << 16) * multiplier, __uint_as_float(w & 0xffff0000u) * multiplier);
+  else
+    w ^= negative ? 0x80008000u : 0u;
+  return flat ? 0u : w;
+}
+template <bool F16> __device__ __forceinline__ uint4 query_piece(uint4 v, float multiplier, bool negative, bool flat) {
+  return make_uint4(query_pair<F16>(v.x, multiplier, negative, flat), query_pair<F16>(v.y, multiplier, negative, flat),
+                    query_pair<F16>(v.z, multiplier, negative, flat), query_pair<F16>(v.w, multiplier, negative, flat));
 }
 
 // DIMS dimensions of a thread's row of O, times `scale` and its gate (in shared memory, where there is one), as bf16 into
@@ -390,9 +389,11 @@ template <int DIMS> __device__ __forceinline__ void unload_row(uint8_t *to, int 
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float x = empty ? 0.0f : __uint_as_float(o[8 * k + 2 * i]) * scale, y = empty ? 0.0f : __uint_as_float(o[8 * k + 2 * i + 1]) * scale;
-        if (gated) {
-          x = times_sigmoid(x, __uint_as_float(g[i] << 16));
-          y = times_sigmoid(y, __uint_as_float(g[i] & 0xffff0000u));
+        if (gated) { // x / (1 + e^-gate); at a gate below -80 the product is 0 beside any other value of a row
+          const float g0 = fminf(__uint_as_float(g[i] << 16) * -1.4426950408889634f, 115.0f), g1 = fminf(__uint_as_float(g[i] & 0xffff0000u) * -1.4426950408889634f, 115.0f);
+          const float2 e = exp2_by_fma(pair(g0, g1));
+          x = __fdividef(x, 1.0f + e.x);
+          y = __fdividef(y, 1.0f + e.y);
         }
         words[i] = pack16<false>(x, y);
       }
@@ -441,8 +442,13 @@ template <int KT, int SLABS> __device__ __forceinline__ void zero_tail(uint8_t *
   __syncwarp();
 }
 
+// Maps of the queries and the gates (another of the queries' where there are none).
+struct RowMaps {
+  CUtensorMap queries, gates;
+};
+
 } // namespace tc
 
-cudaError_t launch_paged_narrow(int head_dim, bool f16, const CUtensorMap &values, const tc::Tile &p, unsigned q_tiles, int *status, cudaStream_t stream);
+cudaError_t launch_paged_narrow(int head_dim, bool f16, const CUtensorMap &values, const tc::RowMaps &maps, const tc::Tile &p, unsigned q_tiles, int *status, cudaStream_t stream);
 
 } // namespace llmcp_b200

@@ -45,7 +45,8 @@ struct Barriers {
   uint64_t p_full[2];                 // its weights are
   uint64_t o_full;                    // every tile's P V has been added
   uint64_t tail_here, tail_ready;     // the last tile of a sequence's values has landed; its rows past the end are zeros
-  uint64_t q_full;                    // the queries are
+  uint64_t q_here;                    // the queries have landed
+  uint64_t q_full;                    // ... and are in tensor memory
   uint64_t o_done[2];                 // [tile & 1]: P V of a tile has been added
   uint64_t reference[2][4];           // [tile & 1][32 rows]: the reference after a tile
   uint32_t tmem_base;
@@ -54,7 +55,7 @@ struct Barriers {
 
 template <bool F16>
 __global__ void __launch_bounds__(kThreads, 1)
-paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_constant__ Tile p, int *__restrict__ status) {
+paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_constant__ RowMaps maps, const __grid_constant__ Tile p, int *__restrict__ status) {
   extern __shared__ uint8_t raw_smem[];
   __shared__ Barriers bars;
   __shared__ float references[kRows], last_reference[2][kRows], sums[2][kRows];
@@ -79,6 +80,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
       for (int w = 0; w < 4; ++w)
         mbar_init(&bars.reference[i][w], 1);
     }
+    mbar_init(&bars.q_here, 1);
     mbar_init(&bars.q_full, kSoftmaxWarps);
     bars.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -115,27 +117,40 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
     const int ahead = min(2, tiles);
     int issued = 0, keys_issued = 0, values_issued = 0;
     bool ok = true;
-    for (int n = 0; n < 2 * tiles && ok; ++n) {
+    const int slab_bytes = p.tokens_per_tile * p.group * 128, token_first = seq.first + token0, head0 = kvh * p.group;
+    if (lane == 0) {
+      mbar_expect_tx(&bars.q_here, kSlabs * slab_bytes);
+      for (int k = 0; k < kSlabs; ++k)
+        load_slab(ring + kQSlot * kSlotBytes + k * (kRows * 128), &maps.queries, k * 64, head0, token_first, &bars.q_here);
+    }
+    const bool gated = p.call.gate && p.chunks == 1;
+    for (int n = 0; n < 2 * tiles + (gated ? 2 : 0) && ok; ++n) { // the gates are the last two items: half of the dimensions each
+      const bool gates = n >= 2 * tiles;
       const int which = keys_issued < tiles && keys_issued - values_issued < ahead ? 0 : 1;
       const int i = which ? values_issued++ : keys_issued++;
-      const int row = tile_box_row(p, seq, table, b, kvh, which, key0 + i * KT + sub * p.box_rows, slab < kSlabs, status);
+      const int row = tile_box_row(p, seq, table, b, kvh, which, key0 + i * KT + sub * p.box_rows, !gates && slab < kSlabs, status);
       const int s = n % kSlots;
-      if (n == kQSlot)
+      if (n == kQSlot || (gates && n == 2 * tiles)) // these slots may still hold the queries
         ok = __all_sync(0xffffffffu, mbar_wait<false>(&bars.q_full, 0, abort_flag, p.spin_limit));
       if (ok && n >= kSlots)
         ok = __all_sync(0xffffffffu, mbar_wait<false>(&bars.empty[s], (n / kSlots - 1) & 1, abort_flag, p.spin_limit));
       if (!ok)
         break;
       if (lane == 0)
-        mbar_expect_tx(&bars.full[s], kSlotBytes);
+        mbar_expect_tx(&bars.full[s], gates ? kSlabs / 2 * slab_bytes : kSlotBytes);
       __syncwarp();
       issued = n + 1;
-      if (slab < kSlabs)
+      if (gates) {
+        if (lane < kSlabs / 2)
+          load_slab(ring + s * kSlotBytes + lane * (kRows * 128), &maps.gates, (n - 2 * tiles) * (D / 2) + lane * 64, head0, token_first, &bars.full[s]);
+      } else if (slab < kSlabs)
         tma_load_2d(ring + s * kSlotBytes + (slab * KT + sub * p.box_rows) * 128, &map_values, slab * 64, row, &bars.full[s]);
     }
-    if (*abort_flag) // copies already requested still write into this CTA's shared memory
+    if (*abort_flag) { // copies already requested still write into this CTA's shared memory
+      mbar_wait_quiet<false>(&bars.q_here, 0, p.spin_limit);
       for (int n = max(0, issued - kSlots); n < issued; ++n)
         mbar_wait_quiet<false>(&bars.full[n % kSlots], (n / kSlots) & 1, p.spin_limit);
+    }
   } else if (warp == kMmaWarp) {
     // ---- MMA issue: one thread ---------------------------------------------------------------------------------------------------
     if (elect_one()) {
@@ -209,11 +224,9 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
     const bool negative = factor < 0.0f; // goes into the queries: the largest product is the largest score
     const bool flat = factor == 0.0f;    // every score is 0: so are the queries, and the factor stays usable beside -infinity
     factor = flat ? 1.0f : fabsf(factor);
-    const TileRows whole{flat ? 0 : rows, group, p.one_over_group, token_first, head0};
-    uint8_t *staged = ring + kQSlot * kSlotBytes; // the loader leaves these slots until the queries have gone on
-    copy_rows_in<D, kSoftmaxWarps>(smem_u32(staged), p.call.q, p.call.q_row, p.call.q_head, whole, warp, lane);
-    copies_done();
-    asm volatile("bar.sync 1, 256;" ::: "memory"); // the softmax warps
+    const uint8_t *staged = ring + kQSlot * kSlotBytes; // the loader leaves these slots until the queries have gone on
+    auto all_wait = [&](uint64_t *bar, int parity) { return __all_sync(0xffffffffu, mbar_wait<false>(bar, parity, abort_flag, p.spin_limit)); };
+    bool ok = all_wait(&bars.q_here, 0);
     float multiplier = 1.0f, unscale = 1.0f;
     if constexpr (F16)
       multiplier = query_multiplier<D>(staged, row, negative, &unscale);
@@ -223,9 +236,8 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
       uint32_t w[16];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(staged + piece_at(row, c * 4 + k));
-        w[4 * k] = query_pair<F16>(v.x, multiplier, negative), w[4 * k + 1] = query_pair<F16>(v.y, multiplier, negative);
-        w[4 * k + 2] = query_pair<F16>(v.z, multiplier, negative), w[4 * k + 3] = query_pair<F16>(v.w, multiplier, negative);
+        const uint4 v = query_piece<F16>(*reinterpret_cast<const uint4 *>(staged + piece_at(row, c * 4 + k)), multiplier, negative, flat);
+        w[4 * k] = v.x, w[4 * k + 1] = v.y, w[4 * k + 2] = v.z, w[4 * k + 3] = v.w;
       }
       tmem_store16(lanes + kQColumn + c * 16, w);
     }
@@ -244,9 +256,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
     r.slope = r.biased && valid ? p.call.slopes[head0 + row % group] * 1.4426950408889634f : 0.0f, r.at = static_cast<float>(position);
     r.sees = valid ? max(0, min(seq.length, max(position + 1, prefix))) : 0, r.sees_least = sees_least;
     float reference = -INFINITY, sum = 0.0f;
-    bool ok = true;
-    auto all_wait = [&](uint64_t *bar, int parity) { return __all_sync(0xffffffffu, mbar_wait<false>(bar, parity, abort_flag, p.spin_limit)); };
-    for (int i = half; i < tiles; i += 2) {
+    for (int i = half; i < tiles && ok; i += 2) {
       ok = all_wait(&bars.s_full[half], (i >> 1) & 1);
       if (!ok)
         break;
@@ -290,21 +300,17 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
     // ---- epilogue: the two halves' sums, then half of the dimensions each -----------------------------------------------------------
     last_reference[half][row] = reference;
     sums[half][row] = sum;
-    // Gates, then results, lie in the two slots after the ring's last item: what was in them, six items before their turn, was
-    // done with before the last scores that either half has seen.
+    // Gates, then results, lie in the two slots after the ring's last item, a half's in its own: what was in them six items
+    // before was done with before the last scores that either half has seen.
     const TileRows mine{rows, group, p.one_over_group, token_first, head0};
-    uint8_t *rows_out = ring + (2 * tiles + half) % kSlots * kSlotBytes;
+    const int place = 2 * tiles + half;
+    uint8_t *rows_out = ring + place % kSlots * kSlotBytes;
     const bool gated = p.call.gate && p.chunks == 1;
     asm volatile("bar.sync 1, 256;" ::: "memory");
     if (ok && gated)
-      copy_rows_in<D / 2, 4>(smem_u32(rows_out), p.call.gate + half * (D / 2), p.call.gate_row, p.call.gate_head, mine, quarter, lane);
+      ok = all_wait(&bars.full[place % kSlots], (place / kSlots) & 1);
     if (ok && tiles > 0)
       ok = all_wait(&bars.o_full, 0);
-    copies_done();
-    if (half == 0)
-      asm volatile("bar.sync 2, 128;" ::: "memory");
-    else
-      asm volatile("bar.sync 3, 128;" ::: "memory");
     if (ok) {
       tc_fence_after();
       const float final_reference = tiles > 0 ? references[row] : -INFINITY;
@@ -403,11 +409,11 @@ cudaError_t expand(const PagedKv &kv, const PagedBatch &batch, uint8_t *to, int 
                         kv, batch, reinterpret_cast<uint4 *>(to), rows, status);
 }
 
-template <bool F16> cudaError_t launch_wide(const CUtensorMap &values, const Tile &p, unsigned q_tiles, int *status, cudaStream_t stream) {
+template <bool F16> cudaError_t launch_wide(const CUtensorMap &values, const RowMaps &maps, const Tile &p, unsigned q_tiles, int *status, cudaStream_t stream) {
   const auto kernel = paged_tile_kernel<F16>;
   if (cudaError_t e = opt_in_shared_memory(reinterpret_cast<const void *>(kernel), kSmem); e != cudaSuccess)
     return e;
-  return launch_chained(kernel, dim3(p.kv.kv_heads * q_tiles, p.batch.sequences, p.chunks), dim3(kThreads), kSmem, stream, values, p, status);
+  return launch_chained(kernel, dim3(p.kv.kv_heads * q_tiles, p.batch.sequences, p.chunks), dim3(kThreads), kSmem, stream, values, maps, p, status);
 }
 
 } // namespace
@@ -460,10 +466,16 @@ cudaError_t launch_paged_tile(const PagedKv &kv, const PagedBatch &batch, const 
   CUtensorMap values;
   if (!paged_value_map(&values, source, rows, p.box_rows))
     return cudaErrorNotSupported;
+  RowMaps maps;
+  if (!paged_rows_map(&maps.queries, call.q, kv.head_dim, call.heads, batch.tokens, call.q_head, call.q_row, p.group, p.tokens_per_tile))
+    return cudaErrorNotSupported;
+  maps.gates = maps.queries;
+  if (call.gate && !paged_rows_map(&maps.gates, call.gate, kv.head_dim, call.heads, batch.tokens, call.gate_head, call.gate_row, p.group, p.tokens_per_tile))
+    return cudaErrorNotSupported;
   const unsigned q_tiles = static_cast<unsigned>((batch.max_q + p.tokens_per_tile - 1) / p.tokens_per_tile);
   if (kv.head_dim != D)
-    return launch_paged_narrow(kv.head_dim, f16, values, p, q_tiles, status, stream);
-  return f16 ? launch_wide<true>(values, p, q_tiles, status, stream) : launch_wide<false>(values, p, q_tiles, status, stream);
+    return launch_paged_narrow(kv.head_dim, f16, values, maps, p, q_tiles, status, stream);
+  return f16 ? launch_wide<true>(values, maps, p, q_tiles, status, stream) : launch_wide<false>(values, maps, p, q_tiles, status, stream);
 }
 
 } // namespace llmcp_b200
