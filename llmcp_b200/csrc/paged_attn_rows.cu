@@ -111,6 +111,16 @@ template <int N> __device__ __forceinline__ void load_words(uint32_t (&w)[N], co
   }
 }
 
+// mbar_expect_tx and tma_load_2d on shared-memory addresses.
+__device__ __forceinline__ void expect_at(uint32_t bar, uint32_t bytes) {
+  asm volatile("{ .reg .b64 t; mbarrier.arrive.expect_tx.shared::cta.b64 t, [%0], %1; }" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_box(uint32_t to, const CUtensorMap *map, int x, int y, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(to),
+               "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+               : "memory");
+}
+
 struct Rows {
   PagedKv kv;
   PagedBatch batch;
@@ -161,41 +171,57 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
   // scales of 16 rows; a box of them starts on a 128-byte boundary
   const int scale_pitch = D == 64 && p.box_rows == 16 ? 128 : D;
   auto first_key = [&](int i) { return key0 + (warp + i * kWarps) * KT; };
-  auto page_of = [&](int i) { // of this lane's rows in tile i; -1: past the sequence
+  auto page_of = [&](int i) { // of this lane's rows in tile i
     const int key = first_key(i) + sub * p.box_rows;
     return i < tiles && lane < boxes && key < seq.length ? table[key >> p.kv.page_shift] : -1;
   };
-  int page_now = page_of(0), page_next = page_of(1), issued = 0;
-  auto issue = [&]() {
-    const int i = issued >> 1, which = issued & 1, s = issued % S::slots;
-    if (i < tiles) {
-      if (lane == 0)
-        mbar_expect_tx(&full[warp][s], S::value_bytes + S::scale_bytes);
-      __syncwarp();
-      if (lane < boxes) {
-        const int key = first_key(i) + sub * p.box_rows;
-        int row = p.out_of_range;
-        if (key < seq.length) {
-          if (page_now >= 0 && page_now < p.kv.num_pages)
-            row = (page_now * 2 + which) * head_rows + (kvh << p.kv.page_shift) + (key & ((1 << p.kv.page_shift) - 1));
-          else if (status)
-            atomicOr(status, kStatusBadBatch);
-        }
-        uint8_t *slot = ring + s * S::slot_bytes;
-        tma_load_2d(slot + (slab * KT + sub * p.box_rows) * S::row_bytes, &map_values, slab * 64, row, &full[warp][s]);
-        if (Q4)
-          tma_load_2d(slot + S::value_bytes + sub * (p.box_rows / 16) * scale_pitch, &map_scales, 0, row >> 4, &full[warp][s]);
-      }
-      if (which) {
-        page_now = page_next;
-        page_next = page_of(i + 2);
-      }
-      ++issued;
+  auto row_of = [&](int i, int page) { // of this lane's box of keys in tile i; out of range past the sequence
+    const int key = first_key(i) + sub * p.box_rows;
+    if (i >= tiles || lane >= boxes || key >= seq.length)
+      return p.out_of_range;
+    if (page >= 0 && page < p.kv.num_pages)
+      return page * 2 * head_rows + (kvh << p.kv.page_shift) + (key & ((1 << p.kv.page_shift) - 1));
+    if (status)
+      atomicOr(status, kStatusBadBatch);
+    return p.out_of_range;
+  };
+  const uint32_t ring_address = smem_u32(ring), full_address = smem_u32(&full[warp][0]);
+  const uint32_t box_at = (slab * KT + sub * p.box_rows) * S::row_bytes, scales_at = S::value_bytes + sub * (p.box_rows / 16) * scale_pitch;
+  int next_tile = 0, issue_slot = 0, issued = 0; // the next items are next_tile's: its row, and the page of the tile behind it
+  int row_next = row_of(0, page_of(0)), page_behind = page_of(1);
+  auto copy = [&](int row) {
+    const uint32_t bar = full_address + issue_slot * 8, slot = ring_address + issue_slot * S::slot_bytes;
+    if (lane == 0)
+      expect_at(bar, S::value_bytes + S::scale_bytes);
+    __syncwarp();
+    if (lane < boxes) {
+      copy_box(slot + box_at, &map_values, slab * 64, row, bar);
+      if (Q4)
+        copy_box(slot + scales_at, &map_scales, 0, row >> 4, bar);
+    }
+    issue_slot = issue_slot + 1 == S::slots ? 0 : issue_slot + 1;
+    ++issued;
+  };
+  auto issue_keys = [&]() {
+    if (next_tile < tiles)
+      copy(row_next);
+  };
+  auto issue_values = [&]() {
+    if (next_tile < tiles) {
+      copy(row_next == p.out_of_range ? row_next : row_next + head_rows);
+      ++next_tile;
+      row_next = row_of(next_tile, page_behind);
+      page_behind = page_of(next_tile + 1);
     }
   };
-  for (int i = 0; i < S::slots; ++i)
-    issue();
+  // three slots: the item behind a tile's values is the next but one tile's keys' place
+  issue_keys();
+  issue_values();
+  issue_keys();
 
+  // The sign of the scale goes into the queries, so that the largest product is the largest score; with a scale of 0 the
+  // queries are zeros and the factor stays usable beside -infinity.
+  const bool negative = p.call.scale < 0.0f, flat = p.call.scale == 0.0f;
   // ---- the queries: row 8 nt + g is token row / group, head kvh * group + row % group --------------------------------------
   uint32_t queries[kQueriesShared ? 1 : NT][Q4 ? NB * 4 : MT * 2];
   uint4 *queries_sm = reinterpret_cast<uint4 *>(base + kWarps * S::slots * S::slot_bytes);
@@ -213,7 +239,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
       uint32_t top = 0;
 #pragma unroll
       for (int k = 0; k < NB; ++k) {
-        raw[k] = row < rows ? *reinterpret_cast<const uint4 *>(q + 32 * k + 8 * t) : make_uint4(0, 0, 0, 0);
+        raw[k] = row < rows && !flat ? *reinterpret_cast<const uint4 *>(q + 32 * k + 8 * t) : make_uint4(0, 0, 0, 0);
         const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -222,7 +248,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const int up = top == 0 ? 0 : min(126, 14 - (static_cast<int>(top >> 7) - 127)); // q * 2^up has its largest in [2^14, 2^15)
-      const float mult = __int_as_float((up + 127) << 23);
+      const float mult = __uint_as_float(static_cast<uint32_t>(up + 127) << 23 | (negative ? 0x80000000u : 0u));
       unscale = __int_as_float(min(254, 24 - up + 127) << 23);
 #pragma unroll
       for (int k = 0; k < NB; ++k) {
@@ -258,7 +284,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
       for (int k = 0; k < MT; ++k)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          fragment[2 * k + i] = row < rows ? *reinterpret_cast<const uint32_t *>(q + 16 * k + 8 * i + 2 * t) : 0;
+          fragment[2 * k + i] = row < rows && !flat ? *reinterpret_cast<const uint32_t *>(q + 16 * k + 8 * i + 2 * t) ^ (negative ? 0x80008000u : 0u) : 0;
     }
     if constexpr (kQueriesShared) {
 #pragma unroll
@@ -290,7 +316,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      factor[nt][i] = p.call.scale * (p.call.softcap > 0.0f ? 1.0f : 1.4426950408889634f) * (Q4 ? unscales[nt * 8 + 2 * t + i] : 1.0f);
+      factor[nt][i] = (flat ? 1.0f : fabsf(p.call.scale) * (p.call.softcap > 0.0f ? 1.0f : 1.4426950408889634f)) * (Q4 ? unscales[nt * 8 + 2 * t + i] : 1.0f);
   }
   // four words of the fragments of dimensions 32 k .. 32 k + 31
   auto query_words = [&](int nt, int k, uint32_t (&w)[4]) {
@@ -321,7 +347,6 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
         out[mt][nt][i] = 0.0f;
   }
 
-  const uint32_t ring_address = smem_u32(ring);
   // where a lane reads for ldmatrix: row `row` of 16, 16-byte piece `piece` as the swizzle placed it; another even piece is
   // an exclusive or with it (rows and slots are aligned to the swizzle's span), another 16 rows an addition
   auto piece_offset = [&](int row, int piece) {
@@ -339,16 +364,23 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
   const int lm_row = lane & 7, lm_matrix = lane >> 3;
   const int rows_first = piece_offset((lm_matrix & 1) * 8 + lm_row, lm_matrix >> 1);   // matrices: rows, then pieces
   const int pieces_first = piece_offset((lm_matrix >> 1) * 8 + lm_row, lm_matrix & 1); // pieces, then rows
+  int slot_now = 0, phase_now = 0;
+  auto next_slot = [&]() {
+    if (++slot_now == S::slots) {
+      slot_now = 0;
+      phase_now ^= 1;
+    }
+  };
   bool ok = true;
   for (int i = 0; i < tiles; ++i) {
     const int j0 = first_key(i);
     // ---- scores -------------------------------------------------------------------------------------------------------------
-    int s = (2 * i) % S::slots;
-    ok = mbar_wait(&full[warp][s], ((2 * i) / S::slots) & 1, &failed, p.spin_limit);
-    ok = __all_sync(0xffffffffu, ok);
+    int s = slot_now;
+    ok = __all_sync(0xffffffffu, mbar_wait(&full[warp][s], phase_now, &failed, p.spin_limit));
     if (!ok)
       break;
     uint32_t slot = ring_address + s * S::slot_bytes;
+    next_slot();
     float x[M][NT][4];
 #pragma unroll
     for (int m = 0; m < M; ++m) {
@@ -410,14 +442,14 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
       }
     }
     __syncwarp();
-    issue();
+    issue_values();
     // ---- weights ------------------------------------------------------------------------------------------------------------
-    s = (2 * i + 1) % S::slots;
-    ok = mbar_wait(&full[warp][s], ((2 * i + 1) / S::slots) & 1, &failed, p.spin_limit);
-    ok = __all_sync(0xffffffffu, ok);
+    s = slot_now;
+    ok = __all_sync(0xffffffffu, mbar_wait(&full[warp][s], phase_now, &failed, p.spin_limit));
     if (!ok)
       break;
     slot = ring_address + s * S::slot_bytes;
+    next_slot();
     const bool tail = j0 + KT > seq.length; // rows of the tile past the sequence: whatever they hold
     if (tail) { // their weights are 0, and so are their values (bf16) or scales now
       if constexpr (Q4) {
@@ -442,28 +474,22 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
 #pragma unroll
         for (int k = 0; k < NB / 2; ++k)
           largest = __vmaxu2(largest, scale_words(s, n * 32 + lane)[k]);
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1)
-        largest = __vmaxu2(largest, __shfl_xor_sync(0xffffffffu, largest, o));
-      shift = fmaxf(shift, static_cast<float>(static_cast<int>(max(largest & 0xffffu, largest >> 16) >> 10) - 29) + kHeadroom);
+      largest = __reduce_max_sync(0xffffffffu, max(largest & 0xffffu, largest >> 16));
+      shift = fmaxf(shift, static_cast<float>(static_cast<int>(largest >> 10) - 29) + kHeadroom);
     }
     const bool masked = j0 + KT > sees_least; // some row does not see some key of the tile
-    float moved[NT][2];
-    bool any_moved = false;
+    bool outgrown = shift != shift_before;    // the reference moves only where a score has outgrown it by 2^8
+    float best[NT][2], scaled[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float best[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-      for (int m = 0; m < M; ++m)
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          x[m][nt][c] *= factor[nt][c & 1];
+      scaled[nt][0] = factor[nt][0], scaled[nt][1] = factor[nt][1];
       if (cap > 0.0f) {
 #pragma unroll
         for (int m = 0; m < M; ++m)
 #pragma unroll
           for (int c = 0; c < 4; ++c)
-            x[m][nt][c] = capped_log2(x[m][nt][c], cap, over_cap);
+            x[m][nt][c] = capped_log2(x[m][nt][c] * factor[nt][c & 1], cap, over_cap);
+        scaled[nt][0] = scaled[nt][1] = 1.0f;
       }
       if (biased || masked) {
 #pragma unroll
@@ -471,42 +497,51 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const int j = j0 + m * 16 + g + (c >> 1) * 8, row = nt * 8 + 2 * t + (c & 1);
-            x[m][nt][c] = j < sees[row] ? x[m][nt][c] - slope[row] * fabsf(at[row] - static_cast<float>(j)) : -INFINITY;
+            x[m][nt][c] = j < sees[row] ? x[m][nt][c] * scaled[nt][c & 1] - slope[row] * fabsf(at[row] - static_cast<float>(j)) : -INFINITY;
           }
+        scaled[nt][0] = scaled[nt][1] = 1.0f;
       }
+      best[nt][0] = best[nt][1] = -INFINITY;
 #pragma unroll
       for (int m = 0; m < M; ++m)
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-          best[c & 1] = fmaxf(best[c & 1], x[m][nt][c]);
+        for (int col = 0; col < 2; ++col)
+          best[nt][col] = fmaxf(best[nt][col], fmaxf(x[m][nt][col], x[m][nt][col + 2]));
 #pragma unroll
       for (int col = 0; col < 2; ++col) {
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1)
-          best[col] = fmaxf(best[col], __shfl_xor_sync(0xffffffffu, best[col], o));
-        // the reference moves only where a score has outgrown it by 2^8
-        const float higher = best[col] > top[nt][col] + kHeadroom ? best[col] : top[nt][col];
-        any_moved |= higher + shift != top[nt][col] + shift_before;
-        moved[nt][col] = higher == -INFINITY ? 1.0f : exp2_approx((top[nt][col] + shift_before) - (higher + shift));
-        top[nt][col] = higher;
+        best[nt][col] = best[nt][col] == -INFINITY ? -INFINITY : best[nt][col] * scaled[nt][col];
+        outgrown |= best[nt][col] > top[nt][col] + kHeadroom;
       }
-#pragma unroll
-      for (int m = 0; m < M; ++m)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) // a row that has seen nothing: 2^(-inf - 0)
-          x[m][nt][c] = exp2_approx(x[m][nt][c] - (top[nt][c & 1] == -INFINITY ? 0.0f : top[nt][c & 1] + shift));
     }
-    if (__any_sync(0xffffffffu, any_moved)) {
+    if (__any_sync(0xffffffffu, outgrown)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        sum[nt][0] *= moved[nt][0];
-        sum[nt][1] *= moved[nt][1];
+        float moved[2];
+#pragma unroll
+        for (int col = 0; col < 2; ++col) {
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1)
+            best[nt][col] = fmaxf(best[nt][col], __shfl_xor_sync(0xffffffffu, best[nt][col], o));
+          const float higher = best[nt][col] > top[nt][col] + kHeadroom ? best[nt][col] : top[nt][col];
+          moved[col] = higher == -INFINITY ? 1.0f : exp2_approx((top[nt][col] + shift_before) - (higher + shift));
+          top[nt][col] = higher;
+          sum[nt][col] *= moved[col];
+        }
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
           for (int c = 0; c < 4; ++c)
-            out[mt][nt][c] *= moved[nt][c & 1];
+            out[mt][nt][c] *= moved[c & 1];
       }
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const float minus[2] = {top[nt][0] == -INFINITY ? 0.0f : -(top[nt][0] + shift), top[nt][1] == -INFINITY ? 0.0f : -(top[nt][1] + shift)};
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) // a row that has seen nothing: 2^(-inf - 0)
+          x[m][nt][c] = exp2_approx(__fmaf_rn(x[m][nt][c], scaled[nt][c & 1], minus[c & 1]));
     }
     if constexpr (!Q4) {
 #pragma unroll
@@ -581,7 +616,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
       }
     }
     __syncwarp();
-    issue();
+    issue_keys();
   }
   if (!ok) // copies already requested still write into this CTA's shared memory
     for (int n = max(0, issued - S::slots); n < issued; ++n)
