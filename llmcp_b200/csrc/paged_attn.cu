@@ -10,14 +10,14 @@ namespace llmcp_b200 {
 
 namespace {
 
-// One CTA per (row, head): groups of head_dim / 8 threads take the chunks in turn.
+// One CTA per (row, head) and 64 dimensions: 32 groups of 8 threads take the chunks in turn, so that a row of many chunks
+// is not longer on its way than a few of their loads.
 template <int D>
 __global__ void __launch_bounds__(256)
 paged_merge_kernel(PagedKv kv, PagedBatch batch, PagedAttention call, PagedSplit split) {
-  constexpr int kLanes = D / 8, kGroups = 256 / kLanes;
   __shared__ float weights[kMaxChunks];
   __shared__ float tops[8], totals[8];
-  __shared__ float4 parts[kGroups][kLanes][2];
+  __shared__ float4 parts[8][8][2];
   const int token = blockIdx.x, head = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   grid_dependency_sync();
   const int b = paged_owner(batch, token);
@@ -31,6 +31,20 @@ paged_merge_kernel(PagedKv kv, PagedBatch batch, PagedAttention call, PagedSplit
   const int used = max(1, (sees + split.chunk - 1) / split.chunk);
   const int64_t row = (static_cast<int64_t>(token) * call.heads + head) * split.chunks;
   const float2 *sums = paged_part_sums(call, batch.tokens, split.chunks, D) + row;
+  // the first parts are on their way before their weights are known
+  const int d = blockIdx.z * 64 + tid % 8 * 8, group = tid / 8;
+  const float4 *src = reinterpret_cast<const float4 *>(static_cast<const float *>(call.workspace) + row * D + d);
+  constexpr int kAhead = 4;
+  float4 first[kAhead][2];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    const int c = group + 32 * i;
+    first[i][0] = first[i][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (c < used) {
+      first[i][0] = src[static_cast<int64_t>(c) * (D / 4)];
+      first[i][1] = src[static_cast<int64_t>(c) * (D / 4) + 1];
+    }
+  }
   float2 mine[kMaxChunks / 256];
   float top = -INFINITY;
 #pragma unroll
@@ -60,55 +74,126 @@ paged_merge_kernel(PagedKv kv, PagedBatch batch, PagedAttention call, PagedSplit
   if (lane == 0)
     totals[warp] = total;
   __syncthreads();
-  const int d = tid % kLanes * 8;
-  const float *src = static_cast<const float *>(call.workspace) + row * D + d;
-  float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f), y = x;
-  auto add = [](float4 &to, const float4 &v, float w) {
-    to.x = __fmaf_rn(v.x, w, to.x), to.y = __fmaf_rn(v.y, w, to.y), to.z = __fmaf_rn(v.z, w, to.z), to.w = __fmaf_rn(v.w, w, to.w);
+  float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+  auto add = [&](float4 x, float4 y, float w) {
+    const float p[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      v[i] = __fmaf_rn(p[i], w, v[i]);
   };
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i)
+    if (group + 32 * i < used)
+      add(first[i][0], first[i][1], weights[group + 32 * i]);
 #pragma unroll 4
-  for (int c = tid / kLanes; c < used; c += kGroups) {
-    const float4 *part = reinterpret_cast<const float4 *>(src + static_cast<int64_t>(c) * D);
-    add(x, part[0], weights[c]);
-    add(y, part[1], weights[c]);
+  for (int c = group + 32 * kAhead; c < used; c += 32)
+    add(src[static_cast<int64_t>(c) * (D / 4)], src[static_cast<int64_t>(c) * (D / 4) + 1], weights[c]);
+#pragma unroll
+  for (int o = 8; o < 32; o <<= 1)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+  if (lane < 8) {
+    parts[warp][lane][0] = make_float4(v[0], v[1], v[2], v[3]);
+    parts[warp][lane][1] = make_float4(v[4], v[5], v[6], v[7]);
   }
-  parts[tid / kLanes][tid % kLanes][0] = x;
-  parts[tid / kLanes][tid % kLanes][1] = y;
   __syncthreads();
-  if (tid < kLanes) {
-    for (int i = 1; i < kGroups; ++i) {
-      add(x, parts[i][tid][0], 1.0f);
-      add(y, parts[i][tid][1], 1.0f);
-    }
+  if (tid < 8) {
     total = 0.0f;
-    for (int w = 0; w < 8; ++w)
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
       total += totals[w];
+      if (w > 0)
+        add(parts[w][tid][0], parts[w][tid][1], 1.0f);
+    }
     const float inv = total == 0.0f ? 0.0f : __fdiv_rn(1.0f, total);
-    paged_store_row(call.out + paged_out_at<D>(call, token, head, d), make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv),
-                    make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv), paged_gate(call, token, head, d), call.gate != nullptr);
+    paged_store_row(call.out + paged_out_at<D>(call, token, head, d), make_float4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
+                    make_float4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv), paged_gate(call, token, head, d), call.gate != nullptr);
   }
+}
+
+// A warp per (row, head): for rows of at most 32 chunks, of which there are many.
+template <int D>
+__global__ void __launch_bounds__(256)
+paged_merge_few_kernel(PagedKv kv, PagedBatch batch, PagedAttention call, PagedSplit split) {
+  constexpr int E = D / 32; // dimensions of a lane
+  const int token = blockIdx.x, head = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  grid_dependency_sync();
+  if (head >= call.heads)
+    return;
+  const int b = paged_owner(batch, token);
+  if (b < 0)
+    return;
+  const PagedSequence s = paged_sequence(batch, kv.page_shift, b, nullptr);
+  if (s.count == 0)
+    return;
+  const int position = s.length - s.count + (token - s.first);
+  const int sees = max(0, min(s.length, max(position + 1, call.prefix ? call.prefix[b] : 0))); // chunks from there on are not written
+  const int used = max(1, (sees + split.chunk - 1) / split.chunk);
+  const int64_t row = (static_cast<int64_t>(token) * call.heads + head) * split.chunks;
+  const float2 mine = lane < used ? paged_part_sums(call, batch.tokens, split.chunks, D)[row + lane] : make_float2(-INFINITY, 0.0f);
+  const float *src = static_cast<const float *>(call.workspace) + row * D + lane * E;
+  float top = mine.x;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float weight = mine.x == -INFINITY ? 0.0f : exp2_approx(mine.x - top);
+  float total = weight * mine.y, v[E];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+#pragma unroll
+  for (int i = 0; i < E; ++i)
+    v[i] = 0.0f;
+#pragma unroll 4
+  for (int c = 0; c < used; ++c) {
+    const float w = __shfl_sync(0xffffffffu, weight, c);
+#pragma unroll
+    for (int i = 0; i < E; i += 2) {
+      const float2 part = *reinterpret_cast<const float2 *>(src + static_cast<int64_t>(c) * D + i);
+      v[i] = __fmaf_rn(part.x, w, v[i]);
+      v[i + 1] = __fmaf_rn(part.y, w, v[i + 1]);
+    }
+  }
+  const float inv = total == 0.0f ? 0.0f : __fdiv_rn(1.0f, total);
+  const int64_t to = paged_out_at<D>(call, token, head, lane * E);
+#pragma unroll
+  for (int i = 0; i < E; i += 2) {
+    float x = v[i] * inv, y = v[i + 1] * inv;
+    if (call.gate) {
+      const uint32_t gate = *reinterpret_cast<const uint32_t *>(call.gate + token * call.gate_row + head * call.gate_head + lane * E + i);
+      x = times_sigmoid(x, __uint_as_float(gate << 16));
+      y = times_sigmoid(y, __uint_as_float(gate & 0xffff0000u));
+    }
+    *reinterpret_cast<uint32_t *>(call.out + to + i) = f32x2_to_bf16x2_hw(x, y);
+  }
+}
+
+template <int D>
+cudaError_t merge(const PagedKv &kv, const PagedBatch &batch, const PagedAttention &call, const PagedSplit &split, cudaStream_t stream) {
+  // one sequence of 131001 tokens, 103 chunks of 16 rows: 4.0 us less by chunk groups; 96 x 3 rows of 20 heads, 4 chunks: 20 us less by warps
+  if (split.chunks <= 32 && static_cast<int64_t>(batch.tokens) * call.heads >= 256)
+    return launch_chained(paged_merge_few_kernel<D>, dim3(batch.tokens, (call.heads + 7) / 8), dim3(256), 0, stream, kv, batch, call, split);
+  return launch_chained(paged_merge_kernel<D>, dim3(batch.tokens, call.heads, D / 64), dim3(256), 0, stream, kv, batch, call, split);
 }
 
 } // namespace
 
 cudaError_t launch_paged_merge(const PagedKv &kv, const PagedBatch &batch, const PagedAttention &call, const PagedSplit &split, cudaStream_t stream) {
-  const dim3 grid(batch.tokens, call.heads);
-  switch (kv.head_dim) {
-  case 64:
-    return launch_chained(paged_merge_kernel<64>, grid, dim3(256), 0, stream, kv, batch, call, split);
-  case 128:
-    return launch_chained(paged_merge_kernel<128>, grid, dim3(256), 0, stream, kv, batch, call, split);
-  default:
-    return launch_chained(paged_merge_kernel<256>, grid, dim3(256), 0, stream, kv, batch, call, split);
-  }
+  return kv.head_dim == 64 ? merge<64>(kv, batch, call, split, stream) : kv.head_dim == 128 ? merge<128>(kv, batch, call, split, stream)
+                                                                                             : merge<256>(kv, batch, call, split, stream);
 }
 
-// Chunks of whole CTA tiles.  One sequence: as many as the SMs hold at a time (131001 keys in 4 bits: 53 us with two or
-// three per SM, 62 with six).  Several: more and shorter ones, which even out their lengths (64 sequences of 2000 to
-// 8000 keys, bf16: 242 us with two per SM, 222 with six, 212 with eight).
+// Chunks of whole CTA tiles, so many for every SM.  One sequence: as many as an SM holds at a time, 2 over bf16 pages and 3
+// over 4 bits (30001 keys in bf16: 27 us with 2, 30 with 4, 38 with 8; 131001 in 4 bits: 44 us with 3, 52 with 4).  A few
+// sequences: 2, or 4 over 4 bits (16 of 1000 to 4000 keys in 4 bits: 27 us with 3, 24 with 4, 30 with 6).  So many that
+// their key heads alone fill the SMs: 8, which evens out their lengths (64 of 2000 to 8000 keys in bf16: 231 us with 4,
+// 217 with 6, 212 with 8, 211 with 12; 96 x 3 rows of 1250 to 5000 in 4 bits: 104, 103, 90, 92).
 PagedSplit paged_rows_split(const PagedKv &kv, const PagedBatch &batch, int rows, int sms) {
   const int64_t tile = paged_rows_tile(kv, rows), tiles = (batch.max_kv + tile - 1) / tile;
-  const int64_t wanted = static_cast<int64_t>(sms) * (batch.sequences == 1 ? 3 : 8);
+  const bool q4 = kv.scales != nullptr;
+  const int64_t per_sm = batch.sequences == 1 ? (q4 ? 3 : 2) : static_cast<int64_t>(batch.sequences) * kv.kv_heads < sms ? (q4 ? 4 : 2) : 8;
+  const int64_t wanted = sms * per_sm;
   const int64_t each = (tiles * batch.sequences * kv.kv_heads + wanted - 1) / wanted;
   const int64_t most = (tiles + kMaxChunks - 1) / kMaxChunks;
   const int64_t chunk = each > most ? each : most;
