@@ -238,22 +238,28 @@ int llmcp_dev_gated_delta_net_noalloc(const uint16_t *conv, const uint16_t *a, c
  *                              in f64, rounded once.  q goes to q_out [tokens][heads][head_dim]; k and v to their
  *                              pages, in 4 bits as d = f16(min(max |y| / 7, 65504)), code = round-to-even(y / d) held to
  *                              -7 .. 7 per 32 dimensions.  heads may be 0 (keys and values only).  rot: a multiple of head_dim / 16.
- *                              No two rows of a call may have the same place in the cache.
+ *                              No two rows of a call may have the same place in the cache.  q_out may be q where q is laid out
+ *                              like it.
  *   llmcp_dev_paged_read     : the cached keys and values of the batch's rows as f32 or bf16 (out_dtype 0 or 1),
- *                              k_out and v_out [tokens][kv_heads][head_dim].  max_q = max_kv reads whole sequences.
+ *                              k_out and v_out [tokens][kv_heads][head_dim].  max_q = max_kv reads whole sequences.  Rows that no
+ *                              sequence has, or whose page does not exist, are left as they are.
  *   llmcp_dev_paged_attention: the second half (LowerAttention.cpp:266-601): out [tokens][heads][head_dim] bf16 =
  *                              softmax(score) v * sigmoid(gate).  score = q k scale; softcap > 0: softcap *
  *                              tanh(score / softcap); slopes ([heads] f32, may be null): minus slope * |p - j| for the
  *                              key j of a row at position p.  Keys j <= p are seen, and j < prefix[b] where prefix ([sequences] int32) is
  *                              given, none from kv_len on; a row that sees none gets zeros.  gate (may be null): bf16 with
- *                              strides.  heads: a multiple of kv_heads.  Products on the tensor cores, sums and softmax in
+ *                              strides.  Rows of q and gate start on 16-byte boundaries, their strides are positive.  heads: a
+ *                              multiple of kv_heads, at most 128 times as many.  Products on the tensor cores, sums and softmax in
  *                              f32.  What the pages hold from kv_len on has no influence, whatever it is; the keys and
- *                              values before it have to be finite.  workspace: device memory of
+ *                              values before it have to be finite.  max_q (times heads / kv_heads: up to 16 rows or more) decides
+ *                              between two kernels; prompts over 4 bits want a workspace of all sequences' rows in 16
+ *                              bits, sequences * 2 * kv_heads * max_kv of them, fewer than 2^31.  workspace: device memory of
  *                              llmcp_dev_paged_attention_workspace bytes (-1 on error; depends on the host's figures only) that no other call uses
  *                              meanwhile, captured graphs that may run at the same time included; needs no clearing.
  * status (device int, may be null; not cleared): bit 1 is raised if a bounded wait inside a kernel ran out (out is then
  * incomplete), bit 4 if lengths or page indices do not fit the figures above: sequences whose lengths do not fit are left out (their
- * rows of out unwritten), a token whose page does not exist is not stored, and counts as zeros in attention. */
+ * rows of out unwritten), a token whose page does not exist or whose position cos and sin do not have is not stored, and
+ * one without a page counts as zeros in attention. */
 typedef struct llmcp_b200_paged_kv {
   void *pages;
   uint16_t *scales;

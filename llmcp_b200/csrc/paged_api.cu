@@ -131,9 +131,13 @@ extern "C" int llmcp_dev_paged_read(const llmcp_b200_paged_kv *kv, const llmcp_b
 }
 
 namespace {
-int checked_heads(const PagedKv &c, int64_t heads) {
+int checked_heads(const PagedKv &c, const PagedBatch &b, int64_t heads) {
   require(heads >= 1 && heads <= 16384 && heads % c.kv_heads == 0, "heads has to be a multiple of kv_heads, at most 16384");
   require(heads / c.kv_heads <= 128, "at most 128 query heads share a key head");
+  // prompts over 4 bits work on rows of 16 bits, numbered in 31 bits too
+  require(!c.scales || b.max_q * (heads / c.kv_heads) <= 16 ||
+              static_cast<int64_t>(b.sequences) * 2 * c.kv_heads * ((b.max_kv + int64_t(127)) / 128 * 128) < (int64_t(1) << 31),
+          "sequences * 2 * kv_heads * max_kv has to stay below 2^31 for prompts over 4 bits; make several calls");
   return static_cast<int>(heads);
 }
 } // namespace
@@ -143,7 +147,7 @@ extern "C" int64_t llmcp_dev_paged_attention_workspace(const llmcp_b200_paged_kv
   entry([&] {
     const PagedKv c = to_kv(kv);
     const PagedBatch b = to_batch(batch);
-    const int h = checked_heads(c, heads);
+    const int h = checked_heads(c, b, heads);
     if (nothing(b)) {
       bytes = 0;
       return;
@@ -162,13 +166,19 @@ extern "C" int llmcp_dev_paged_attention(const llmcp_b200_paged_kv *kv, const ll
   return entry([&] {
     const PagedKv c = to_kv(kv);
     const PagedBatch b = to_batch(batch);
-    const int h = checked_heads(c, heads);
+    const int h = checked_heads(c, b, heads);
     require(std::isfinite(scale) && std::isfinite(softcap) && softcap >= 0.0f, "scale and softcap have to be finite, softcap not negative");
     if (nothing(b))
       return;
     require(q && out, "q or out is missing");
+    // the stride of a dimension with one entry means nothing
+    if (b.tokens == 1)
+      q_row = gate_row = int64_t(8);
+    if (h == 1)
+      q_head = gate_head = int64_t(8);
     require(on(q, 16) && q_row % 8 == 0 && q_head % 8 == 0 && on(out, 16) && on(gate, 16) && (!gate || (gate_row % 8 == 0 && gate_head % 8 == 0)),
             "rows of q, gate and out have to start on 16-byte boundaries");
+    require(q_row > 0 && q_head > 0 && (!gate || (gate_row > 0 && gate_head > 0)), "strides of q and gate have to be positive");
     require(on(slopes, 4) && on(prefix, 4), "slopes and prefix have to start on one of their elements");
     int sms = 0;
     check(current_sm_count(&sms), "paged attention");

@@ -452,9 +452,7 @@ cudaError_t launch_paged_tile(const PagedKv &kv, const PagedBatch &batch, const 
   if (f16) {
     p.expanded_rows = expanded_rows(batch);
     p.box_rows = KT;
-    rows = static_cast<int64_t>(batch.sequences) * 2 * kv.kv_heads * p.expanded_rows;
-    if (rows > (int64_t(1) << 31) - 1)
-      return cudaErrorInvalidValue;
+    rows = static_cast<int64_t>(batch.sequences) * 2 * kv.kv_heads * p.expanded_rows; // the entry has seen that they are less than 2^31
     source.pages = static_cast<uint8_t *>(call.workspace) + (paged_parts_bytes(kv, batch, call.heads, split) + 255) / 256 * 256;
     source.scales = nullptr;
     const cudaError_t e = kv.head_dim == 64 ? expand<64>(kv, batch, source.pages, status, stream) : kv.head_dim == 128 ? expand<128>(kv, batch, source.pages, status, stream)

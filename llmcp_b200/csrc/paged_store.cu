@@ -318,6 +318,7 @@ __device__ __forceinline__ void store_heads(Place &place, Row<E> row, int heads,
         // and n are off by 2 of themselves, which makes y's 2 |x c| + 3 |p| + |y| <= 5 |p| + 3 |y|; inv is off by 9.7 (sum
         // of squares of exact terms, mean and eps: E + 7, at most 15, half of which is left by the root; rsqrt 2.2) and its
         // product by 1 more.  And |y| for the interval's ends; the last percents are for the bound's own rounding.
+        bool sure = true;
         float inv = 1.0f, of_y = 2.03f / 16777216.0f, p_to_y = 0.51f;
         if (weight) {
           uint64_t squares = mul2(unpacked(row.w[0]), unpacked(row.w[0]));
@@ -331,8 +332,9 @@ __device__ __forceinline__ void store_heads(Place &place, Row<E> row, int heads,
           asm("rsqrt.approx.f32 %0, %1;" : "=f"(inv) : "f"(sum * (1.0f / D) + eps));
           of_y = inv * (15.0f / 16777216.0f);
           p_to_y = 0.35f;
+          // squares that overflow, or vanish beside an eps of 0, are f64's
+          sure = sum >= 0x1p-80f && sum <= 0x1p120f;
         }
-        bool sure = true;
         Row<E> done;
 #pragma unroll
         for (int i = 0; i < E / 2; ++i) {

@@ -473,3 +473,138 @@ def test_a_call_on_another_stream_follows_that_stream():
         second = paged.attention(cache, call, late)
     side.synchronize()
     assert torch.equal(first, second)
+
+
+def test_append_in_place_and_rows_past_the_range_of_f32():
+    """q_out may be q; rows whose squares leave f32's range, zeros without eps, infinities and NaN are as the definition has them."""
+    heads, dim, rot = 3, 128, 128
+    g = torch.Generator().manual_seed(8)
+    size = torch.tensor([1.0, 1e-30, 1e-38, 1e25, 2e37, 0.0, 1.0, 1.0])
+    batch = [(8, 20)]
+    q_start, kv_len, table, count = R.tables(batch, 16, 0, 1)
+    for eps in (1e-6, 0.0):
+        x = (torch.randn(8, heads, dim, generator=g) * size[:, None, None]).to(BF)
+        x[6, :, 5], x[7, :, 70] = math.inf, math.nan
+        weight = (0.2 * torch.randn(dim, generator=g)).to(BF)
+        angle = torch.rand(20, rot // 2, generator=g) * 6
+        cos, sin = (torch.cat((f(angle), f(angle)), 1).contiguous() for f in (torch.cos, torch.sin))
+        want = R.bf16_round(R.rotate(x, weight, cos[12:], sin[12:], eps))
+        pages, _ = empty_cache(count, heads, 16, dim, 16)
+        cache, call, q = paged.Cache(pages), make_batch(q_start, kv_len, table, batch), x.cuda()
+        got = paged.append(cache, call, q, *cuda(x, x, cos, sin), q_norm=weight.cuda(), k_norm=weight.cuda(), eps=eps, q_out=q)
+        assert got is q
+        k, v = paged.read(cache, call, 8)
+        assert torch.equal(v.cpu().view(torch.int16), x.view(torch.int16))
+        for y in (q, k):
+            assert torch.equal(y.cpu().isnan(), want.isnan())
+            assert torch.equal(y.cpu().double().nan_to_num(), want.nan_to_num())
+
+
+@pytest.mark.parametrize("rows", [1, 3, 60])
+@pytest.mark.parametrize("heads,groups,dim,bits", [(8, 2, 256, 16), (4, 2, 64, 4), (6, 2, 128, 4), (1, 1, 128, 16)])
+def test_attention_of_queries_with_strides(rows, heads, groups, dim, bits):
+    """Queries and gates as the projection leaves them, and with tokens next to each other, give what dense ones give."""
+    batch = [(rows, 200), (rows, 61)]
+    q_start, kv_len, table, count = R.tables(batch, 32, 1, 2)
+    pages, scales, _ = filled_cache(3, batch, table, count, groups, 32, dim, bits)
+    cache, call = paged.Cache(pages, scales), make_batch(q_start, kv_len, table, batch)
+    qg = torch.randn(2 * rows, heads, 2, dim, generator=torch.Generator().manual_seed(1)).to(BF).cuda()
+    dense = paged.attention(cache, call, qg[:, :, 0].contiguous(), gate=qg[:, :, 1].contiguous())
+    assert torch.equal(paged.attention(cache, call, qg[:, :, 0], gate=qg[:, :, 1]), dense)
+    turned = qg.permute(2, 1, 0, 3).contiguous()  # [2, heads, tokens, dim]
+    assert torch.equal(paged.attention(cache, call, turned[0].transpose(0, 1), gate=turned[1].transpose(0, 1)), dense)
+    assert torch.equal(paged.attention(cache, call, turned[0].transpose(0, 1), gate=qg[:, :, 1]), dense)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("heads,groups,dim", [(128, 1, 64), (128, 1, 256), (256, 2, 128), (96, 2, 64), (33, 1, 256), (17, 1, 128)])
+def test_attention_many_heads_on_one_key(heads, groups, dim, bits):
+    check_attention([(1, 150), (3, 40)], heads, groups, dim, bits, 32, gate=True)
+
+
+def test_workspaces_that_are_refused():
+    batch = [(1, 5000)]
+    q_start, kv_len, table, count = R.tables(batch, 64, 0, 1)
+    pages, scales, _ = filled_cache(1, batch, table, count, 2, 64, 64, 16)
+    cache, call = paged.Cache(pages, scales), make_batch(q_start, kv_len, table, batch)
+    q = torch.randn(1, 4, 64, generator=torch.Generator().manual_seed(1)).to(BF).cuda()
+    size = paged.workspace_bytes(cache, call, 1, 4)
+    assert size > 16  # one row over many keys is split
+    whole = torch.empty(size + 16, dtype=torch.uint8, device="cuda")
+    for bad in (whole[:size - 1], whole[8:], whole[:0]):
+        with pytest.raises(L.LlmcpError, match="workspace"):
+            paged.attention(cache, call, q, workspace=bad)
+    assert torch.equal(paged.attention(cache, call, q, workspace=whole[:size]), paged.attention(cache, call, q))
+
+
+@pytest.mark.parametrize("dim,bits", [(64, 16), (128, 4), (256, 16), (256, 4)])
+def test_prompts_in_captured_graphs(dim, bits):
+    """The pieces of prompts of changing lengths through one captured append and attention, twice at the same time on two
+    streams with workspaces of their own."""
+    heads, groups, size, most = 4, 2, 32, 400
+    g = torch.Generator().manual_seed(4)
+    _, _, table, count = R.tables([(1, most)] * 3, size, 0, 8)
+    start, lengths = torch.zeros(4, dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    tokens, states = 160, []
+    for _ in range(2):
+        pages, scales = empty_cache(count, groups, size, dim, bits)
+        x = [torch.zeros(tokens, h, dim, dtype=BF, device="cuda") for h in (heads, groups, groups)]
+        cache, call = paged.Cache(pages, scales), paged.Batch(start, lengths, cuda(table), 150, most)
+        ws = torch.full((paged.workspace_bytes(cache, call, tokens, heads) + 16,), 0xFF, dtype=torch.uint8, device="cuda")
+        out, status = torch.full((tokens, heads, dim), 7.0, dtype=BF, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+        paged.attention(cache, call, paged.append(cache, call, *x, status=status), out=out, workspace=ws, status=status)  # loads the kernels
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            paged.attention(cache, call, paged.append(cache, call, *x, status=status), out=out, workspace=ws, status=status)
+        states.append((graph, x, out, cache, call, ws, status))
+    values, held, side = torch.zeros(count, 2, groups, size, dim), [0, 0, 0], torch.cuda.Stream()
+    for news in ((100, 1, 40), (1, 150, 0), (3, 2, 77), (0, 0, 0), (150, 5, 5)):
+        held = [t + n for t, n in zip(held, news)]
+        starts = [0, *torch.tensor(news).cumsum(0).tolist()]
+        start.copy_(torch.tensor(starts, dtype=torch.int32))
+        lengths.copy_(torch.tensor(held, dtype=torch.int32))
+        fresh = [torch.randn(tokens, h, dim, generator=g).to(BF) for h in (heads, groups, groups)]
+        for _, x, out, *_ in states:
+            out.fill_(7.0)
+            for a, b in zip(x, fresh):
+                a.copy_(b)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            states[1][0].replay()
+        states[0][0].replay()
+        torch.cuda.synchronize()
+        for b, (n, t) in enumerate(zip(news, held)):
+            j = torch.arange(t - n, t)
+            for which in (0, 1):
+                rows = fresh[1 + which][starts[b]:starts[b + 1]].double()
+                if bits == 4:
+                    codes, d = R.quantise(rows)
+                    rows = (codes.unflatten(-1, (-1, 32)) * d.double()[..., None]).flatten(-2)
+                values[table[b, j // size].long(), which, :, j % size] = rows.float()
+        used = starts[-1]
+        want, weight, reach = R.attention(fresh[0][:used], values, starts, held, table, dim ** -0.5)
+        for _, _, out, *_, status in states:
+            assert int(status) == 0
+            assert ((out[:used].cpu().double() - want).abs() <= R.attention_bound(want, weight, reach, bits)).all()
+            assert (out[used:] == 7.0).all()
+
+
+@pytest.mark.parametrize("rows,bits", [(1, 4), (200, 4), (200, 16)])
+def test_two_calls_at_once(rows, bits):
+    """Calls on two streams whose workspaces come from torch's allocator do not touch each other's."""
+    batch = [(rows, 3000), (rows, 1234)]
+    q_start, kv_len, table, count = R.tables(batch, 64, 0, 1)
+    pages, scales, _ = filled_cache(1, batch, table, count, 2, 64, 128, bits)
+    cache, call = paged.Cache(pages, scales), make_batch(q_start, kv_len, table, batch)
+    queries = [torch.randn(2 * rows, 8, 128, generator=torch.Generator().manual_seed(s)).to(BF).cuda() for s in range(2)]
+    want = [paged.attention(cache, call, q) for q in queries]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(10):
+        for q, stream, results in zip(queries, streams, got):
+            with torch.cuda.stream(stream):
+                results.append(paged.attention(cache, call, q))
+    torch.cuda.synchronize()
+    for w, results in zip(want, got):
+        assert all(torch.equal(w, r) for r in results)

@@ -123,3 +123,19 @@ def test_reference_attention_is_a_softmax():
     mask = torch.ones(5, total, dtype=torch.bool).tril(total - 5)
     want = torch.nn.functional.scaled_dot_product_attention(q.double().transpose(0, 1), k, v, attn_mask=mask, scale=0.125)
     assert torch.allclose(out, want.transpose(0, 1), rtol=1e-12, atol=1e-12) and (weight >= out.abs() - 1e-12).all()
+
+
+@pytest.mark.parametrize("change", [dict(q_row=0), dict(q_head=0), dict(q_row=-256), dict(gate=FAKE, gate_row=256, gate_head=0),
+                                    dict(gate=FAKE, gate_row=0, gate_head=64)])
+def test_rows_of_queries_and_gates_that_overlap_are_refused(change):
+    _refused(_attention(_kv(), _batch(), **change), "positive")
+
+
+def test_prompts_over_4_bits_have_a_limit():
+    """Their rows of 16 bits are numbered in 31 bits: refused, for the call and for its workspace, where they are more; few
+    rows, and bf16 pages, have no such copy."""
+    kv, long = _kv(scales=FAKE), dict(max_kv=1 << 29, table_width=1 << 25, table_stride=1 << 25)
+    _refused(_attention(kv, _batch(max_q=9, **long)), "below 2^31")
+    assert paged._library().llmcp_dev_paged_attention_workspace(kv, _batch(max_q=9, **long), 4) == -1
+    assert "below 2^31" in L.last_error()
+    L.lib().llmcp_b200_clear_error()
