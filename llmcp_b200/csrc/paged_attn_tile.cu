@@ -427,9 +427,11 @@ PagedSplit paged_tile_split(const PagedKv &kv, const PagedBatch &batch, int head
   const int64_t ctas = static_cast<int64_t>((batch.max_q + per_cta - 1) / per_cta) * kv.kv_heads * batch.sequences;
   const int64_t tiles = (batch.max_kv + KT - 1) / KT;
   // Pieces of at least four tiles, as many as the SMs take at a time.  64 rows of 16 heads of 256 over 4000 keys: 28 us with
-  // eight tiles and more, 23 with four, 23 with two; 60 of 32 heads of 128 over 1000, twice: 21, 16, 19.
+  // eight tiles and more, 23 with four, 23 with two; 60 of 32 heads of 128 over 1000, twice: 21, 16, 19.  Of at least eight
+  // where a piece's sums take more than 4 MB to write and read again: 512 of 32 heads of 128, 20 us with four, 15 with eight.
+  const int64_t least = static_cast<int64_t>(batch.tokens) * heads * kv.head_dim * 4 > 4 << 20 ? 8 : 4;
   int64_t pieces = static_cast<int64_t>(sms) * (kv.head_dim == D ? 1 : 2) / ctas;
-  pieces = pieces > tiles / 4 ? tiles / 4 : pieces;
+  pieces = pieces > tiles / least ? tiles / least : pieces;
   pieces = pieces > kMaxChunks ? kMaxChunks : pieces;
   if (pieces <= 1)
     return PagedSplit{batch.max_kv > 0 ? static_cast<int>(tiles * KT) : 1, 1};
