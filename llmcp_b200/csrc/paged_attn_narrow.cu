@@ -7,7 +7,9 @@
 // A tile of 64 keys costs 512 cycles of exponentials (16 a cycle, less what the multipliers take over) and, at 128
 // dimensions, 640 cycles of products: the scores' operands both come from shared memory, 128 bytes a cycle.
 //
-//   warps 0-3  softmax;  4  MMA issue (one thread);  5  TMA loads;  6  zeroes the rows of the last value tile past the sequence.
+//   warps 0-3  softmax;  4  MMA issue (one thread);  5  TMA loads of queries, keys and gates;  6  of values, the last of which
+//   it gives zeros past the sequence.  (An item costs its warp some 1100 cycles,
+//   the wait for its slot and the issue of its boxes among them; one warp for both bound every tile.)
 
 #include "paged_attn_tc.cuh"
 
@@ -19,7 +21,7 @@ using namespace tc;
 
 constexpr int KT = 64;
 
-constexpr int kMmaWarp = 4, kLoadWarp = 5, kTailWarp = 6, kThreads = 224;
+constexpr int kMmaWarp = 4, kLoadWarp = 5, kValueWarp = 6, kThreads = 224;
 
 template <int D> struct Shape {
   static constexpr int slabs = D / 64;
@@ -100,25 +102,19 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap map_values, const __grid
   tc_fence_after();
   const uint32_t tmem = bars.tmem_base;
 
-  if (warp == kLoadWarp) {
-    // ---- loader: K0 K1 V0 K2 V1 ... as the MMAs take them; a box per lane -----------------------------------------------------------
+  // ---- loaders: a warp for the keys, one for the values; K0 K1 V0 K2 V1 ... as the MMAs take them, a box per lane ------------------
+  int issued = -1; // this warp's last item of the ring
+  auto load_tiles = [&](int which) {
     const int sub_boxes = KT / p.box_rows;
     const int slab = lane / sub_boxes, sub = lane % sub_boxes;
     const int32_t *table = p.batch.page_table + b * p.batch.table_stride;
-    const int ahead = min(2, tiles);
-    int issued = 0, keys_issued = 0, values_issued = 0;
     bool ok = true;
-    const int slab_bytes = p.tokens_per_tile * p.group * 128, token_first = seq.first + token0, head0 = kvh * p.group;
-    if (lane == 0) {
-      mbar_expect_tx(&bars.q_here, S::slabs * slab_bytes);
-      for (int k = 0; k < S::slabs; ++k)
-        load_slab(q_sm + k * (kRows * 128), &maps.queries, k * 64, head0, token_first, &bars.q_here);
-    }
-    for (int n = 0; n < 2 * tiles && ok; ++n) {
-      const int which = keys_issued < tiles && keys_issued - values_issued < ahead ? 0 : 1;
-      const int i = which ? values_issued++ : keys_issued++;
+    for (int i = 0; i < tiles; ++i) {
+      const int n = which ? (i == tiles - 1 ? 2 * tiles - 1 : 2 * i + 2) : max(0, 2 * i - 1);
       const int row = tile_box_row(p, seq, table, b, kvh, which, key0 + i * KT + sub * p.box_rows, slab < S::slabs, status);
       const int s = n % S::slots;
+      // Parity tells a phase from its neighbours only; the one before is over: for a warp's own items because it waited for
+      // them, for the last values (in a slot of keys) because those before them have been there.
       if (n >= S::slots)
         ok = __all_sync(0xffffffffu, mbar_wait<false>(&bars.empty[s], (n / S::slots - 1) & 1, abort_flag, p.spin_limit));
       if (!ok)
@@ -126,10 +122,25 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap map_values, const __grid
       if (lane == 0)
         mbar_expect_tx(&bars.full[s], S::slot_bytes);
       __syncwarp();
-      issued = n + 1;
+      issued = n;
       if (slab < S::slabs)
         tma_load_2d(ring + s * S::slot_bytes + (slab * KT + sub * p.box_rows) * 128, &map_values, slab * 64, row, &bars.full[s]);
     }
+    return ok;
+  };
+  auto wait_for_copies = [&]() { // after an abort: they still write into this CTA's shared memory
+    for (int n = max(0, issued - S::slots + 1); n <= issued; ++n)
+      mbar_wait_quiet<false>(&bars.full[n % S::slots], (n / S::slots) & 1, p.spin_limit);
+  };
+
+  if (warp == kLoadWarp) {
+    const int slab_bytes = p.tokens_per_tile * p.group * 128, token_first = seq.first + token0, head0 = kvh * p.group;
+    if (lane == 0) {
+      mbar_expect_tx(&bars.q_here, S::slabs * slab_bytes);
+      for (int k = 0; k < S::slabs; ++k)
+        load_slab(q_sm + k * (kRows * 128), &maps.queries, k * 64, head0, token_first, &bars.q_here);
+    }
+    const bool ok = load_tiles(0);
     // the gates take the queries' place, once the last keys' product is done (or nobody has wanted them)
     bool gates = false;
     if (ok && p.call.gate && p.chunks == 1) {
@@ -146,8 +157,7 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap map_values, const __grid
       mbar_wait_quiet<false>(&bars.q_here, 0, p.spin_limit);
       if (gates)
         mbar_wait_quiet<false>(&bars.gates_here, 0, p.spin_limit);
-      for (int n = max(0, issued - S::slots); n < issued; ++n)
-        mbar_wait_quiet<false>(&bars.full[n % S::slots], (n / S::slots) & 1, p.spin_limit);
+      wait_for_copies();
     }
   } else if (warp == kMmaWarp) {
     // ---- MMA issue: one thread ---------------------------------------------------------------------------------------------------
@@ -204,13 +214,16 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap map_values, const __grid
         mma_commit(&bars.o_full);
     }
     __syncwarp();
-  } else if (warp == kTailWarp) {
+  } else if (warp == kValueWarp) {
+    load_tiles(1);
     const int past = seq.length - key0 - (tiles - 1) * KT;
     if (tiles > 0 && past < KT && __all_sync(0xffffffffu, mbar_wait<false>(&bars.tail_here, 0, abort_flag, p.spin_limit))) {
       zero_tail<KT, S::slabs>(ring + (2 * tiles - 1) % S::slots * S::slot_bytes, past, lane);
       if (lane == 0)
         mbar_arrive(&bars.tail_ready);
     }
+    if (*abort_flag)
+      wait_for_copies();
   } else {
     // ---- softmax: a thread per row -----------------------------------------------------------------------------------------------
     const int row = warp * 32 + lane;

@@ -14,8 +14,9 @@
 //              warps that share 32 rows, through shared memory; the exponentials of two tiles run side by side.
 //   warp 8     one thread issues the MMAs: Q and P from tensor memory, K (K-major) and V (MN-major: rows are keys) from
 //              shared memory, both with the 128-byte swizzle.  Scores are issued two tiles ahead of P V.
-//   warp 9     issues the TMA loads into a ring of tiles, in the order in which the MMAs take them: K0 K1 V0 K2 V1 ...
-//   warp 10    zeroes the rows of the last value tile that lie past the sequence: 0 times whatever they hold is not 0.
+//   warps 9, 10  issue the TMA loads of keys (and queries and gates) and of values into a ring of tiles, in the order in
+//              which the MMAs take them: K0 K1 V0 K2 V1 ...  Warp 10 zeroes the rows of the last value tile that lie past
+//              the sequence, too: 0 times whatever they hold is not 0.
 // Queries come in as whole rows through ring slots that are not in use yet, results leave as whole rows through the ring.
 //
 // Every wait on a barrier is bounded; one that runs out raises a flag that all roles observe, the loader waits (bounded)
@@ -37,7 +38,7 @@ constexpr size_t kSmem = 1024 + static_cast<size_t>(kSlots) * kSlotBytes;
 // Tensor memory, in columns: two score buffers, O, Q.
 constexpr int kOColumn = 2 * KT, kQColumn = kOColumn + D;
 static_assert(kQColumn + D / 2 <= 512, "tensor memory");
-constexpr int kSoftmaxWarps = 8, kMmaWarp = 8, kLoadWarp = 9, kTailWarp = 10, kThreads = 352;
+constexpr int kSoftmaxWarps = 8, kMmaWarp = 8, kLoadWarp = 9, kValueWarp = 10, kThreads = 352;
 
 struct Barriers {
   uint64_t full[kSlots], empty[kSlots]; // a tile of keys or values
@@ -109,47 +110,68 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
   tc_fence_after();
   const uint32_t tmem = bars.tmem_base;
 
-  if (warp == kLoadWarp) {
-    // ---- loader: K0 K1 V0 K2 V1 ... as the MMAs take them; a box per lane -----------------------------------------------------------
+  // ---- loaders: a warp for the keys, one for the values; K0 K1 V0 K2 V1 ... as the MMAs take them, a box per lane ------------------
+  int issued = -1; // this warp's last item of the ring
+  // Parity tells a phase from its neighbours only; the one before is over: for a warp's own items because it waited for them,
+  // for the last values (in a slot of keys) and the gates because the items before them have been there.
+  auto slot_free = [&](int n, bool others) {
+    bool ok = true;
+    if (others) // these slots may still hold the queries
+      ok = __all_sync(0xffffffffu, mbar_wait<false>(&bars.q_full, 0, abort_flag, p.spin_limit));
+    if (ok && n >= kSlots)
+      ok = __all_sync(0xffffffffu, mbar_wait<false>(&bars.empty[n % kSlots], (n / kSlots - 1) & 1, abort_flag, p.spin_limit));
+    return ok;
+  };
+  auto load_tiles = [&](int which) {
     const int sub_boxes = KT / p.box_rows;
     const int slab = lane / sub_boxes, sub = lane % sub_boxes;
     const int32_t *table = p.batch.page_table + b * p.batch.table_stride;
-    const int ahead = min(2, tiles);
-    int issued = 0, keys_issued = 0, values_issued = 0;
     bool ok = true;
+    for (int i = 0; i < tiles && ok; ++i) {
+      const int n = which ? (i == tiles - 1 ? 2 * tiles - 1 : 2 * i + 2) : max(0, 2 * i - 1);
+      const int row = tile_box_row(p, seq, table, b, kvh, which, key0 + i * KT + sub * p.box_rows, slab < kSlabs, status);
+      ok = slot_free(n, n >= kQSlot && n < kSlots);
+      if (!ok)
+        break;
+      const int s = n % kSlots;
+      if (lane == 0)
+        mbar_expect_tx(&bars.full[s], kSlotBytes);
+      __syncwarp();
+      issued = n;
+      if (slab < kSlabs)
+        tma_load_2d(ring + s * kSlotBytes + (slab * KT + sub * p.box_rows) * 128, &map_values, slab * 64, row, &bars.full[s]);
+    }
+    return ok;
+  };
+  auto wait_for_copies = [&]() { // after an abort: they still write into this CTA's shared memory
+    for (int n = max(0, issued - kSlots + 1); n <= issued; ++n)
+      mbar_wait_quiet<false>(&bars.full[n % kSlots], (n / kSlots) & 1, p.spin_limit);
+  };
+
+  if (warp == kLoadWarp) {
     const int slab_bytes = p.tokens_per_tile * p.group * 128, token_first = seq.first + token0, head0 = kvh * p.group;
     if (lane == 0) {
       mbar_expect_tx(&bars.q_here, kSlabs * slab_bytes);
       for (int k = 0; k < kSlabs; ++k)
         load_slab(ring + kQSlot * kSlotBytes + k * (kRows * 128), &maps.queries, k * 64, head0, token_first, &bars.q_here);
     }
-    const bool gated = p.call.gate && p.chunks == 1;
-    for (int n = 0; n < 2 * tiles + (gated ? 2 : 0) && ok; ++n) { // the gates are the last two items: half of the dimensions each
-      const bool gates = n >= 2 * tiles;
-      const int which = keys_issued < tiles && keys_issued - values_issued < ahead ? 0 : 1;
-      const int i = which ? values_issued++ : keys_issued++;
-      const int row = tile_box_row(p, seq, table, b, kvh, which, key0 + i * KT + sub * p.box_rows, !gates && slab < kSlabs, status);
-      const int s = n % kSlots;
-      if (n == kQSlot || (gates && n == 2 * tiles)) // these slots may still hold the queries
-        ok = __all_sync(0xffffffffu, mbar_wait<false>(&bars.q_full, 0, abort_flag, p.spin_limit));
-      if (ok && n >= kSlots)
-        ok = __all_sync(0xffffffffu, mbar_wait<false>(&bars.empty[s], (n / kSlots - 1) & 1, abort_flag, p.spin_limit));
-      if (!ok)
-        break;
-      if (lane == 0)
-        mbar_expect_tx(&bars.full[s], gates ? kSlabs / 2 * slab_bytes : kSlotBytes);
-      __syncwarp();
-      issued = n + 1;
-      if (gates) {
+    bool ok = load_tiles(0);
+    if (p.call.gate && p.chunks == 1)
+      for (int half = 0; half < 2 && ok; ++half) { // the gates are the last two items: half of the dimensions each
+        const int n = 2 * tiles + half, s = n % kSlots;
+        ok = slot_free(n, half == 0);
+        if (!ok)
+          break;
+        if (lane == 0)
+          mbar_expect_tx(&bars.full[s], kSlabs / 2 * slab_bytes);
+        __syncwarp();
+        issued = n;
         if (lane < kSlabs / 2)
-          load_slab(ring + s * kSlotBytes + lane * (kRows * 128), &maps.gates, (n - 2 * tiles) * (D / 2) + lane * 64, head0, token_first, &bars.full[s]);
-      } else if (slab < kSlabs)
-        tma_load_2d(ring + s * kSlotBytes + (slab * KT + sub * p.box_rows) * 128, &map_values, slab * 64, row, &bars.full[s]);
-    }
-    if (*abort_flag) { // copies already requested still write into this CTA's shared memory
+          load_slab(ring + s * kSlotBytes + lane * (kRows * 128), &maps.gates, half * (D / 2) + lane * 64, head0, token_first, &bars.full[s]);
+      }
+    if (*abort_flag) {
       mbar_wait_quiet<false>(&bars.q_here, 0, p.spin_limit);
-      for (int n = max(0, issued - kSlots); n < issued; ++n)
-        mbar_wait_quiet<false>(&bars.full[n % kSlots], (n / kSlots) & 1, p.spin_limit);
+      wait_for_copies();
     }
   } else if (warp == kMmaWarp) {
     // ---- MMA issue: one thread ---------------------------------------------------------------------------------------------------
@@ -206,13 +228,16 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
         mma_commit(&bars.o_full);
     }
     __syncwarp();
-  } else if (warp == kTailWarp) {
+  } else if (warp == kValueWarp) {
+    load_tiles(1);
     const int past = seq.length - key0 - (tiles - 1) * KT;
     if (tiles > 0 && past < KT && __all_sync(0xffffffffu, mbar_wait<false>(&bars.tail_here, 0, abort_flag, p.spin_limit))) {
       zero_tail<KT, kSlabs>(ring + (2 * tiles - 1) % kSlots * kSlotBytes, past, lane);
       if (lane == 0)
         mbar_arrive(&bars.tail_ready);
     }
+    if (*abort_flag)
+      wait_for_copies();
   } else {
     // ---- softmax: a thread per row -----------------------------------------------------------------------------------------------
     const int half = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
