@@ -374,48 +374,53 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
 }
 
 // A 4-bit cache's rows of the batch's sequences as f16 / 8: [sequence][keys, values][kv head][rows][D], zeros from a
-// sequence's length to the end of its last tile.  A warp takes a row of a head's keys or values per lane group.
+// sequence's length to the end of its last tile.
 template <int DIM>
 __global__ void __launch_bounds__(256)
 paged_expand_kernel(PagedKv kv, PagedBatch batch, uint4 *__restrict__ out, int64_t rows, int *__restrict__ status) {
-  constexpr int kLanes = DIM / 32; // a block of 32 dimensions (16 bytes of codes) per thread
+  constexpr int kLanes = DIM / 8, kAhead = 4; // eight dimensions (4 bytes of codes, 16 bytes out) per thread, of four keys at a time
   grid_dependency_sync();
   const int b = blockIdx.z, which = blockIdx.y / kv.kv_heads, head = blockIdx.y % kv.kv_heads;
   const PagedSequence s = paged_sequence(batch, kv.page_shift, b, nullptr);
   if (s.count == 0)
     return;
   const int padded = (s.length + 127) / 128 * 128;
-  for (int64_t u = blockIdx.x * static_cast<int64_t>(256) + threadIdx.x; u < static_cast<int64_t>(padded) * kLanes; u += static_cast<int64_t>(gridDim.x) * 256) {
-    const int key = static_cast<int>(u / kLanes), block = static_cast<int>(u % kLanes);
-    uint4 codes = make_uint4(0, 0, 0, 0);
-    uint32_t scale = 0;
-    if (key < s.length) {
-      const int64_t row = paged_row(kv, batch, b, key, which, head);
-      if (row >= 0) {
-        codes = *reinterpret_cast<const uint4 *>(kv.pages + row * (DIM / 2) + block * 16);
-        scale = kv.scales[row * (DIM / 32) + block];
-      } else if (status) {
-        atomicOr(status, kStatusBadBatch);
+  const int piece = threadIdx.x % kLanes, step = gridDim.x * (256 / kLanes);
+  uint4 *to = out + (((static_cast<int64_t>(b) * 2 + which) * kv.kv_heads + head) * rows) * kLanes + piece;
+  const uint8_t *from = kv.pages + piece * 4;
+  const uint16_t *scales = kv.scales + piece / 4;
+  for (int first = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes; first < padded; first += kAhead * step) {
+    uint32_t codes[kAhead], scale[kAhead];
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      const int key = first + a * step;
+      codes[a] = scale[a] = 0;
+      if (key < s.length) {
+        const int64_t row = paged_row(kv, batch, b, key, which, head);
+        if (row >= 0) {
+          codes[a] = *reinterpret_cast<const uint32_t *>(from + row * (DIM / 2));
+          scale[a] = scales[row * (DIM / 32)];
+        } else if (status) {
+          atomicOr(status, kStatusBadBatch);
+        }
       }
     }
-    uint32_t d2; // scale / 8 twice
-    const uint32_t pair = scale | scale << 16, eighth = 0x30003000u;
-    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d2) : "r"(pair), "r"(eighth));
-    const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
-    uint4 *dst = out + (((static_cast<int64_t>(b) * 2 + which) * kv.kv_heads + head) * rows + key) * (DIM / 8) + block * 4;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      // code + 8 in the low bits of 1024, 1024 off again: exact; nibbles n and n + 4 come together
-      uint32_t v[4], r[4];
+    for (int a = 0; a < kAhead; ++a) {
+      const int key = first + a * step;
+      if (key >= padded)
+        break;
+      uint32_t d2, v[4]; // d2: scale / 8 twice
+      const uint32_t pair = scale[a] | scale[a] << 16, eighth = 0x30003000u;
+      asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d2) : "r"(pair), "r"(eighth));
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
-        const uint32_t biased = (w[i] >> (4 * n) & 0x000f000fu) | 0x64006400u, offset = 0x64086408u;
+        // code + 8 in the low bits of 1024, 1024 off again: exact; nibbles n and n + 4 come together
+        const uint32_t biased = (codes[a] >> (4 * n) & 0x000f000fu) | 0x64006400u, offset = 0x64086408u;
         asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(v[n]) : "r"(biased), "r"(offset));
         asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(v[n]) : "r"(v[n]), "r"(d2));
       }
-      r[0] = __byte_perm(v[0], v[1], 0x5410), r[1] = __byte_perm(v[2], v[3], 0x5410);
-      r[2] = __byte_perm(v[0], v[1], 0x7632), r[3] = __byte_perm(v[2], v[3], 0x7632);
-      dst[i] = make_uint4(r[0], r[1], r[2], r[3]);
+      to[static_cast<int64_t>(key) * kLanes] = make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632));
     }
   }
 }
@@ -429,7 +434,7 @@ size_t expanded_bytes(const PagedKv &kv, const PagedBatch &batch) {
 // Rows of keys and values as 16 bits: the pages themselves, or an expanded copy in the workspace.
 template <int DIM>
 cudaError_t expand(const PagedKv &kv, const PagedBatch &batch, uint8_t *to, int *status, cudaStream_t stream) {
-  const int64_t rows = expanded_rows(batch), blocks = (rows * (DIM / 32) + 255) / 256;
+  const int64_t rows = expanded_rows(batch), blocks = (rows * (DIM / 8) + 1023) / 1024; // a turn of the kernel's loop each
   return launch_chained(paged_expand_kernel<DIM>, dim3(static_cast<unsigned>(blocks < 4096 ? blocks : 4096), 2 * kv.kv_heads, batch.sequences), dim3(256), 0, stream,
                         kv, batch, reinterpret_cast<uint4 *>(to), rows, status);
 }
