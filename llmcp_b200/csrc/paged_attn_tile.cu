@@ -19,6 +19,9 @@
 //              the sequence, too: 0 times whatever they hold is not 0.
 // Queries come in as whole rows through ring slots that are not in use yet, results leave as whole rows through the ring.
 //
+// A key tile is 1024 cycles of products beside a softmax of about 1300; the gates' sigmoids and the results take 7 thousand
+// cycles a CTA.  4 prompts of 1024 to 2048 tokens of 16 heads, gated: 119 us, 735 TFLOP/s (141 us with one loading warp).
+//
 // Every wait on a barrier is bounded; one that runs out raises a flag that all roles observe, the loader waits (bounded)
 // for its copies in flight, tensor memory is released and the status bit is set.
 
@@ -374,7 +377,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
 }
 
 // A 4-bit cache's rows of the batch's sequences as f16 / 8: [sequence][keys, values][kv head][rows][D], zeros from a
-// sequence's length to the end of its last tile.
+// sequence's length to the end of its last tile.  16000 rows of 8 heads of 128: 22 us, of 13 that its bytes take.
 template <int DIM>
 __global__ void __launch_bounds__(256)
 paged_expand_kernel(PagedKv kv, PagedBatch batch, uint4 *__restrict__ out, int64_t rows, int *__restrict__ status) {
