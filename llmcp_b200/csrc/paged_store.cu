@@ -90,54 +90,24 @@ template <int E> __device__ __forceinline__ float value_at(const Row<E> &r, int 
   return __uint_as_float(i & 1 ? r.w[i / 2] & 0xffff0000u : r.w[i / 2] << 16);
 }
 
-// A pair of f32 values, as the two-wide instructions take them.
-__device__ __forceinline__ uint64_t pair_of(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-
-__device__ __forceinline__ float2 parts_of(uint64_t a) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
-  return r;
-}
-
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-
 // The two bf16 values of a word.
-__device__ __forceinline__ uint64_t unpacked(uint32_t w) { return pair_of(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+__device__ __forceinline__ uint64_t unpacked(uint32_t w) { return pair(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
 
 // A lane's values to codes and their block's scale; 32 / E lanes share a block.
 template <int E> __device__ __forceinline__ uint32_t quantise(const Row<E> &r, uint16_t *scale) {
-  uint32_t pair = 0;
+  uint32_t largest = 0;
 #pragma unroll
   for (int i = 0; i < E / 2; ++i)
-    pair = __vmaxu2(pair, r.w[i] & 0x7fff7fffu);
+    largest = __vmaxu2(largest, r.w[i] & 0x7fff7fffu);
 #pragma unroll
   for (int o = 1; o < 32 / E; o <<= 1)
-    pair = __vmaxu2(pair, __shfl_xor_sync(0xffffffffu, pair, o));
-  const uint32_t top = max(pair & 0xffffu, pair >> 16);
+    largest = __vmaxu2(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+  const uint32_t top = max(largest & 0xffffu, largest >> 16);
   // Scales between the least normal f16 and 32768: top has 8 significant bits and a middle between two f16 values 12, so
   // top / 7 is at least 2^-15 of itself away from every middle and the product rounds as the quotient does; no |y| / d is
-  // above 7.01.  The product with the reciprocal is within 2^-22 of y / d, and with its remainder's share added it is y / d
-  // where that is half way between two codes (a seventh of all blocks has d = top / 7 exactly, and such quotients).
+  // above 7.01.  The product with the reciprocal is within 2^-22 of y / d; with its remainder's share added (a step of
+  // iterative refinement) it is y / d itself where that is half way between two codes.  (A seventh of all blocks has
+  // d = top / 7 exactly, and such quotients.)
   float d = __uint_as_float(top << 16) * (1.0f / 7.0f);
   const bool plain = top == 0 || (d >= 0x1p-14f && d < 32768.0f);
   uint16_t d16;
@@ -151,8 +121,8 @@ template <int E> __device__ __forceinline__ uint32_t quantise(const Row<E> &r, u
   uint32_t codes = 0, high = 0;
 #pragma unroll
   for (int i = 0; i < E / 2; ++i) {
-    const uint64_t y = unpacked(r.w[i]), z = mul2(y, pair_of(inv, inv));
-    const float2 t = parts_of(add2(fma2(fma2(z, pair_of(-d, -d), y), pair_of(inv, inv), z), pair_of(kRound, kRound)));
+    const uint64_t y = unpacked(r.w[i]), z = mul2(y, pair(inv, inv));
+    const float2 t = halves(add2(fma2(fma2(z, pair(-d, -d), y), pair(inv, inv), z), pair(kRound, kRound)));
     codes += (__float_as_uint(t.x) << (8 * i)) + (__float_as_uint(t.y) << (8 * i + 4));
     high += (__float_as_uint(kRound - 8.0f) << (8 * i)) + (__float_as_uint(kRound - 8.0f) << (8 * i + 4)); // a constant
   }
@@ -276,8 +246,8 @@ __device__ __forceinline__ Turn<E> turn_of(const Place &place, const float *cs, 
   Turn<E> r;
 #pragma unroll
   for (int i = 0; i < E / 2; ++i) {
-    r.c[i] = pair_of(c[2 * i], c[2 * i + 1]);
-    r.n[i] = pair_of(place.sign * n[2 * i], place.sign * n[2 * i + 1]);
+    r.c[i] = pair(c[2 * i], c[2 * i + 1]);
+    r.n[i] = pair(place.sign * n[2 * i], place.sign * n[2 * i + 1]);
   }
   return r;
 }
@@ -325,7 +295,7 @@ __device__ __forceinline__ void store_heads(Place &place, Row<E> row, int heads,
 #pragma unroll
           for (int i = 1; i < E / 2; ++i)
             squares = fma2(unpacked(row.w[i]), unpacked(row.w[i]), squares);
-          float sum = parts_of(squares).x + parts_of(squares).y;
+          float sum = halves(squares).x + halves(squares).y;
 #pragma unroll
           for (int o = kLanes / 2; o > 0; o >>= 1)
             sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -339,10 +309,10 @@ __device__ __forceinline__ void store_heads(Place &place, Row<E> row, int heads,
 #pragma unroll
         for (int i = 0; i < E / 2; ++i) {
           const uint64_t p = mul2(unpacked(__shfl_sync(0xffffffffu, row.w[i], lane + place.to_partner)), turn.n[i]);
-          const uint64_t y = fma2(unpacked(row.w[i]), turn.c[i], p), scaled = mul2(y, pair_of(inv, inv));
-          const float2 a = parts_of(p), z = parts_of(y);
-          const uint64_t off = pair_of(__fmaf_rn(fabsf(a.x), p_to_y, fabsf(z.x)), __fmaf_rn(fabsf(a.y), p_to_y, fabsf(z.y)));
-          const float2 up = parts_of(fma2(off, pair_of(of_y, of_y), scaled)), down = parts_of(fma2(off, pair_of(-of_y, -of_y), scaled));
+          const uint64_t y = fma2(unpacked(row.w[i]), turn.c[i], p), scaled = mul2(y, pair(inv, inv));
+          const float2 a = halves(p), z = halves(y);
+          const uint64_t off = pair(__fmaf_rn(fabsf(a.x), p_to_y, fabsf(z.x)), __fmaf_rn(fabsf(a.y), p_to_y, fabsf(z.y)));
+          const float2 up = halves(fma2(off, pair(of_y, of_y), scaled)), down = halves(fma2(off, pair(-of_y, -of_y), scaled));
           done.w[i] = f32x2_to_bf16x2_hw(up.x, up.y);
           sure &= done.w[i] == f32x2_to_bf16x2_hw(down.x, down.y);
         }
