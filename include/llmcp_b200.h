@@ -227,7 +227,8 @@ int llmcp_dev_gated_delta_net_noalloc(const uint16_t *conv, const uint16_t *a, c
  * and out (q_start ascending, from 0); they are the last tokens of the kv_len[b] it has, these included, so row i of n
  * has position kv_len - n + i.  Its token j lies in page page_table[b * table_stride + j / page_size] (table_width
  * entries a row).  The three arrays are int32 device memory and may change between replays of a captured call;
- * tokens (rows of q, k, v and out), max_q and max_kv bound them on the host: no sequence may have more rows or a greater kv_len.  Rows from
+ * tokens (rows of q, k, v and out), max_q and max_kv bound them on the host: no sequence may have more rows or a greater kv_len (wider
+ * bounds than tokens and table_width * page_size lay out no more than those).  Rows from
  * q_start[sequences] on are left as they are (padding).
  *
  *   llmcp_dev_paged_append   : the first half of llmcp.attention (LowerAttention.cpp:54-265) for a batch: q [tokens]

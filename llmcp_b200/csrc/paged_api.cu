@@ -1,5 +1,6 @@
 // C entry points of the paged key/value cache: every argument is checked here, before anything touches the GPU.
 
+#include <algorithm>
 #include <cmath>
 #include <stdexcept>
 #include <string>
@@ -41,7 +42,7 @@ PagedKv to_kv(const llmcp_b200_paged_kv *kv) {
                  static_cast<int>(kv->head_dim)};
 }
 
-PagedBatch to_batch(const llmcp_b200_paged_batch *b) {
+PagedBatch to_batch(const llmcp_b200_paged_batch *b, const PagedKv &kv) {
   require(b != nullptr, "no batch");
   constexpr int64_t most = int64_t(1) << 30; // arithmetic on positions and tiles stays in 31 bits
   require(b->sequences >= 0 && b->sequences <= 65535, "sequences has to be 0 to 65535");
@@ -60,7 +61,8 @@ PagedBatch to_batch(const llmcp_b200_paged_batch *b) {
   out.table_width = static_cast<int>(b->table_width);
   out.tokens = static_cast<int>(b->tokens);
   out.max_q = static_cast<int>(b->max_q);
-  out.max_kv = static_cast<int>(b->max_kv);
+  // no sequence has more keys than its pages hold: a wider bound would only lay out empty work
+  out.max_kv = static_cast<int>(std::min(b->max_kv, b->table_width << kv.page_shift));
   return out;
 }
 
@@ -92,7 +94,7 @@ extern "C" int llmcp_dev_paged_append(const llmcp_b200_paged_kv *kv, const llmcp
                                       void *stream) {
   return entry([&] {
     const PagedKv c = to_kv(kv);
-    const PagedBatch b = to_batch(batch);
+    const PagedBatch b = to_batch(batch, c);
     require(heads >= 0 && heads <= 16384, "heads has to be 0 to 16384");
     require(rot >= 0 && rot <= c.head_dim && rot % (c.head_dim / 16) == 0, "rot has to be a multiple of head_dim / 16, at most head_dim");
     require(cos_rows >= 0, "cos_rows is negative");
@@ -120,7 +122,7 @@ extern "C" int llmcp_dev_paged_read(const llmcp_b200_paged_kv *kv, const llmcp_b
                                     int out_dtype, int *status, void *stream) {
   return entry([&] {
     const PagedKv c = to_kv(kv);
-    const PagedBatch b = to_batch(batch);
+    const PagedBatch b = to_batch(batch, c);
     require(out_dtype == kF32 || out_dtype == kBF16, "out_dtype has to be 0 (f32) or 1 (bf16)");
     if (nothing(b))
       return;
@@ -146,7 +148,7 @@ extern "C" int64_t llmcp_dev_paged_attention_workspace(const llmcp_b200_paged_kv
   int64_t bytes = -1;
   entry([&] {
     const PagedKv c = to_kv(kv);
-    const PagedBatch b = to_batch(batch);
+    const PagedBatch b = to_batch(batch, c);
     const int h = checked_heads(c, b, heads);
     if (nothing(b)) {
       bytes = 0;
@@ -165,7 +167,7 @@ extern "C" int llmcp_dev_paged_attention(const llmcp_b200_paged_kv *kv, const ll
                                          void *workspace, int64_t workspace_bytes, int *status, void *stream) {
   return entry([&] {
     const PagedKv c = to_kv(kv);
-    const PagedBatch b = to_batch(batch);
+    const PagedBatch b = to_batch(batch, c);
     const int h = checked_heads(c, b, heads);
     require(std::isfinite(scale) && std::isfinite(softcap) && softcap >= 0.0f, "scale and softcap have to be finite, softcap not negative");
     if (nothing(b))

@@ -428,6 +428,11 @@ paged_expand_kernel(PagedKv kv, PagedBatch batch, uint4 *__restrict__ out, int64
   }
 }
 
+// Tiles of a sequence's rows; a bound past the call's rows would only lay out empty CTAs.
+int64_t row_tiles(const PagedBatch &batch, int per_tile) {
+  return (static_cast<int64_t>(batch.max_q < batch.tokens ? batch.max_q : batch.tokens) + per_tile - 1) / per_tile;
+}
+
 int64_t expanded_rows(const PagedBatch &batch) { return (static_cast<int64_t>(batch.max_kv) + 127) / 128 * 128; }
 
 size_t expanded_bytes(const PagedKv &kv, const PagedBatch &batch) {
@@ -456,8 +461,7 @@ size_t paged_tile_workspace(const PagedKv &kv, const PagedBatch &batch, int head
 }
 
 PagedSplit paged_tile_split(const PagedKv &kv, const PagedBatch &batch, int heads, int sms) {
-  const int per_cta = kRows / (heads / kv.kv_heads);
-  const int64_t ctas = static_cast<int64_t>((batch.max_q + per_cta - 1) / per_cta) * kv.kv_heads * batch.sequences;
+  const int64_t ctas = row_tiles(batch, kRows / (heads / kv.kv_heads)) * kv.kv_heads * batch.sequences;
   const int64_t tiles = (batch.max_kv + KT - 1) / KT;
   // Pieces of at least four tiles, as many as the SMs take at a time.  64 rows of 16 heads of 256 over 4000 keys: 28 us with
   // eight tiles and more, 23 with four, 23 with two; 60 of 32 heads of 128 over 1000, twice: 21, 16, 19.  Of at least eight
@@ -506,7 +510,7 @@ cudaError_t launch_paged_tile(const PagedKv &kv, const PagedBatch &batch, const 
   maps.gates = maps.queries;
   if (call.gate && !paged_rows_map(&maps.gates, call.gate, kv.head_dim, call.heads, batch.tokens, call.gate_head, call.gate_row, p.group, p.tokens_per_tile))
     return cudaErrorNotSupported;
-  const unsigned q_tiles = static_cast<unsigned>((batch.max_q + p.tokens_per_tile - 1) / p.tokens_per_tile);
+  const unsigned q_tiles = static_cast<unsigned>(row_tiles(batch, p.tokens_per_tile));
   if (kv.head_dim != D)
     return launch_paged_narrow(kv.head_dim, f16, values, maps, p, q_tiles, status, stream);
   return f16 ? launch_wide<true>(values, maps, p, q_tiles, status, stream) : launch_wide<false>(values, maps, p, q_tiles, status, stream);

@@ -608,3 +608,24 @@ def test_two_calls_at_once(rows, bits):
     torch.cuda.synchronize()
     for w, results in zip(want, got):
         assert all(torch.equal(w, r) for r in results)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("batch", [[(1, 1)], [(1, 300), (2, 40)], [(70, 300), (5, 40)]])
+def test_bounds_far_above_the_lengths(batch, bits):
+    """max_q and max_kv of 2^30 lay out no more than rows and pages allow, and the results are as ever."""
+    q_start, kv_len, table, count = R.tables(batch, 32, 0, 2)
+    pages, scales, values = filled_cache(3, batch, table, count, 2, 32, 128, bits)
+    tokens = int(q_start[-1])
+    q = torch.randn(tokens, 256, 128, generator=torch.Generator().manual_seed(1)).to(BF)
+    cache, call = paged.Cache(pages, scales), make_batch(q_start, kv_len, table, batch, max_q=1 << 30, max_kv=1 << 30)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for heads in (8, 256):
+        assert paged.workspace_bytes(cache, call, tokens, heads) < 1 << 28
+        got = paged.attention(cache, call, q[:, :heads].cuda(), status=status).cpu().double()
+        want, weight, reach = R.attention(q[:, :heads], values, q_start, kv_len, table, 128 ** -0.5)
+        assert int(status) == 0
+        assert ((got - want).abs() <= R.attention_bound(want, weight, reach, bits)).all()
+    k, v = paged.read(cache, call, tokens)
+    again = paged.read(cache, make_batch(q_start, kv_len, table, batch), tokens)
+    assert torch.equal(k, again[0]) and torch.equal(v, again[1])
