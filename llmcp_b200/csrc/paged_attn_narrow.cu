@@ -39,7 +39,7 @@ template <int D> struct Shape {
 
 template <int SLOTS> struct Barriers {
   uint64_t full[SLOTS], empty[SLOTS]; // a tile of keys or values
-  uint64_t q_here;                    // the queries have landed
+  uint64_t q_here;                    // the queries (and the divisors) have landed
   uint64_t q_full;                    // ... and are as the products take them
   uint64_t gates_here;
   uint64_t s_full[2];                 // [key tile & 1]: scores are in tensor memory
@@ -49,6 +49,7 @@ template <int SLOTS> struct Barriers {
   uint64_t tail_here, tail_ready;     // the last tile of a sequence's values has landed; its rows past the end are zeros
   uint32_t tmem_base;
   int abort_flag;
+  float divisors[2];                  // of the expanded keys and values
 };
 
 template <int D, bool F16>
@@ -74,7 +75,7 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap map_values, const __grid
       mbar_init(&bars.p_full[i], 4);
       mbar_init(&bars.o_done[i], 1);
     }
-    mbar_init(&bars.q_here, 1);
+    mbar_init(&bars.q_here, F16 ? 2 : 1);
     mbar_init(&bars.q_full, 4);
     mbar_init(&bars.gates_here, 1);
     mbar_init(&bars.o_full, 1);
@@ -219,6 +220,8 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap map_values, const __grid
     }
     __syncwarp();
   } else if (warp == kValueWarp) {
+    if constexpr (F16)
+      fetch_divisors(bars.divisors, p, b, kvh, lane, &bars.q_here);
     load_tiles(1);
     const int past = seq.length - key0 - (tiles - 1) * KT;
     if (tiles > 0 && past < KT && __all_sync(0xffffffffu, mbar_wait<false>(&bars.tail_here, 0, abort_flag, p.spin_limit))) {
@@ -246,7 +249,7 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap map_values, const __grid
       float multiplier = 1.0f, unscale = 1.0f;
       if constexpr (F16)
         multiplier = query_multiplier<D>(q_sm, row, negative, &unscale);
-      r.factor *= unscale;
+      r.factor *= F16 ? unscale * bars.divisors[0] : 1.0f;
 #pragma unroll 2
       for (int piece = 0; piece < D / 8; ++piece) {
         uint4 *at = reinterpret_cast<uint4 *>(q_sm + piece_at(row, piece));
@@ -305,8 +308,8 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap map_values, const __grid
       ok = all_wait(&bars.o_full, 0);
     if (ok) {
       tc_fence_after();
-      // f16 values are 1 / 8 of themselves; where a row has seen nothing O may hold anything
-      const float scale = (F16 ? 8.0f : 1.0f) * (p.chunks == 1 && sum != 0.0f ? __fdiv_rn(1.0f, sum) : 1.0f);
+      // where a row has seen nothing O may hold anything
+      const float scale = (F16 ? bars.divisors[1] : 1.0f) * (p.chunks == 1 && sum != 0.0f ? __fdiv_rn(1.0f, sum) : 1.0f);
       if (p.chunks == 1) {
         unload_row<D>(q_sm, row, lanes + S::o_column, scale, sum == 0.0f, gated);
       } else {

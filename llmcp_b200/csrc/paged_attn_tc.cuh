@@ -3,8 +3,8 @@
 //
 // In both, 128 rows (tokens x the query heads that share a key head) lie in the 128 lanes of tensor memory, a thread of a
 // warpgroup each, and scores S = Q K^T, weights P = 2^(S - reference) and O += P V are tcgen05 products.  Keys and values
-// are 16-bit tiles: bf16 from the pages, or f16 / 8 from an expanded 4-bit cache, whose factors go into the score and
-// the end; f16 queries are scaled by a power of two per row.
+// are 16-bit tiles: bf16 from the pages, or f16 from an expanded 4-bit cache (an eighth of the values where they are large,
+// taken back in the score and at the end); f16 queries are scaled by a power of two per row.
 #pragma once
 
 #include "common.cuh"
@@ -29,6 +29,7 @@ struct Tile {
   int tokens_per_tile;   // of 128 rows
   unsigned group, one_over_group; // query heads that share a key head; 2^16 / group rounded up
   int64_t expanded_rows; // rows of a sequence's keys in the expanded cache; 0: pages
+  const float *divisors; // [sequence][keys, values][kv head]: what the expanded values were divided by
   int out_of_range;      // a row coordinate past the last row: reads as zeros
   uint32_t spin_limit;
 };
@@ -317,7 +318,7 @@ __device__ __forceinline__ void copy_rows_out(uint16_t *to, int64_t token_stride
 }
 
 // f16 queries: the power of two that takes a row's largest |q| into [2^14, 2^15) (1 for a row of zeros), with the sign of
-// the scale; and what takes it back, with the keys' 1 / 8.
+// the scale; and what takes it back.
 template <int D> __device__ __forceinline__ float query_multiplier(const uint8_t *queries, int row, bool negative, float *unscale) {
   uint32_t top2 = 0;
 #pragma unroll 4
@@ -327,7 +328,7 @@ template <int D> __device__ __forceinline__ float query_multiplier(const uint8_t
   }
   const uint32_t top = max(top2 & 0xffffu, top2 >> 16);
   const int up = top == 0 ? 0 : min(126, 14 - (static_cast<int>(top >> 7) - 127));
-  *unscale = __int_as_float(min(254, 3 - up + 127) << 23);
+  *unscale = __int_as_float((127 - up) << 23);
   return __uint_as_float(static_cast<uint32_t>(up + 127) << 23 | (negative ? 0x80000000u : 0u));
 }
 
@@ -390,6 +391,15 @@ template <int DIMS> __device__ __forceinline__ void unload_part(float *to, uint3
                                                            : make_float4(__uint_as_float(o[u]) * scale, __uint_as_float(o[u + 1]) * scale,
                                                                          __uint_as_float(o[u + 2]) * scale, __uint_as_float(o[u + 3]) * scale);
   }
+}
+
+// What the keys and values of a head of the expanded cache were divided by, into shared memory; then `bar` is told.
+__device__ __forceinline__ void fetch_divisors(float (&to)[2], const Tile &p, int b, int kvh, int lane, uint64_t *bar) {
+  if (lane < 2)
+    to[lane] = p.divisors[(b * 2 + lane) * p.kv.kv_heads + kvh];
+  __syncwarp();
+  if (lane == 0)
+    mbar_arrive(bar);
 }
 
 // This lane's box of a tile of keys (which = 0) or values: its row coordinate.

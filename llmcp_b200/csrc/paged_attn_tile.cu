@@ -4,8 +4,11 @@
 //   S = Q K^T,  P = 2^(S scale log2 e - m),  O = sum P V / sum P,   128 rows (tokens x the query heads of one key head) a CTA
 //
 // Keys and values come as 16-bit tiles by TMA: bf16 straight from the pages; a 4-bit cache is expanded once per call into
-// f16 rows (paged_expand_kernel), value = code * scale / 8 rounded to f16 (2^-11; the 8 keeps the largest below f16's
-// end and goes into the factors), because every tile of rows would otherwise unpack the same keys again.
+// f16 rows (paged_expand_kernel), value = code * scale rounded to f16, because every tile of rows would otherwise unpack the
+// same keys again.  The rounding is 2^-11 for every scale, f16's subnormal ones too: a whole number of its steps stays one.
+// A sequence's head whose largest scale is 8192 or more (7 times that may leave f16) has its codes divided by 8 (exactly),
+// and its factors are that much larger; what a small block beside such a large one loses then is 2^-22, 2^-37 of the
+// largest value.  paged_largest_scale_kernel finds those.
 //
 // One CTA, 352 threads, all 512 columns of tensor memory (O 256, Q 128, two tiles of 64 scores):
 //   warps 0-7  softmax, a thread per row: warps 0-3 take the even key tiles, 4-7 the odd ones.  A thread reads its scores
@@ -49,12 +52,13 @@ struct Barriers {
   uint64_t p_full[2];                 // its weights are
   uint64_t o_full;                    // every tile's P V has been added
   uint64_t tail_here, tail_ready;     // the last tile of a sequence's values has landed; its rows past the end are zeros
-  uint64_t q_here;                    // the queries have landed
+  uint64_t q_here;                    // the queries (and the divisors) have landed
   uint64_t q_full;                    // ... and are in tensor memory
   uint64_t o_done[2];                 // [tile & 1]: P V of a tile has been added
   uint64_t reference[2][4];           // [tile & 1][32 rows]: the reference after a tile
   uint32_t tmem_base;
   int abort_flag;
+  float divisors[2];                  // of the expanded keys and values
 };
 
 template <bool F16>
@@ -84,7 +88,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
       for (int w = 0; w < 4; ++w)
         mbar_init(&bars.reference[i][w], 1);
     }
-    mbar_init(&bars.q_here, 1);
+    mbar_init(&bars.q_here, F16 ? 2 : 1);
     mbar_init(&bars.q_full, kSoftmaxWarps);
     bars.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -232,6 +236,8 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
     }
     __syncwarp();
   } else if (warp == kValueWarp) {
+    if constexpr (F16)
+      fetch_divisors(bars.divisors, p, b, kvh, lane, &bars.q_here);
     load_tiles(1);
     const int past = seq.length - key0 - (tiles - 1) * KT;
     if (tiles > 0 && past < KT && __all_sync(0xffffffffu, mbar_wait<false>(&bars.tail_here, 0, abort_flag, p.spin_limit))) {
@@ -258,7 +264,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
     float multiplier = 1.0f, unscale = 1.0f;
     if constexpr (F16)
       multiplier = query_multiplier<D>(staged, row, negative, &unscale);
-    factor *= unscale;
+    factor *= F16 ? unscale * bars.divisors[0] : 1.0f;
 #pragma unroll 1
     for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c) { // 32 dimensions = 16 columns at a time; half of them each
       uint32_t w[16];
@@ -346,8 +352,8 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         total += last_reference[h][row] == -INFINITY ? 0.0f : sums[h][row] * exp2_approx(last_reference[h][row] - final_reference);
-      // f16 values are 1 / 8 of themselves; where a row has seen nothing O may hold anything
-      const float scale = (F16 ? 8.0f : 1.0f) * (p.chunks == 1 && total != 0.0f ? __fdiv_rn(1.0f, total) : 1.0f);
+      // where a row has seen nothing O may hold anything
+      const float scale = (F16 ? bars.divisors[1] : 1.0f) * (p.chunks == 1 && total != 0.0f ? __fdiv_rn(1.0f, total) : 1.0f);
       const uint32_t o_at = lanes + kOColumn + half * (D / 2);
       if (p.chunks == 1) {
         unload_row<D / 2>(rows_out, row, o_at, scale, total == 0.0f, gated);
@@ -376,20 +382,74 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
     atomicOr(status, kStatusWaitRanOut);
 }
 
-// A 4-bit cache's rows of the batch's sequences as f16 / 8: [sequence][keys, values][kv head][rows][D], zeros from a
-// sequence's length to the end of its last tile.  16000 rows of 8 heads of 128: 22 us, of 13 that its bytes take.
+// The largest scale (its bits) of every sequence's keys and values by head, in `gridDim.x` parts: [sequence][keys, values]
+// [kv head][kScaleParts].
+constexpr int kScaleParts = 32;
+
 template <int DIM>
 __global__ void __launch_bounds__(256)
-paged_expand_kernel(PagedKv kv, PagedBatch batch, uint4 *__restrict__ out, int64_t rows, int *__restrict__ status) {
+paged_largest_scale_kernel(PagedKv kv, PagedBatch batch, uint32_t *__restrict__ out) {
+  constexpr int kWords = DIM / 64, kAhead = 4; // two scales to a word; a key per thread, four at a time
+  __shared__ uint32_t tops[8];
+  grid_dependency_sync();
+  const int b = blockIdx.z, which = blockIdx.y / kv.kv_heads, head = blockIdx.y % kv.kv_heads;
+  const PagedSequence s = paged_sequence(batch, kv.page_shift, b, nullptr);
+  if (s.count == 0)
+    return;
+  const uint32_t *scales = reinterpret_cast<const uint32_t *>(kv.scales);
+  const int step = gridDim.x * 256;
+  uint32_t top = 0;
+  for (int first = blockIdx.x * 256 + threadIdx.x; first < s.length; first += kAhead * step) {
+    int64_t row[kAhead];
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a)
+      row[a] = first + a * step < s.length ? paged_row(kv, batch, b, first + a * step, which, head) : -1;
+    uint32_t words[kAhead][kWords];
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+      for (int k = 0; k < kWords; ++k)
+        words[a][k] = row[a] >= 0 ? scales[row[a] * kWords + k] : 0;
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+      for (int k = 0; k < kWords; ++k)
+        top = __vmaxu2(top, words[a][k] & 0x7fff7fffu);
+  }
+  top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
+  if (threadIdx.x % 32 == 0)
+    tops[threadIdx.x / 32] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 8; ++w)
+      top = max(top, tops[w]);
+    out[((static_cast<int64_t>(b) * 2 + which) * kv.kv_heads + head) * kScaleParts + blockIdx.x] = top;
+  }
+}
+
+// A 4-bit cache's rows of the batch's sequences as f16: [sequence][keys, values][kv head][rows][D], zeros from a
+// sequence's length to the end of its last tile; an eighth of the values where the head's largest scale needs it.
+// 16000 rows of 8 heads of 128: 21 us, of 13 that its bytes take, after 6 us for the largest scales.
+template <int DIM>
+__global__ void __launch_bounds__(256)
+paged_expand_kernel(PagedKv kv, PagedBatch batch, uint4 *__restrict__ out, int64_t rows, const uint32_t *__restrict__ largest, int parts,
+                    float *__restrict__ divisors, int *__restrict__ status) {
   constexpr int kLanes = DIM / 8, kAhead = 4; // eight dimensions (4 bytes of codes, 16 bytes out) per thread, of four keys at a time
   grid_dependency_sync();
   const int b = blockIdx.z, which = blockIdx.y / kv.kv_heads, head = blockIdx.y % kv.kv_heads;
   const PagedSequence s = paged_sequence(batch, kv.page_shift, b, nullptr);
   if (s.count == 0)
     return;
+  const int64_t of_head = (static_cast<int64_t>(b) * 2 + which) * kv.kv_heads + head;
+  const int lane = threadIdx.x & 31;
+  const bool large = __reduce_max_sync(0xffffffffu, lane < parts ? largest[of_head * kScaleParts + lane] : 0) >= 0x7000; // 8192
+  if (blockIdx.x == 0 && threadIdx.x == 0)
+    divisors[of_head] = large ? 8.0f : 1.0f;
+  // code + 8 in the low bits of 1024, 1032 off again: exact; in those of 128 it is an eighth
+  const uint32_t base = large ? 0x58005800u : 0x64006400u, offset = base | 0x00080008u;
   const int padded = (s.length + 127) / 128 * 128;
   const int piece = threadIdx.x % kLanes, step = gridDim.x * (256 / kLanes);
-  uint4 *to = out + (((static_cast<int64_t>(b) * 2 + which) * kv.kv_heads + head) * rows) * kLanes + piece;
+  uint4 *to = out + of_head * rows * kLanes + piece;
   const uint8_t *from = kv.pages + piece * 4;
   const uint16_t *scales = kv.scales + piece / 4;
   for (int first = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes; first < padded; first += kAhead * step) {
@@ -413,13 +473,11 @@ paged_expand_kernel(PagedKv kv, PagedBatch batch, uint4 *__restrict__ out, int64
       const int key = first + a * step;
       if (key >= padded)
         break;
-      uint32_t d2, v[4]; // d2: scale / 8 twice
-      const uint32_t pair = scale[a] | scale[a] << 16, eighth = 0x30003000u;
-      asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d2) : "r"(pair), "r"(eighth));
+      const uint32_t d2 = scale[a] | scale[a] << 16;
+      uint32_t v[4];
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
-        // code + 8 in the low bits of 1024, 1024 off again: exact; nibbles n and n + 4 come together
-        const uint32_t biased = (codes[a] >> (4 * n) & 0x000f000fu) | 0x64006400u, offset = 0x64086408u;
+        const uint32_t biased = (codes[a] >> (4 * n) & 0x000f000fu) | base; // nibbles n and n + 4 come together
         asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(v[n]) : "r"(biased), "r"(offset));
         asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(v[n]) : "r"(v[n]), "r"(d2));
       }
@@ -439,12 +497,19 @@ size_t expanded_bytes(const PagedKv &kv, const PagedBatch &batch) {
   return kv.scales ? static_cast<size_t>(batch.sequences) * 2 * kv.kv_heads * expanded_rows(batch) * kv.head_dim * 2 : 0;
 }
 
-// Rows of keys and values as 16 bits: the pages themselves, or an expanded copy in the workspace.
+// Behind them: the largest scales' parts, and the divisors.
+int64_t expanded_heads(const PagedKv &kv, const PagedBatch &batch) { return kv.scales ? static_cast<int64_t>(batch.sequences) * 2 * kv.kv_heads : 0; }
+
+// The expanded copy in the workspace.
 template <int DIM>
-cudaError_t expand(const PagedKv &kv, const PagedBatch &batch, uint8_t *to, int *status, cudaStream_t stream) {
+cudaError_t expand(const PagedKv &kv, const PagedBatch &batch, uint8_t *to, uint32_t *largest, float *divisors, int *status, cudaStream_t stream) {
   const int64_t rows = expanded_rows(batch), blocks = (rows * (DIM / 8) + 1023) / 1024; // a turn of the kernel's loop each
-  return launch_chained(paged_expand_kernel<DIM>, dim3(static_cast<unsigned>(blocks < 4096 ? blocks : 4096), 2 * kv.kv_heads, batch.sequences), dim3(256), 0, stream,
-                        kv, batch, reinterpret_cast<uint4 *>(to), rows, status);
+  const unsigned heads = 2 * kv.kv_heads, sequences = batch.sequences;
+  const int parts = static_cast<int>(rows > kScaleParts * 1024 ? kScaleParts : (rows + 1023) / 1024); // likewise
+  if (cudaError_t e = launch_chained(paged_largest_scale_kernel<DIM>, dim3(parts, heads, sequences), dim3(256), 0, stream, kv, batch, largest); e != cudaSuccess)
+    return e;
+  return launch_chained(paged_expand_kernel<DIM>, dim3(static_cast<unsigned>(blocks < 4096 ? blocks : 4096), heads, sequences), dim3(256), 0, stream,
+                        kv, batch, reinterpret_cast<uint4 *>(to), rows, largest, parts, divisors, status);
 }
 
 template <bool F16> cudaError_t launch_wide(const CUtensorMap &values, const RowMaps &maps, const Tile &p, unsigned q_tiles, int *status, cudaStream_t stream) {
@@ -457,7 +522,8 @@ template <bool F16> cudaError_t launch_wide(const CUtensorMap &values, const Row
 } // namespace
 
 size_t paged_tile_workspace(const PagedKv &kv, const PagedBatch &batch, int heads, const PagedSplit &split) {
-  return (paged_parts_bytes(kv, batch, heads, split) + 255) / 256 * 256 + expanded_bytes(kv, batch);
+  return (paged_parts_bytes(kv, batch, heads, split) + 255) / 256 * 256 + expanded_bytes(kv, batch) +
+         expanded_heads(kv, batch) * (kScaleParts + 1) * sizeof(uint32_t);
 }
 
 PagedSplit paged_tile_split(const PagedKv &kv, const PagedBatch &batch, int heads, int sms) {
@@ -486,6 +552,7 @@ cudaError_t launch_paged_tile(const PagedKv &kv, const PagedBatch &batch, const 
   p.tokens_per_tile = kRows / p.group;
   p.spin_limit = kSpinLimit<false>;
   p.expanded_rows = 0;
+  p.divisors = nullptr;
   p.box_rows = KT < 1 << kv.page_shift ? KT : 1 << kv.page_shift;
   PagedKv source = kv;
   int64_t rows = kv.num_pages * 2 * kv.kv_heads << kv.page_shift;
@@ -495,9 +562,11 @@ cudaError_t launch_paged_tile(const PagedKv &kv, const PagedBatch &batch, const 
     rows = static_cast<int64_t>(batch.sequences) * 2 * kv.kv_heads * p.expanded_rows; // the entry has seen that they are less than 2^31
     source.pages = static_cast<uint8_t *>(call.workspace) + (paged_parts_bytes(kv, batch, call.heads, split) + 255) / 256 * 256;
     source.scales = nullptr;
-    const cudaError_t e = kv.head_dim == 64 ? expand<64>(kv, batch, source.pages, status, stream) : kv.head_dim == 128 ? expand<128>(kv, batch, source.pages, status, stream)
-                                                                                                  : expand<256>(kv, batch, source.pages, status, stream);
-    if (e != cudaSuccess)
+    uint32_t *largest = reinterpret_cast<uint32_t *>(source.pages + expanded_bytes(kv, batch));
+    float *divisors = reinterpret_cast<float *>(largest + expanded_heads(kv, batch) * kScaleParts);
+    p.divisors = divisors;
+    const auto run = kv.head_dim == 64 ? expand<64> : kv.head_dim == 128 ? expand<128> : expand<256>;
+    if (const cudaError_t e = run(kv, batch, source.pages, largest, divisors, status, stream); e != cudaSuccess)
       return e;
   }
   p.out_of_range = static_cast<int>(rows);

@@ -1,0 +1,63 @@
+"""The paged key/value cache at the ends of its ranges: sizes of values, gates and caps, positions past 2^24, rows without keys.
+Compared with plain 64-bit arithmetic (tests/paged_reference.py), as tests/test_gpu_paged.py is."""
+import math
+
+import pytest
+import torch
+
+import paged_reference as R
+from llmcp_b200 import paged
+from test_gpu_paged import BF, cuda, empty_cache, filled_cache, make_batch
+
+pytestmark = pytest.mark.gpu
+
+
+def pack(values):
+    """float64 [pages, 2, heads, size, dim] -> 4-bit (pages, scales, the values that they stand for) on the CPU."""
+    codes, d = R.quantise(R.bf16_round(values))
+    code8 = (codes + 8).to(torch.uint8)
+    return code8[..., 0::2] | code8[..., 1::2] << 4, d, (codes.unflatten(-1, (-1, 32)) * d.double()[..., None]).flatten(-2)
+
+
+def within(got, want, bound):
+    off = (got.cpu().double() - want).abs() / bound
+    assert not off.isnan().any() and off.max() <= 1, f"{off.max():.3f} of the bound"
+
+
+# ---- 4-bit values of any size --------------------------------------------------------------------------------------------
+
+STEPS, PROMPTS = [(1, 300), (2, 70), (1, 6000)], [(150, 333), (40, 41), (20, 4000)]
+SHAPES_4BIT = [(4, 2, 64), (6, 2, 128), (4, 1, 256)]
+
+
+@pytest.mark.parametrize("size", [1e-2, 1e-3, 1e-4, 1e-5, 2e-6, 1e5])
+@pytest.mark.parametrize("batch", [STEPS, PROMPTS], ids=["steps", "prompts"])
+@pytest.mark.parametrize("heads,groups,dim", SHAPES_4BIT)
+def test_attention_over_4_bit_values_of_any_size(heads, groups, dim, batch, size):
+    """From scales that are f16's last bits to values past f16's end; queries as much larger keep the scores' size."""
+    g = torch.Generator().manual_seed(dim)
+    q_start, kv_len, table, count = R.tables(batch, 64, 1, 5)
+    pages, scales, values = filled_cache(7, batch, table, count, groups, 64, dim, 4, scale=size)
+    q = (torch.randn(int(q_start[-1]), heads, dim, generator=g) / size).to(BF)
+    got = paged.attention(paged.Cache(pages, scales), make_batch(q_start, kv_len, table, batch), q.cuda())
+    want, weight, extent = R.attention(q, values, q_start, kv_len, table, dim ** -0.5)
+    within(got, want, R.attention_bound(want, weight, extent, 4))
+
+
+@pytest.mark.parametrize("largest", [3.0, 3e5])
+@pytest.mark.parametrize("batch", [STEPS, PROMPTS], ids=["steps", "prompts"])
+@pytest.mark.parametrize("heads,groups,dim", SHAPES_4BIT)
+def test_attention_over_4_bit_blocks_of_mixed_sizes(heads, groups, dim, batch, largest):
+    """Blocks between 1e-6 and `largest` side by side; only one sequence, one head, keys or values has the largest ones."""
+    g = torch.Generator().manual_seed(dim + 1)
+    q_start, kv_len, table, count = R.tables(batch, 64, 1, 5)
+    blocks = 10.0 ** (-6 + 6.4 * torch.rand(count, 2, groups, 64, dim // 32, 1, generator=g, dtype=torch.float64))
+    raw = (blocks * torch.rand(count, 2, groups, 64, dim // 32, 32, generator=g, dtype=torch.float64).sub(0.5)).flatten(-2)
+    raw[table[0, 2].long(), 1, groups - 1, 5] *= largest / raw[table[0, 2].long(), 1, groups - 1, 5].abs().max()
+    raw[table[1, 0].long(), 0, 0, 9] *= largest / raw[table[1, 0].long(), 0, 0, 9].abs().max()
+    pages, scales, values = pack(raw)
+    q = torch.randn(int(q_start[-1]), heads, dim, generator=g).to(BF)
+    scale = dim ** -0.5 / largest
+    got = paged.attention(paged.Cache(*cuda(pages, scales)), make_batch(q_start, kv_len, table, batch), q.cuda(), scale=scale)
+    want, weight, extent = R.attention(q, values, q_start, kv_len, table, scale)
+    within(got, want, R.attention_bound(want, weight, extent, 4))
