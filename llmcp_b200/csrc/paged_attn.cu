@@ -221,7 +221,7 @@ cudaError_t launch_paged_attention(const PagedKv &kv, const PagedBatch &batch, c
   const int rows = few_rows(kv, batch, call.heads);
   const PagedSplit split = rows ? paged_rows_split(kv, batch, rows, sms) : paged_tile_split(kv, batch, call.heads, sms);
   const cudaError_t e = rows ? launch_paged_rows(kv, batch, call, split, status, stream) : launch_paged_tile(kv, batch, call, split, status, stream);
-  *launches = rows || !kv.scales ? 1 : 3;
+  *launches = rows || !kv.scales || batch.max_kv == 0 ? 1 : 3;
   if (e != cudaSuccess || split.chunks == 1)
     return e;
   *launches += 1;

@@ -29,7 +29,7 @@ struct Tile {
   int tokens_per_tile;   // of 128 rows
   unsigned group, one_over_group; // query heads that share a key head; 2^16 / group rounded up
   int64_t expanded_rows; // rows of a sequence's keys in the expanded cache; 0: pages
-  const float *divisors; // [sequence][keys, values][kv head]: what the expanded values were divided by
+  const float *divisors; // [sequence][keys, values][kv head]: what the expanded values were divided by; null where there are none
   int out_of_range;      // a row coordinate past the last row: reads as zeros
   uint32_t spin_limit;
 };
@@ -396,7 +396,7 @@ template <int DIMS> __device__ __forceinline__ void unload_part(float *to, uint3
 // What the keys and values of a head of the expanded cache were divided by, into shared memory; then `bar` is told.
 __device__ __forceinline__ void fetch_divisors(float (&to)[2], const Tile &p, int b, int kvh, int lane, uint64_t *bar) {
   if (lane < 2)
-    to[lane] = p.divisors[(b * 2 + lane) * p.kv.kv_heads + kvh];
+    to[lane] = p.divisors ? p.divisors[(b * 2 + lane) * p.kv.kv_heads + kvh] : 1.0f;
   __syncwarp();
   if (lane == 0)
     mbar_arrive(bar);

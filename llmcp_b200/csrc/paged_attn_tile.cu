@@ -498,7 +498,7 @@ size_t expanded_bytes(const PagedKv &kv, const PagedBatch &batch) {
 }
 
 // Behind them: the largest scales' parts, and the divisors.
-int64_t expanded_heads(const PagedKv &kv, const PagedBatch &batch) { return kv.scales ? static_cast<int64_t>(batch.sequences) * 2 * kv.kv_heads : 0; }
+int64_t expanded_heads(const PagedKv &kv, const PagedBatch &batch) { return kv.scales && batch.max_kv > 0 ? static_cast<int64_t>(batch.sequences) * 2 * kv.kv_heads : 0; }
 
 // The expanded copy in the workspace.
 template <int DIM>
@@ -557,11 +557,14 @@ cudaError_t launch_paged_tile(const PagedKv &kv, const PagedBatch &batch, const 
   PagedKv source = kv;
   int64_t rows = kv.num_pages * 2 * kv.kv_heads << kv.page_shift;
   if (f16) {
-    p.expanded_rows = expanded_rows(batch);
     p.box_rows = KT;
+    source.scales = nullptr;
+    rows = 1; // without keys nothing is expanded, and no tile comes through the map
+  }
+  if (f16 && batch.max_kv > 0) {
+    p.expanded_rows = expanded_rows(batch);
     rows = static_cast<int64_t>(batch.sequences) * 2 * kv.kv_heads * p.expanded_rows; // the entry has seen that they are less than 2^31
     source.pages = static_cast<uint8_t *>(call.workspace) + (paged_parts_bytes(kv, batch, call.heads, split) + 255) / 256 * 256;
-    source.scales = nullptr;
     uint32_t *largest = reinterpret_cast<uint32_t *>(source.pages + expanded_bytes(kv, batch));
     float *divisors = reinterpret_cast<float *>(largest + expanded_heads(kv, batch) * kScaleParts);
     p.divisors = divisors;

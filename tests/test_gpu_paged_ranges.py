@@ -61,3 +61,23 @@ def test_attention_over_4_bit_blocks_of_mixed_sizes(heads, groups, dim, batch, l
     got = paged.attention(paged.Cache(*cuda(pages, scales)), make_batch(q_start, kv_len, table, batch), q.cuda(), scale=scale)
     want, weight, extent = R.attention(q, values, q_start, kv_len, table, scale)
     within(got, want, R.attention_bound(want, weight, extent, 4))
+
+
+# ---- rows without keys ---------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("width,most", [(0, 0), (0, 100), (4, 0)])
+def test_rows_of_sequences_without_keys_are_zeros(width, most, rows, dim, bits):
+    pages, scales = empty_cache(2, 2, 16, dim, bits)
+    starts, lengths = torch.tensor([0, rows, 2 * rows], dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    call = paged.Batch(*cuda(starts, lengths, torch.zeros(2, width, dtype=torch.int32)), rows, most)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    q = torch.randn(2 * rows + 1, 4, dim, device="cuda").to(BF)
+    for gate in (None, q):
+        out = torch.full_like(q, 7.0)
+        paged.attention(paged.Cache(pages, scales), call, q, gate=gate, out=out, status=status)
+        assert int(status) == 0
+        assert (out[:2 * rows] == 0).all() and (out[2 * rows:] == 7.0).all()
