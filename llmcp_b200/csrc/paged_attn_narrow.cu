@@ -263,7 +263,7 @@ paged_narrow_kernel(const __grid_constant__ CUtensorMap map_values, const __grid
     const int position = seq.length - seq.count + token0 + static_cast<int>(row / group);
     r.cap = p.call.softcap, r.over_cap = r.cap > 0.0f ? 1.0f / r.cap : 0.0f;
     r.biased = p.call.slopes != nullptr;
-    r.slope = r.biased && valid ? p.call.slopes[head0 + row % group] * 1.4426950408889634f : 0.0f, r.at = static_cast<float>(position);
+    r.slope = r.biased && valid ? p.call.slopes[head0 + row % group] * 1.4426950408889634f : 0.0f, r.at = position;
     r.sees = valid ? max(0, min(seq.length, max(position + 1, prefix))) : 0, r.sees_least = sees_least;
     float reference = -INFINITY, sum = 0.0f;
     for (int i = 0; i < tiles && ok; ++i) {

@@ -145,7 +145,8 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
   __shared__ uint64_t full[kWarps][S::slots];
   __shared__ float warp_max[kWarps][NT * 8], warp_sum[kWarps][NT * 8];
   __shared__ int sees[NT * 8];                       // keys below it
-  __shared__ float slope[NT * 8], at[NT * 8], unscales[NT * 8];
+  __shared__ float slope[NT * 8], unscales[NT * 8];
+  __shared__ int at[NT * 8]; // position
   __shared__ uint2 offsets_sm[Q4 ? NT : 1][32];
   __shared__ int failed;
   uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
@@ -307,7 +308,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
     const int position = seq.length - seq.count + tid / group;
     sees[tid] = tid < rows ? min(seq.length, max(position + 1, p.call.prefix ? p.call.prefix[b] : 0)) : seq.length;
     slope[tid] = p.call.slopes && tid < rows ? p.call.slopes[kvh * group + tid % group] * 1.4426950408889634f : 0.0f;
-    at[tid] = static_cast<float>(position);
+    at[tid] = position;
   }
   __syncthreads();
   uint32_t offsets[NT][2]; // 4 bits: what a block's scale is multiplied by to take the 8 off its codes, as f16 and its rest
@@ -496,12 +497,16 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
         scaled[nt][0] = scaled[nt][1] = 1.0f;
       }
       if (biased || masked) {
+        float from[2]; // distances to the lane's first key: whole numbers are exact to 2^24, positions go past it
+#pragma unroll
+        for (int col = 0; col < 2; ++col)
+          from[col] = static_cast<float>(at[nt * 8 + 2 * t + col] - j0 - g);
 #pragma unroll
         for (int m = 0; m < M; ++m)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const int j = j0 + m * 16 + g + (c >> 1) * 8, row = nt * 8 + 2 * t + (c & 1);
-            x[m][nt][c] = j < sees[row] ? x[m][nt][c] * scaled[nt][c & 1] - slope[row] * fabsf(at[row] - static_cast<float>(j)) : -INFINITY;
+            x[m][nt][c] = j < sees[row] ? x[m][nt][c] * scaled[nt][c & 1] - slope[row] * fabsf(from[c & 1] - static_cast<float>(m * 16 + (c >> 1) * 8)) : -INFINITY;
           }
         scaled[nt][0] = scaled[nt][1] = 1.0f;
       }

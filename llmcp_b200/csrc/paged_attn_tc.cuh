@@ -144,7 +144,8 @@ template <int KT> __device__ __forceinline__ void load_scores(uint32_t (&x)[KT /
 struct RowScores {
   float factor;        // to units of log 2, or (capped) to scores
   float cap, over_cap; // cap 0: none
-  float slope, at;     // bias by distance from position `at`
+  float slope;         // bias by distance from position `at`
+  int at;
   int sees, sees_least; // keys below: this row, every row of its tile
   bool biased;
 };
@@ -207,7 +208,7 @@ template <int KT> __device__ __forceinline__ float shape_scores(uint32_t (&x)[KT
     scaled = 1.0f;
   }
   if (r.biased) {
-    const float from = r.at - static_cast<float>(j0); // whole numbers: exact to 2^24
+    const float from = static_cast<float>(r.at - j0); // a distance: whole numbers are exact to 2^24, positions go past it
 #pragma unroll
     for (int c = 0; c < KT / 32; ++c)
 #pragma unroll

@@ -81,3 +81,24 @@ def test_rows_of_sequences_without_keys_are_zeros(width, most, rows, dim, bits):
         paged.attention(paged.Cache(pages, scales), call, q, gate=gate, out=out, status=status)
         assert int(status) == 0
         assert (out[:2 * rows] == 0).all() and (out[2 * rows:] == 7.0).all()
+
+
+# ---- positions that f32 does not hold --------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("rows,heads,dim,bits", [(1, 2, 64, 4), (3, 2, 64, 16), (1, 2, 256, 16), (20, 2, 64, 16), (20, 2, 256, 16)])
+def test_bias_by_distance_past_2_to_the_24_keys(rows, heads, dim, bits):
+    """The bias leaves nothing of keys some thousands away, so that the last ones are the whole answer."""
+    size, count, near = 256, 40, 4096
+    total = (1 << 24) + 2817
+    g = torch.Generator().manual_seed(dim + rows)
+    table = torch.randint(0, count, (1, -(-total // size)), generator=g, dtype=torch.int32)  # pages may be a sequence's more than once
+    pages, scales, values = filled_cache(3, [(0, count * size)], torch.arange(count, dtype=torch.int32)[None], count, 1, size, dim, bits)
+    q = torch.randn(rows, heads, dim, generator=g).to(BF)
+    slopes = torch.tensor([0.25, 1.0])
+    starts = torch.tensor([0, rows], dtype=torch.int32)
+    call = paged.Batch(*cuda(starts, torch.tensor([total], dtype=torch.int32), table), rows, total)
+    got = paged.attention(paged.Cache(pages, scales), call, q.cuda(), slopes=slopes.cuda())
+    first = total // size * size - near
+    want, weight, (reach, span) = R.attention(q, values, [0, rows], [total - first], table[:, first // size:], dim ** -0.5, slopes=slopes)
+    within(got, want, R.attention_bound(want, weight, (reach, span), bits))
