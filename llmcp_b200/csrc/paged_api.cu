@@ -189,6 +189,12 @@ extern "C" int llmcp_dev_paged_attention(const llmcp_b200_paged_kv *kv, const ll
             "the workspace is smaller than llmcp_dev_paged_attention_workspace says, or off a 16-byte boundary");
     PagedAttention a = {};
     a.q = q, a.q_row = q_row, a.q_head = q_head, a.heads = h;
+    // A cap whose ratio to a score (or its reciprocal) could leave f32: above 2^64 it changes nothing that f32 scores show, and
+    // below 2^-64 what it leaves of them is 0.
+    if (softcap > 0.0f && softcap < 0x1p-64f)
+      scale = 0.0f;
+    if (softcap > 0x1p64f || softcap < 0x1p-64f)
+      softcap = 0.0f;
     a.scale = scale, a.softcap = softcap, a.slopes = slopes, a.prefix = prefix;
     a.gate = gate, a.gate_row = gate_row, a.gate_head = gate_head;
     a.out = out, a.workspace = workspace;

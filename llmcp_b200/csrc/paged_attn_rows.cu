@@ -492,8 +492,11 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
 #pragma unroll
         for (int m = 0; m < M; ++m)
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            x[m][nt][c] = capped_log2(x[m][nt][c] * factor[nt][c & 1], cap, over_cap);
+          for (int c = 0; c < 4; c += 2) {
+            const float2 v = capped_log2(mul2(pair(x[m][nt][c], x[m][nt][c + 1]), pair(factor[nt][0], factor[nt][1])), cap, over_cap);
+            x[m][nt][c] = v.x;
+            x[m][nt][c + 1] = v.y;
+          }
         scaled[nt][0] = scaled[nt][1] = 1.0f;
       }
       if (biased || masked) {

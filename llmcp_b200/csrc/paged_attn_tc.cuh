@@ -150,27 +150,6 @@ struct RowScores {
   bool biased;
 };
 
-// scale * tanh of two values by an odd polynomial, fitted likewise: of at most 1 by degree 13 (absolute error 4.4e-8), of at
-// most 1/2 by degree 9 (6.3e-9).
-template <bool HALF> __device__ __forceinline__ uint64_t tanh_by_fma(uint64_t y, float scale) {
-  const uint64_t u = mul2(y, y);
-  uint64_t r;
-  if constexpr (HALF) {
-    r = fma2(u, pair(0.017151297808556672f, 0.017151297808556672f), pair(-0.05299423135979913f, -0.05299423135979913f));
-    r = fma2(r, u, pair(0.13324906986917054f, 0.13324906986917054f));
-    r = fma2(r, u, pair(-0.333330757952904f, -0.333330757952904f));
-    r = fma2(r, u, pair(0.9999999873746263f, 0.9999999873746263f));
-  } else {
-    r = fma2(u, pair(0.0010531353245070575f, 0.0010531353245070575f), pair(-0.006239815943848765f, -0.006239815943848765f));
-    r = fma2(r, u, pair(0.020331109759454728f, 0.020331109759454728f));
-    r = fma2(r, u, pair(-0.05347844709285361f, -0.05347844709285361f));
-    r = fma2(r, u, pair(0.1332570887576237f, 0.1332570887576237f));
-    r = fma2(r, u, pair(-0.33332882758746407f, -0.33332882758746407f));
-    r = fma2(r, u, pair(0.9999999563685537f, 0.9999999563685537f));
-  }
-  return mul2(mul2(y, pair(scale, scale)), r);
-}
-
 template <int KT, bool HALF> __device__ __forceinline__ void cap_scores(uint32_t (&x)[KT / 32][32], float into, float scale) {
 #pragma unroll
   for (int c = 0; c < KT / 32; ++c)
@@ -202,8 +181,11 @@ template <int KT> __device__ __forceinline__ float shape_scores(uint32_t (&x)[KT
 #pragma unroll
       for (int c = 0; c < KT / 32; ++c)
 #pragma unroll
-        for (int u = 0; u < 32; ++u)
-          x[c][u] = __float_as_uint(capped_log2(__uint_as_float(x[c][u]) * r.factor, r.cap, r.over_cap));
+        for (int u = 0; u < 32; u += 2) {
+          const float2 v = capped_log2(mul2(pair(__uint_as_float(x[c][u]), __uint_as_float(x[c][u + 1])), pair(r.factor, r.factor)), r.cap, r.over_cap);
+          x[c][u] = __float_as_uint(v.x);
+          x[c][u + 1] = __float_as_uint(v.y);
+        }
     }
     scaled = 1.0f;
   }

@@ -102,3 +102,24 @@ def test_bias_by_distance_past_2_to_the_24_keys(rows, heads, dim, bits):
     first = total // size * size - near
     want, weight, (reach, span) = R.attention(q, values, [0, rows], [total - first], table[:, first // size:], dim ** -0.5, slopes=slopes)
     within(got, want, R.attention_bound(want, weight, (reach, span), bits))
+
+
+# ---- caps -----------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("cap", [1e-39, 1e-30, 3.0, 1e4, 1e6, 1e30])
+@pytest.mark.parametrize("batch", [[(1, 300), (2, 70)], [(150, 333), (40, 41)]], ids=["steps", "prompts"])
+@pytest.mark.parametrize("heads,groups,dim,bits", [(4, 2, 64, 16), (6, 2, 128, 4), (4, 1, 256, 16), (4, 1, 256, 4)])
+@pytest.mark.parametrize("spread", [1.0, 8.0])
+def test_caps_of_any_size(heads, groups, dim, bits, batch, cap, spread):
+    """tanh keeps the scores' relative precision: 2^-20 (exp and reciprocal 2^-21.5 each of a tanh of 0.46 at least, the
+    polynomial below that 2^-21), so a cap far above them changes nothing."""
+    g = torch.Generator().manual_seed(dim + 3)
+    q_start, kv_len, table, count = R.tables(batch, 64, 1, 5)
+    pages, scales, values = filled_cache(7, batch, table, count, groups, 64, dim, bits)
+    q = (spread * torch.randn(int(q_start[-1]), heads, dim, generator=g)).to(BF)
+    q[0] = 0  # scores of 0, beside a cap whose reciprocal is past f32's end
+    got = paged.attention(paged.Cache(pages, scales), make_batch(q_start, kv_len, table, batch), q.cuda(), softcap=cap)
+    want, weight, extent = R.attention(q, values, q_start, kv_len, table, dim ** -0.5, softcap=float(torch.tensor(cap)))
+    bound = R.attention_bound(want, weight, extent, bits) + weight * 2 * extent[0] * 2.0 ** -20
+    within(got, want, bound)
