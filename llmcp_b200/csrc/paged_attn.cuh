@@ -115,9 +115,10 @@ __device__ __forceinline__ float2 capped_log2(uint64_t x, float cap, float over_
   return make_float2(fabsf(y.x) <= 0.5f ? near.x : far(y.x), fabsf(y.y) <= 0.5f ? near.y : far(y.y));
 }
 
-// x sigmoid(gate); below -80 the product is 0 beside any other value of a row.
+// x sigmoid(gate) = x / (1 + e^-gate).  Where the divisor is above 2^126 (gates below -87.3, -infinity among them) __fdividef
+// gives 0, and the product would be below f32's normal range; a NaN stays one.
 __device__ __forceinline__ float times_sigmoid(float x, float gate) {
-  return __fdividef(x, 1.0f + exp2_approx(fminf(gate * -1.4426950408889634f, 115.0f)));
+  return __fdividef(x, 1.0f + exp2_approx(gate * -1.4426950408889634f));
 }
 
 // Eight dimensions of a finished row: times their gate, where there is one, as bf16.

@@ -123,3 +123,28 @@ def test_caps_of_any_size(heads, groups, dim, bits, batch, cap, spread):
     want, weight, extent = R.attention(q, values, q_start, kv_len, table, dim ** -0.5, softcap=float(torch.tensor(cap)))
     bound = R.attention_bound(want, weight, extent, bits) + weight * 2 * extent[0] * 2.0 ** -20
     within(got, want, bound)
+
+
+# ---- gates ----------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("batch", [[(1, 40), (1, 3)], [(1, 20011)], [(2, 3000)] * 20, [(150, 333), (40, 41)], [(20, 6000)]], ids=str)
+@pytest.mark.parametrize("heads,groups,dim,bits", [(8, 2, 64, 16), (8, 2, 128, 4), (8, 2, 256, 16)])
+def test_gates_that_close(heads, groups, dim, bits, batch):
+    """Sigmoids of gates down to -87 keep their relative precision, from f32's normal range on (2^-126) nothing is left,
+    -infinity closes, infinity opens, NaN stays."""
+    g = torch.Generator().manual_seed(dim + 4)
+    q_start, kv_len, table, count = R.tables(batch, 64, 1, 5)
+    pages, scales, values = filled_cache(7, batch, table, count, groups, 64, dim, bits)
+    tokens = int(q_start[-1])
+    q = torch.randn(tokens, heads, dim, generator=g).to(BF)
+    choices = torch.tensor([-math.inf, math.inf, math.nan, -60.0, -79.5, -80.5, -83.0, -86.5, -95.0, -3e38, 3e38, 0.0])
+    gate = choices[torch.randint(0, len(choices), (tokens, heads, dim), generator=g)].to(BF)
+    got = paged.attention(paged.Cache(pages, scales), make_batch(q_start, kv_len, table, batch), q.cuda(), gate=gate.cuda()).cpu().double()
+    want, weight, extent = R.attention(q, values, q_start, kv_len, table, dim ** -0.5)
+    s = torch.sigmoid(gate.double())
+    assert torch.equal(got.isnan(), gate.isnan())
+    assert (got[gate == -math.inf] == 0).all()
+    bound = (R.attention_bound(want, weight, extent, bits) - 1e-30) * s + weight * (2.0 ** -126 + s * 2.0 ** -17)
+    near = (got - want * s).abs() <= bound  # both 0 behind a closed gate where a row's only value is 0
+    assert near[~gate.isnan() & (gate != -math.inf)].all()
