@@ -145,8 +145,8 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
   __shared__ uint64_t full[kWarps][S::slots];
   __shared__ float warp_max[kWarps][NT * 8], warp_sum[kWarps][NT * 8];
   __shared__ int sees[NT * 8];                       // keys below it
-  __shared__ float slope[NT * 8], unscales[NT * 8];
-  __shared__ int at[NT * 8]; // position
+  __shared__ float slope[NT * 8];
+  __shared__ int at[NT * 8], exponents[NT * 8]; // position; of the power of two that takes a row's products back
   __shared__ uint2 offsets_sm[Q4 ? NT : 1][32];
   __shared__ int failed;
   uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
@@ -237,7 +237,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
     const int row = nt * 8 + g;
     const uint16_t *q = p.call.q + (seq.first + row / group) * p.call.q_row + (kvh * group + row % group) * p.call.q_head;
     uint32_t fragment[Q4 ? NB * 4 : MT * 2];
-    float unscale = 1.0f;
+    int exponent = 0;
     if constexpr (Q4) {
       uint4 raw[NB];
       float sums[NB];
@@ -254,7 +254,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const int up = top == 0 ? 0 : min(126, 14 - (static_cast<int>(top >> 7) - 127)); // q * 2^up has its largest in [2^14, 2^15)
       const float mult = __uint_as_float(static_cast<uint32_t>(up + 127) << 23 | (negative ? 0x80000000u : 0u));
-      unscale = __int_as_float(min(254, 24 - up + 127) << 23);
+      exponent = 24 - up;
 #pragma unroll
       for (int k = 0; k < NB; ++k) {
         const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
@@ -301,7 +301,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
         queries[nt][k] = fragment[k];
     }
     if (Q4 && t == 0)
-      unscales[row] = unscale;
+      exponents[row] = exponent;
   }
   // what each row sees, and its bias
   if (tid < NT * 8) {
@@ -320,8 +320,13 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
       offsets[nt][1] = offsets_sm[nt][lane].y;
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      factor[nt][i] = (flat ? 1.0f : fabsf(p.call.scale) * (p.call.softcap > 0.0f ? 1.0f : 1.4426950408889634f)) * (Q4 ? unscales[nt * 8 + 2 * t + i] : 1.0f);
+    for (int i = 0; i < 2; ++i) {
+      factor[nt][i] = flat ? 1.0f : fabsf(p.call.scale) * (p.call.softcap > 0.0f ? 1.0f : 1.4426950408889634f);
+      if constexpr (Q4) { // -102 to 138: two powers of two, one may be past f32's end
+        const int e = exponents[nt * 8 + 2 * t + i];
+        factor[nt][i] = factor[nt][i] * __int_as_float((127 + e / 2) << 23) * __int_as_float((127 + e - e / 2) << 23);
+      }
+    }
   }
   // four words of the fragments of dimensions 32 k .. 32 k + 31
   auto query_words = [&](int nt, int k, uint32_t (&w)[4]) {

@@ -148,3 +148,19 @@ def test_gates_that_close(heads, groups, dim, bits, batch):
     bound = (R.attention_bound(want, weight, extent, bits) - 1e-30) * s + weight * (2.0 ** -126 + s * 2.0 ** -17)
     near = (got - want * s).abs() <= bound  # both 0 behind a closed gate where a row's only value is 0
     assert near[~gate.isnan() & (gate != -math.inf)].all()
+
+
+# ---- queries -----------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("batch", [[(1, 300), (2, 70)], [(150, 333), (40, 41)]], ids=["steps", "prompts"])
+@pytest.mark.parametrize("heads,groups,dim", SHAPES_4BIT)
+def test_queries_next_to_the_end_of_their_type(heads, groups, dim, batch):
+    g = torch.Generator().manual_seed(dim + 5)
+    q_start, kv_len, table, count = R.tables(batch, 64, 1, 5)
+    pages, scales, values = filled_cache(7, batch, table, count, groups, 64, dim, 4, scale=1e-3)
+    q = (torch.rand(int(q_start[-1]), heads, dim, generator=g, dtype=torch.float64).sub(0.5) * 2.0 ** 122).to(BF)
+    scale = 2.0 ** -112
+    got = paged.attention(paged.Cache(pages, scales), make_batch(q_start, kv_len, table, batch), q.cuda(), scale=scale)
+    want, weight, extent = R.attention(q, values, q_start, kv_len, table, scale)
+    within(got, want, R.attention_bound(want, weight, extent, 4))
