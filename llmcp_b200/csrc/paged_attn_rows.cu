@@ -483,7 +483,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
       for (int n = 0; n < KT / 32; ++n)
 #pragma unroll
         for (int k = 0; k < NB / 2; ++k)
-          largest = __vmaxu2(largest, scale_words(s, n * 32 + lane)[k]);
+          largest = __vmaxu2(largest, scale_words(s, n * 32 + lane)[k] & 0x7fff7fffu);
       largest = __reduce_max_sync(0xffffffffu, max(largest & 0xffffu, largest >> 16));
       shift = fmaxf(shift, static_cast<float>(static_cast<int>(largest >> 10) - 29) + kHeadroom);
     }

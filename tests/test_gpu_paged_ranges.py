@@ -164,3 +164,22 @@ def test_queries_next_to_the_end_of_their_type(heads, groups, dim, batch):
     got = paged.attention(paged.Cache(pages, scales), make_batch(q_start, kv_len, table, batch), q.cuda(), scale=scale)
     want, weight, extent = R.attention(q, values, q_start, kv_len, table, scale)
     within(got, want, R.attention_bound(want, weight, extent, 4))
+
+
+# ---- scales ------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("batch", [STEPS, PROMPTS], ids=["steps", "prompts"])
+@pytest.mark.parametrize("heads,groups,dim", SHAPES_4BIT)
+def test_scales_below_zero(heads, groups, dim, batch):
+    """append writes none, but a cache may come from elsewhere: they multiply codes like any other."""
+    g = torch.Generator().manual_seed(dim + 6)
+    q_start, kv_len, table, count = R.tables(batch, 64, 1, 5)
+    pages, scales, _ = filled_cache(7, batch, table, count, groups, 64, dim, 4)
+    sign = torch.where(torch.rand(scales.shape, generator=g) < 0.5, -1.0, 1.0)
+    scales *= sign.half().cuda()
+    values = R.unpack(pages.cpu(), scales.cpu()).nan_to_num()
+    q = torch.randn(int(q_start[-1]), heads, dim, generator=g).to(BF)
+    got = paged.attention(paged.Cache(pages, scales), make_batch(q_start, kv_len, table, batch), q.cuda())
+    want, weight, extent = R.attention(q, values, q_start, kv_len, table, dim ** -0.5)
+    within(got, want, R.attention_bound(want, weight, extent, 4))
