@@ -60,8 +60,9 @@ PagedBatch to_batch(const llmcp_b200_paged_batch *b, const PagedKv &kv) {
   out.sequences = static_cast<int>(b->sequences);
   out.table_width = static_cast<int>(b->table_width);
   out.tokens = static_cast<int>(b->tokens);
-  out.max_q = static_cast<int>(b->max_q);
-  // no sequence has more keys than its pages hold: a wider bound would only lay out empty work
+  // no sequence has more rows than the call, or more keys than its pages hold: wider bounds would only lay out empty work, or
+  // choose the kernel for rows that are not there
+  out.max_q = static_cast<int>(std::min(b->max_q, b->tokens));
   out.max_kv = static_cast<int>(std::min(b->max_kv, b->table_width << kv.page_shift));
   return out;
 }
@@ -133,11 +134,11 @@ extern "C" int llmcp_dev_paged_read(const llmcp_b200_paged_kv *kv, const llmcp_b
 }
 
 namespace {
-int checked_heads(const PagedKv &c, const PagedBatch &b, int64_t heads) {
+int checked_heads(const PagedKv &c, const PagedBatch &b, int64_t max_q, int64_t heads) {
   require(heads >= 1 && heads <= 16384 && heads % c.kv_heads == 0, "heads has to be a multiple of kv_heads, at most 16384");
   require(heads / c.kv_heads <= 128, "at most 128 query heads share a key head");
   // prompts over 4 bits work on rows of 16 bits, numbered in 31 bits too
-  require(!c.scales || b.max_q * (heads / c.kv_heads) <= 16 ||
+  require(!c.scales || max_q * (heads / c.kv_heads) <= 16 ||
               static_cast<int64_t>(b.sequences) * 2 * c.kv_heads * ((b.max_kv + int64_t(127)) / 128 * 128) < (int64_t(1) << 31),
           "sequences * 2 * kv_heads * max_kv has to stay below 2^31 for prompts over 4 bits; make several calls");
   return static_cast<int>(heads);
@@ -149,7 +150,7 @@ extern "C" int64_t llmcp_dev_paged_attention_workspace(const llmcp_b200_paged_kv
   entry([&] {
     const PagedKv c = to_kv(kv);
     const PagedBatch b = to_batch(batch, c);
-    const int h = checked_heads(c, b, heads);
+    const int h = checked_heads(c, b, batch->max_q, heads);
     if (nothing(b)) {
       bytes = 0;
       return;
@@ -168,7 +169,7 @@ extern "C" int llmcp_dev_paged_attention(const llmcp_b200_paged_kv *kv, const ll
   return entry([&] {
     const PagedKv c = to_kv(kv);
     const PagedBatch b = to_batch(batch, c);
-    const int h = checked_heads(c, b, heads);
+    const int h = checked_heads(c, b, batch->max_q, heads);
     require(std::isfinite(scale) && std::isfinite(softcap) && softcap >= 0.0f, "scale and softcap have to be finite, softcap not negative");
     if (nothing(b))
       return;

@@ -486,10 +486,8 @@ paged_expand_kernel(PagedKv kv, PagedBatch batch, uint4 *__restrict__ out, int64
   }
 }
 
-// Tiles of a sequence's rows; a bound past the call's rows would only lay out empty CTAs.
-int64_t row_tiles(const PagedBatch &batch, int per_tile) {
-  return (static_cast<int64_t>(batch.max_q < batch.tokens ? batch.max_q : batch.tokens) + per_tile - 1) / per_tile;
-}
+// Tiles of a sequence's rows.
+int64_t row_tiles(const PagedBatch &batch, int per_tile) { return (static_cast<int64_t>(batch.max_q) + per_tile - 1) / per_tile; }
 
 int64_t expanded_rows(const PagedBatch &batch) { return (static_cast<int64_t>(batch.max_kv) + 127) / 128 * 128; }
 

@@ -183,3 +183,18 @@ def test_scales_below_zero(heads, groups, dim, batch):
     got = paged.attention(paged.Cache(pages, scales), make_batch(q_start, kv_len, table, batch), q.cuda())
     want, weight, extent = R.attention(q, values, q_start, kv_len, table, dim ** -0.5)
     within(got, want, R.attention_bound(want, weight, extent, 4))
+
+
+# ---- bounds ------------------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_a_bound_above_the_calls_rows_changes_nothing(bits):
+    """No sequence has more rows than the call: max_q past them takes no other kernel and no more memory."""
+    batch = [(1, 3000), (1, 50)]
+    q_start, kv_len, table, count = R.tables(batch, 64, 1, 5)
+    pages, scales, _ = filled_cache(7, batch, table, count, 2, 64, 128, bits)
+    cache, q = paged.Cache(pages, scales), torch.randn(2, 8, 128, device="cuda").to(BF)
+    tight, wide = (make_batch(q_start, kv_len, table, batch, max_q=most) for most in (2, 1 << 30))
+    assert paged.workspace_bytes(cache, wide, 2, 8) == paged.workspace_bytes(cache, tight, 2, 8)
+    assert torch.equal(paged.attention(cache, wide, q), paged.attention(cache, tight, q))
