@@ -7,10 +7,11 @@
 //
 // y is the correctly rounded value: a last-bit difference would now and then move it to its neighbour and, in 4 bits, a
 // code with it.  The f32 result is taken where its error bound cannot reach the middle between two bf16 values (the
-// rounded ends of its error interval are equal); a row with a value nearer than that is computed again in f64 (bf16 x f32
-// products are exact there), one row of 256 in ten or so with norms, one in fifty without.  The step from y to the code needs
-// no more than f32: y has 8 significant bits, d 11 and code + 1/2 at most 4, so y / d is either exactly half way between two
-// codes or at least 2^-15 away from it, and a quotient with its remainder's share added tells the two apart.
+// rounded ends of its error interval are equal) and nothing leaves f32's normal range; a row with a value for which that
+// fails is computed again in f64 (bf16 x f32 products are exact there), one row of 256 in ten or so with norms, one in fifty
+// without.  The step from y to the code needs no more than f32: y has 8 significant bits, d 11 and code + 1/2 at most 4, so
+// y / d is either exactly half way between two codes or at least 2^-15 away from it, and a quotient with its remainder's
+// share added tells the two apart.
 //
 // Append is bound by instructions (170 for 256 query values, 120 more for 256 values' codes), read by HBM.  8192 tokens of 32
 // + 2 x 8 heads of 128: 52 us over bf16 pages, 67 us over 4 bits, of 26 and 28 us that their bytes take.  30001 tokens of 4
@@ -252,6 +253,25 @@ __device__ __forceinline__ Turn<E> turn_of(const Place &place, const float *cs, 
   return r;
 }
 
+__device__ __forceinline__ float least_of(float a, float b, float c) {
+  float r;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// Whether a lane has a value below 2^-50 or a coefficient below 2^-30 that is not 0.
+template <int E> __device__ __forceinline__ bool has_small(const Row<E> &row, const Turn<E> &turn) {
+  bool small = false;
+#pragma unroll
+  for (int i = 0; i < E / 2; ++i) {
+    const float2 x = halves(unpacked(row.w[i])), c = halves(turn.c[i]), n = halves(turn.n[i]);
+    small |= (x.x != 0.0f && fabsf(x.x) < 0x1p-50f) || (x.y != 0.0f && fabsf(x.y) < 0x1p-50f);
+    small |= (c.x != 0.0f && fabsf(c.x) < 0x1p-30f) || (c.y != 0.0f && fabsf(c.y) < 0x1p-30f);
+    small |= (n.x != 0.0f && fabsf(n.x) < 0x1p-30f) || (n.y != 0.0f && fabsf(n.y) < 0x1p-30f);
+  }
+  return small;
+}
+
 // A warp's part of the heads of one kind of its token.  row: the first of them, requested before.  kTurns: normalised and
 // rotated; kCodes: stored as codes and scales.  Rows that need f64 are left for the end of up to 32 turns: a call inside the
 // loop would take its registers from it.
@@ -288,6 +308,8 @@ __device__ __forceinline__ void store_heads(Place &place, Row<E> row, int heads,
         // and n are off by 2 of themselves, which makes y's 2 |x c| + 3 |p| + |y| <= 5 |p| + 3 |y|; inv is off by 9.7 (sum
         // of squares of exact terms, mean and eps: E + 7, at most 15, half of which is left by the root; rsqrt 2.2) and its
         // product by 1 more.  And |y| for the interval's ends; the last percents are for the bound's own rounding.
+        // That holds where nothing leaves f32's normal range: where |p| + |y| is below 2^-100, before or after its product
+        // with inv, it has to be because it is 0.
         bool sure = true;
         float inv = 1.0f, of_y = 2.03f / 16777216.0f, p_to_y = 0.51f;
         if (weight) {
@@ -306,17 +328,22 @@ __device__ __forceinline__ void store_heads(Place &place, Row<E> row, int heads,
           sure = sum >= 0x1p-80f && sum <= 0x1p120f;
         }
         Row<E> done;
+        float least = INFINITY;
 #pragma unroll
         for (int i = 0; i < E / 2; ++i) {
           const uint64_t p = mul2(unpacked(__shfl_sync(0xffffffffu, row.w[i], lane + place.to_partner)), turn.n[i]);
           const uint64_t y = fma2(unpacked(row.w[i]), turn.c[i], p), scaled = mul2(y, pair(inv, inv));
           const float2 a = halves(p), z = halves(y);
-          const uint64_t off = pair(__fmaf_rn(fabsf(a.x), p_to_y, fabsf(z.x)), __fmaf_rn(fabsf(a.y), p_to_y, fabsf(z.y)));
+          const float off_x = __fmaf_rn(fabsf(a.x), p_to_y, fabsf(z.x)), off_y = __fmaf_rn(fabsf(a.y), p_to_y, fabsf(z.y));
+          const uint64_t off = pair(off_x, off_y);
+          least = least_of(least, off_x, off_y);
           const float2 up = halves(fma2(off, pair(of_y, of_y), scaled)), down = halves(fma2(off, pair(-of_y, -of_y), scaled));
           done.w[i] = f32x2_to_bf16x2_hw(up.x, up.y);
           sure &= done.w[i] == f32x2_to_bf16x2_hw(down.x, down.y);
         }
-        if (__any_sync(0xffffffffu, changed && !sure && here)) {
+        const bool in_range = least * fminf(inv, 1.0f) >= 0x1p-100f;
+        if (__any_sync(0xffffffffu, changed && !(sure && in_range) && here) &&
+            (__any_sync(0xffffffffu, changed && !sure && here) || __any_sync(0xffffffffu, (inv < 0x1p-20f || has_small(row, turn)) && here))) {
           again |= 1u << turn_no;
           here = false;
         }

@@ -198,3 +198,32 @@ def test_a_bound_above_the_calls_rows_changes_nothing(bits):
     tight, wide = (make_batch(q_start, kv_len, table, batch, max_q=most) for most in (2, 1 << 30))
     assert paged.workspace_bytes(cache, wide, 2, 8) == paged.workspace_bytes(cache, tight, 2, 8)
     assert torch.equal(paged.attention(cache, wide, q), paged.attention(cache, tight, q))
+
+
+# ---- append ---------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("heads,dim,rot", [(16, 128, 128), (8, 64, 4), (8, 256, 64)])
+def test_append_rounds_products_below_f32s_range_once(heads, dim, rot, norm):
+    """Values whose f32 products are subnormal (all of a row's without norm, every other one's beside ordinary ones with it)
+    come out as the correctly rounded value like any other."""
+    g = torch.Generator().manual_seed(dim)
+    tokens = 3000
+    x = torch.randn(tokens, heads, dim, generator=g, dtype=torch.float64)
+    tiny = 2.0 ** -(119 + 14 * torch.rand(tokens, heads, dim, generator=g, dtype=torch.float64))
+    x = (torch.where(torch.arange(dim) % 2 == 0, x, x * tiny) if norm else x * tiny).to(BF)
+    weight = (0.2 * torch.randn(dim, generator=g)).to(BF) if norm else None
+    angle = torch.rand(tokens, rot // 2, generator=g) * 6
+    if norm:  # partners are both ordinary or both tiny; a rotation by next to nothing keeps them apart from each other
+        angle = angle * 0 + 1e-3
+    cos, sin = (torch.cat((f(angle), f(angle)), 1).contiguous() for f in (torch.cos, torch.sin))
+    want = R.bf16_round(R.rotate(x, weight, cos, sin)).to(BF)
+    pages, _ = empty_cache(-(-tokens // 256), heads, 256, dim, 16)
+    table = torch.arange(pages.shape[0], dtype=torch.int32)[None]
+    call = make_batch(torch.tensor([0, tokens], dtype=torch.int32), torch.tensor([tokens], dtype=torch.int32), table, [(tokens, tokens)])
+    cache = paged.Cache(pages)
+    got = paged.append(cache, call, *cuda(x, x, x, cos, sin), q_norm=cuda(weight), k_norm=cuda(weight))
+    k, _ = paged.read(cache, call, tokens)
+    for y in (got, k):
+        assert torch.equal(y.cpu().double(), want.double())
