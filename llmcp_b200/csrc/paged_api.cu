@@ -114,7 +114,9 @@ extern "C" int llmcp_dev_paged_append(const llmcp_b200_paged_kv *kv, const llmcp
     a.cos = cos, a.sin = sin, a.cos_rows = cos_rows;
     a.heads = static_cast<int>(heads), a.rot = static_cast<int>(rot);
     a.q_out = q_out;
-    check(launch_paged_append(c, b, a, status, static_cast<cudaStream_t>(stream)), "paged append");
+    int sms = 0;
+    check(current_sm_count(&sms), "paged append");
+    check(launch_paged_append(c, b, a, status, sms, static_cast<cudaStream_t>(stream)), "paged append");
     count_launches(1);
   });
 }
@@ -128,7 +130,9 @@ extern "C" int llmcp_dev_paged_read(const llmcp_b200_paged_kv *kv, const llmcp_b
     if (nothing(b))
       return;
     require(k_out && v_out && on(k_out, 16) && on(v_out, 16), "k_out and v_out have to start on a 16-byte boundary");
-    check(launch_paged_read(c, b, k_out, v_out, out_dtype, status, static_cast<cudaStream_t>(stream)), "paged read");
+    int sms = 0;
+    check(current_sm_count(&sms), "paged read");
+    check(launch_paged_read(c, b, k_out, v_out, out_dtype, status, sms, static_cast<cudaStream_t>(stream)), "paged read");
     count_launches(1);
   });
 }

@@ -553,30 +553,30 @@ bool aligned(const void *p, int64_t stride0, int64_t stride1, int elements) {
 
 // Warps per token: as many as the SMs hold at a time, 32 each.  256 tokens of 16 + 2 x 2 heads of 128: 9.2 us with half of
 // them, 8.1 with these or more; 4000 of 16 + 2 x 1 heads of 64: 14.8 us with these, 19.9 with four times as many.
-int warps_per_token(int tokens, int groups) {
-  const int share = 148 * 32 / tokens;
+int warps_per_token(int tokens, int groups, int sms) {
+  const int share = sms * 32 / tokens;
   return share < 1 ? 1 : share < groups ? share : groups;
 }
 
 dim3 grid(int tokens, int share) { return dim3(static_cast<unsigned>((static_cast<int64_t>(tokens) * share + kWarps - 1) / kWarps)); }
 
 template <int D, int E>
-cudaError_t append(const PagedKv &kv, const PagedBatch &batch, const PagedAppend &call, int *status, cudaStream_t stream) {
+cudaError_t append(const PagedKv &kv, const PagedBatch &batch, const PagedAppend &call, int *status, int sms, cudaStream_t stream) {
   constexpr int kRows = 32 * E / D;
   const bool tables = reinterpret_cast<uintptr_t>(call.cos) % 16 == 0 && reinterpret_cast<uintptr_t>(call.sin) % 16 == 0 && call.rot % 4 == 0;
   const int vectors = (call.heads == 0 || aligned(call.q, call.q_row, call.q_head, E) ? 1 : 0) | (aligned(call.k, call.k_row, call.k_head, E) ? 2 : 0) |
                       (aligned(call.v, call.v_row, call.v_head, E) ? 4 : 0) | (tables ? 8 : 0) |
                       (aligned(call.q_norm, 0, 0, E) && aligned(call.k_norm, 0, 0, E) ? 16 : 0);
-  const int share = warps_per_token(batch.tokens, (call.heads + kRows - 1) / kRows + 2 * ((kv.kv_heads + kRows - 1) / kRows));
+  const int share = warps_per_token(batch.tokens, (call.heads + kRows - 1) / kRows + 2 * ((kv.kv_heads + kRows - 1) / kRows), sms);
   if (kv.scales)
     return launch_chained(paged_append_kernel<D, E, true>, grid(batch.tokens, share), dim3(32 * kWarps), 0, stream, kv, batch, call, vectors, share, status);
   return launch_chained(paged_append_kernel<D, E, false>, grid(batch.tokens, share), dim3(32 * kWarps), 0, stream, kv, batch, call, vectors, share, status);
 }
 
 template <int E, bool F32>
-cudaError_t read(const PagedKv &kv, const PagedBatch &batch, void *k_out, void *v_out, int *status, cudaStream_t stream) {
+cudaError_t read(const PagedKv &kv, const PagedBatch &batch, void *k_out, void *v_out, int *status, int sms, cudaStream_t stream) {
   constexpr int D = 32 * E;
-  const int rows = kv.scales ? 512 / D : 1, share = warps_per_token(batch.tokens, (2 * kv.kv_heads + rows - 1) / rows);
+  const int rows = kv.scales ? 512 / D : 1, share = warps_per_token(batch.tokens, (2 * kv.kv_heads + rows - 1) / rows, sms);
   if (kv.scales)
     return launch_chained(paged_read_q4_kernel<D, F32>, grid(batch.tokens, share), dim3(32 * kWarps), 0, stream, kv, batch, k_out, v_out, share, status);
   return launch_chained(paged_read_kernel<E, F32>, grid(batch.tokens, share), dim3(32 * kWarps), 0, stream, kv, batch, k_out, v_out, share, status);
@@ -584,30 +584,30 @@ cudaError_t read(const PagedKv &kv, const PagedBatch &batch, void *k_out, void *
 
 } // namespace
 
-cudaError_t launch_paged_append(const PagedKv &kv, const PagedBatch &batch, const PagedAppend &call, int *status, cudaStream_t stream) {
+cudaError_t launch_paged_append(const PagedKv &kv, const PagedBatch &batch, const PagedAppend &call, int *status, int sms, cudaStream_t stream) {
   const bool eights = call.rot % 16 == 0;
   switch (kv.head_dim) {
   case 64:
-    return eights ? append<64, 8>(kv, batch, call, status, stream) : append<64, 2>(kv, batch, call, status, stream);
+    return eights ? append<64, 8>(kv, batch, call, status, sms, stream) : append<64, 2>(kv, batch, call, status, sms, stream);
   case 128:
-    return eights ? append<128, 8>(kv, batch, call, status, stream) : append<128, 4>(kv, batch, call, status, stream);
+    return eights ? append<128, 8>(kv, batch, call, status, sms, stream) : append<128, 4>(kv, batch, call, status, sms, stream);
   case 256:
-    return append<256, 8>(kv, batch, call, status, stream);
+    return append<256, 8>(kv, batch, call, status, sms, stream);
   default:
     return cudaErrorInvalidValue;
   }
 }
 
-cudaError_t launch_paged_read(const PagedKv &kv, const PagedBatch &batch, void *k_out, void *v_out, int out_dtype, int *status,
+cudaError_t launch_paged_read(const PagedKv &kv, const PagedBatch &batch, void *k_out, void *v_out, int out_dtype, int *status, int sms,
                               cudaStream_t stream) {
   const bool f32 = out_dtype == kF32;
   switch (kv.head_dim) {
   case 64:
-    return f32 ? read<2, true>(kv, batch, k_out, v_out, status, stream) : read<2, false>(kv, batch, k_out, v_out, status, stream);
+    return f32 ? read<2, true>(kv, batch, k_out, v_out, status, sms, stream) : read<2, false>(kv, batch, k_out, v_out, status, sms, stream);
   case 128:
-    return f32 ? read<4, true>(kv, batch, k_out, v_out, status, stream) : read<4, false>(kv, batch, k_out, v_out, status, stream);
+    return f32 ? read<4, true>(kv, batch, k_out, v_out, status, sms, stream) : read<4, false>(kv, batch, k_out, v_out, status, sms, stream);
   case 256:
-    return f32 ? read<8, true>(kv, batch, k_out, v_out, status, stream) : read<8, false>(kv, batch, k_out, v_out, status, stream);
+    return f32 ? read<8, true>(kv, batch, k_out, v_out, status, sms, stream) : read<8, false>(kv, batch, k_out, v_out, status, sms, stream);
   default:
     return cudaErrorInvalidValue;
   }
