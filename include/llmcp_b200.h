@@ -240,7 +240,7 @@ int llmcp_dev_gated_delta_net_noalloc(const uint16_t *conv, const uint16_t *a, c
  *                              pages, in 4 bits as d = f16(min(max |y| / 7, 65504)), code = round-to-even(y / d) held to
  *                              -7 .. 7 per 32 dimensions.  heads may be 0 (keys and values only).  rot: a multiple of head_dim / 16.
  *                              No two rows of a call may have the same place in the cache.  q_out may be q where q is laid out
- *                              like it.
+ *                              like it, and overlaps nothing else.
  *   llmcp_dev_paged_read     : the cached keys and values of the batch's rows as f32 or bf16 (out_dtype 0 or 1),
  *                              k_out and v_out [tokens][kv_heads][head_dim].  max_q = max_kv reads whole sequences.  Rows that no
  *                              sequence has, or whose page does not exist, are left as they are.
@@ -249,11 +249,12 @@ int llmcp_dev_gated_delta_net_noalloc(const uint16_t *conv, const uint16_t *a, c
  *                              tanh(score / softcap); slopes ([heads] f32, may be null): minus slope * |p - j| for the
  *                              key j of a row at position p.  Keys j <= p are seen, and j < prefix[b] where prefix ([sequences] int32) is
  *                              given, none from kv_len on; a row that sees none gets zeros.  gate (may be null): bf16 with
- *                              strides.  Rows of q and gate start on 16-byte boundaries, their strides are positive.  heads: a
+ *                              strides.  Rows of q and gate start on 16-byte boundaries, their strides are positive.  out may be q or
+ *                              gate where that is dense like it, and overlaps nothing else.  heads: a
  *                              multiple of kv_heads, at most 128 times as many.  Products on the tensor cores, sums and softmax in
  *                              f32.  What the pages hold from kv_len on has no influence, whatever it is; the keys and
- *                              values before it have to be finite.  max_q (times heads / kv_heads: up to 16 rows or more) decides
- *                              between two kernels; prompts over 4 bits want a workspace of all sequences' rows in 16
+ *                              values before it have to be finite.  max_q, or tokens where they are fewer (times heads / kv_heads: up to
+ *                              16 rows or more), decides between two kernels; prompts over 4 bits want a workspace of all sequences' rows in 16
  *                              bits, sequences * 2 * kv_heads * max_kv of them, fewer than 2^31.  workspace: device memory of
  *                              llmcp_dev_paged_attention_workspace bytes (-1 on error; depends on the host's figures only) that no other call uses
  *                              meanwhile, captured graphs that may run at the same time included; needs no clearing.

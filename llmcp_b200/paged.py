@@ -2,7 +2,9 @@
 
 The calls of include/llmcp_b200.h (llmcp_dev_paged_*) with their checks; layouts, formulas and what ``status`` reports
 are described there.  Everything is enqueued on the current stream of the tensors' device and nothing is synchronised,
-so the calls can be captured into a graph; lengths and page tables may then change between replays.
+so the calls can be captured into a graph; lengths and page tables may then change between replays.  Rows whose lengths or
+pages do not fit (more than ``max_q`` or ``max_kv``, a page that does not exist) are left out, and results are not cleared
+before: only ``status`` (one int32, raised and never cleared by the calls) tells, so pass one where that may happen.
 
     cache = Cache(pages, scales)                # pages bf16, or uint8 with f16 scales (4 bits)
     batch = Batch(q_start, kv_len, page_table, max_q, max_kv)
@@ -208,8 +210,8 @@ def workspace_bytes(cache, batch, tokens, heads):
 
 @_on_device
 def attention(cache, batch, q, scale=None, softcap=0.0, slopes=None, prefix=None, gate=None, out=None, workspace=None, status=None):
-    """softmax(score) v, times sigmoid(gate) where there is a gate: [tokens, heads, head_dim] bf16.  ``q`` as ``append``
-    returns it; ``scale`` 1 / sqrt(head_dim) by default; ``slopes`` float32 [heads]; ``prefix`` int32 [sequences];
+    """softmax(score) v, times sigmoid(gate) where there is a gate: [tokens, heads, head_dim] bf16.  ``out`` may be q or gate
+    where that is contiguous, and overlaps nothing else.  ``q`` as ``append`` returns it; ``scale`` 1 / sqrt(head_dim) by default; ``slopes`` float32 [heads]; ``prefix`` int32 [sequences];
     ``gate`` like q.  ``workspace``: a uint8 tensor of workspace_bytes() that no other call uses meanwhile; taken from
     torch's allocator where it is not given."""
     dev, bf = cache.device, torch.bfloat16

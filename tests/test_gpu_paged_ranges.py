@@ -200,6 +200,73 @@ def test_a_bound_above_the_calls_rows_changes_nothing(bits):
     assert torch.equal(paged.attention(cache, wide, q), paged.attention(cache, tight, q))
 
 
+# ---- refused rows ----------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("dim,bits", [(64, 16), (64, 4), (256, 16), (256, 4)])
+def test_refused_sequences_leave_their_rows_and_no_others(rows, dim, bits):
+    batch = [(rows, 100), (rows, 90)]
+    q_start, kv_len, table, count = R.tables(batch, 32, 1, 2)
+    pages, scales, values = filled_cache(3, batch, table, count, 2, 32, dim, bits)
+    q = torch.randn(2 * rows, 4, dim, generator=torch.Generator().manual_seed(1)).to(BF)
+    want, weight, extent = R.attention(q, values, q_start, kv_len, table, dim ** -0.5)
+    bound = R.attention_bound(want, weight, extent, bits)
+    cache = paged.Cache(pages, scales)
+    for change, valid in ((dict(max_kv=95), [1]), (dict(lengths=[100, 129]), [0]), (dict(lengths=[-5, 90]), [1]), (dict(starts=[0, -1, 2 * rows]), []),
+                          (dict(starts=[0, rows, 5000]), [0]), (dict(starts=[0, 5000, 2 * rows]), [])):
+        change = dict(change)
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        lengths, starts = change.pop("lengths", [100, 90]), change.pop("starts", q_start.tolist())
+        call = make_batch(torch.tensor(starts, dtype=torch.int32), torch.tensor(lengths, dtype=torch.int32), table, batch, **dict(dict(max_kv=2000), **change))
+        out = torch.full((2 * rows, 4, dim), 7.0, dtype=BF, device="cuda")
+        paged.attention(cache, call, q.cuda(), out=out, status=status)
+        assert int(status) == 4
+        for b in range(2):
+            part = slice(b * rows, (b + 1) * rows)
+            if b in valid:
+                within(out[part], want[part], bound[part])
+            else:
+                assert (out[part] == 7.0).all()
+
+
+@pytest.mark.parametrize("bits,dtype", [(16, torch.float32), (16, BF), (4, torch.float32), (4, BF)])
+def test_read_leaves_refused_rows(bits, dtype):
+    """Through the C entry, into buffers that show what was written."""
+    batch = [(3, 20), (2, 40), (1, 5), (4, 4)]
+    q_start, kv_len, table, count = R.tables(batch, 16, 1, 2)
+    pages, scales, values = filled_cache(3, batch, table, count, 2, 16, 64, bits)
+    broken = table.clone()
+    broken[0, 1] = count  # the page of the first sequence's last rows
+    cache, call = paged.Cache(pages, scales), make_batch(q_start, kv_len, broken, batch, max_kv=39)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = torch.full((2, 12, 2, 64), 7.0, dtype=dtype, device="cuda")
+    assert paged._library().llmcp_dev_paged_read(cache._c, call._c(cache, 12), out[0].data_ptr(), out[1].data_ptr(), 0 if dtype is torch.float32 else 1,
+                                                 status.data_ptr(), None) == 0
+    torch.cuda.synchronize()
+    assert int(status) == 4
+    assert (out[:, :5] == 7.0).all() and (out[:, 10:] == 7.0).all()
+    for which in (0, 1):
+        rows = torch.cat([R.sequence_rows(values, table, b, which, t)[t - n:] for b, (n, t) in list(enumerate(batch))[2:]]).double()
+        assert torch.equal(out[which, 5:10].cpu().double(), rows if dtype is torch.float32 else R.bf16_round(rows))
+
+
+# ---- results in place ------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("batch", [[(1, 40), (1, 3)], [(1, 20011), (2, 60)], [(2, 3000)] * 20, [(150, 333), (40, 41)], [(20, 6000)]], ids=str)
+@pytest.mark.parametrize("heads,groups,dim,bits", [(8, 2, 64, 16), (10, 2, 128, 4), (8, 2, 256, 16), (8, 2, 256, 4)])
+def test_results_in_place_of_queries_or_gates(heads, groups, dim, bits, batch):
+    q_start, kv_len, table, count = R.tables(batch, 64, 1, 5)
+    pages, scales, _ = filled_cache(7, batch, table, count, groups, 64, dim, bits)
+    cache, call, tokens = paged.Cache(pages, scales), make_batch(q_start, kv_len, table, batch), int(q_start[-1])
+    q, gate = torch.randn(2, tokens, heads, dim, device="cuda", generator=torch.Generator("cuda").manual_seed(1)).to(BF)
+    want = paged.attention(cache, call, q, gate=gate)
+    over_q, over_gate = q.clone(), gate.clone()
+    assert paged.attention(cache, call, over_q, gate=gate, out=over_q) is over_q and torch.equal(over_q, want)
+    assert paged.attention(cache, call, q, gate=over_gate, out=over_gate) is over_gate and torch.equal(over_gate, want)
+
+
 # ---- append ---------------------------------------------------------------------------------------------------------------
 
 
