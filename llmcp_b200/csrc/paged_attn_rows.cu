@@ -25,9 +25,10 @@
 // weight, p' = f16(f16(p 2^k) d): k = 15, or less where the largest d so far would take p' past 2^15 (it moves as the
 // running maximum does), so that weights down to 2^-29 of the largest keep f16's relative rounding, 2^-11 twice.
 //
-// One token of 64 sequences over 2000 to 8191 keys of 4 heads of 256 in bf16: 211 us, 6.5 TB/s.  Over 4 bits instructions
-// bound it (48 % of the issue slots, 1182 of them for 32 keys of 256): one token over 131000 keys 44 us, 3.4 TB/s; three
-// tokens of 20 heads of 128, 96 sequences over 1250 to 5000 keys, 89 us, 2 TB/s.
+// One token of 64 sequences over 2000 to 8191 keys of 4 heads of 256 in bf16: 211 us, 6.5 TB/s.  Over 4 bits neither memory
+// (43 % of its rate) nor issue (48 % of the slots, 1182 instructions for 32 keys of 256) is full: scores, maximum, weights and
+// values of a warp's tile follow on one another, and three warps a scheduler do not hide their latencies.  One token over
+// 131000 keys 44 us, 3.4 TB/s; three tokens of 20 heads of 128, 96 sequences over 1250 to 5000 keys, 90 us, 2 TB/s.
 
 #include "common.cuh"
 #include "paged.h"

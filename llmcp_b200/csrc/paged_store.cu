@@ -13,10 +13,11 @@
 // y / d is either exactly half way between two codes or at least 2^-15 away from it, and a quotient with its remainder's
 // share added tells the two apart.
 //
-// Append is bound by instructions (170 for 256 query values, 120 more for 256 values' codes), read by HBM.  8192 tokens of 32
-// + 2 x 8 heads of 128: 52 us over bf16 pages, 67 us over 4 bits, of 26 and 28 us that their bytes take.  30001 tokens of 4
-// heads of 256 read from bf16 pages: 40 us, 6.2 TB/s.  One token: 4.5 us.  A warp takes a whole token where there are enough of
-// them (a block for each, with four warps that each found sequence, page and angles: 64 and 82 us, and 45 us to read).
+// Append is bound by instructions (180 for 256 query values, 120 more for 256 values' codes), read by HBM.  In a captured
+// graph, 8192 tokens of 32 + 2 x 8 heads of 128: 63 us over bf16 pages, 65 us over 4 bits, of 26 and 28 us that their bytes
+// take.  30001 tokens of 4 heads of 256 read from bf16 pages: 40 us, 6.2 TB/s.  One token: 4.9 us.  A warp takes a whole token
+// where there are enough of them (a block for each, with four warps that each found sequence, page and angles: 22 % longer,
+// and 12 % to read).
 // A lane takes eight neighbouring dimensions (rows of 64 to 256: 8 to 32 lanes).  Partners of a rotation lie in the same
 // place of another lane and come by shuffle; where rot / 2 is not a multiple of 8 a lane takes head_dim / 32 dimensions.
 
@@ -370,8 +371,9 @@ __device__ __forceinline__ void store_heads(Place &place, Row<E> row, int heads,
 }
 
 // `share` warps take one token, 32 / kLanes of its query, then key, then value heads at a time each, and request the next
-// ones while they work on these.  Registers: rows of 256 gain more from 80 each (8192 tokens with norms: 66 us, 70 with 64),
-// shorter ones from more warps (9066 tokens of 32 + 2 x 8 heads in 4 bits: 74 us with 64, 80 with 80).
+// ones while they work on these.  Registers: rows of 256 gain more from 80 each (8192 tokens with norms: 6 % longer with 64),
+// shorter ones from more warps (9066 tokens of 32 + 2 x 8 heads in 4 bits: 8 % longer with 80).  Either way some 30 words a
+// thread are kept in local memory, most of them around the loop and not in it.
 template <int D, int E, bool kCodes>
 __global__ void __launch_bounds__(32 * kWarps, D == 256 ? 6 : 8)
 paged_append_kernel(PagedKv kv, PagedBatch batch, PagedAppend call, int vectors, unsigned share, int *__restrict__ status) {
@@ -501,7 +503,7 @@ paged_read_q4_kernel(PagedKv kv, PagedBatch batch, void *__restrict__ k_out, voi
   const uint8_t *src = kv.pages + first * (D / 2) + l * 8;
   const uint16_t *scales = kv.scales + first * (D / 32) + l / 2;
   const int64_t at = static_cast<int64_t>(t) * kv.kv_heads * D + l * 16;
-    const int step = static_cast<int>(share) * kRows;
+  const int step = static_cast<int>(share) * kRows;
   for (int front = static_cast<int>(warp % share) * kRows + lane / kLanes; front < 2 * kv.kv_heads; front += kAhead * step) {
     uint2 codes[kAhead];
     uint16_t scale[kAhead];
