@@ -22,8 +22,9 @@
 // otherwise be the difference of two large sums.  q is scaled by a power of two per row so that its largest element lies
 // in [2^14, 2^15): f16 holds every bf16 value that matters beside it.  A block's score is multiplied by its key scale in
 // f32 (the part of the 8s is one more product, scales times -8 sum q in two f16 pieces); the value scale goes into the
-// weight, p' = f16(f16(p 2^k) d): k = 15, or less where the largest d so far would take p' past 2^15 (it moves as the
-// running maximum does), so that weights down to 2^-29 of the largest keep f16's relative rounding, 2^-11 twice.
+// weight, p' = f16(f16(p 2^k) d 2^j): k = 15, or less where the largest d so far would take p' past 2^15, and j = 0, or what
+// takes that d to [1/2, 1) where it is less (at most 14; both move as the running maximum does).  Weights down to 2^-29 of the
+// largest keep f16's relative rounding, 2^-11 twice, for d of 1 and less.
 //
 // One token of 64 sequences over 2000 to 8191 keys of 4 heads of 256 in bf16: 211 us, 6.5 TB/s.  Over 4 bits neither memory
 // (43 % of its rate) nor issue (48 % of the slots, 1182 instructions for 32 keys of 256) is full: scores, maximum, weights and
@@ -347,6 +348,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
 
   float top[NT][2], sum[NT][2], out[MT][NT][4];
   float shift = Q4 ? kHeadroom - 15.0f : 0.0f; // references are kept without it; weights are 2^(score - maximum - shift)
+  int lift = 14;                               // 4 bits: value scales, and outputs with them, are 2^lift times themselves
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     top[nt][0] = top[nt][1] = -INFINITY;
@@ -477,6 +479,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
       __syncwarp();
     }
     const float shift_before = shift;
+    const int lift_before = lift;
     if constexpr (Q4) {
       // the largest value scale so far as a power of two above it: weights stay at 2^15 or below, and times a scale too
       uint32_t largest = 0;
@@ -487,9 +490,10 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
           largest = __vmaxu2(largest, scale_words(s, n * 32 + lane)[k] & 0x7fff7fffu);
       largest = __reduce_max_sync(0xffffffffu, max(largest & 0xffffu, largest >> 16));
       shift = fmaxf(shift, static_cast<float>(static_cast<int>(largest >> 10) - 29) + kHeadroom);
+      lift = min(lift, max(14 - static_cast<int>(largest >> 10), 0));
     }
     const bool masked = j0 + KT > sees_least; // some row does not see some key of the tile
-    bool outgrown = shift != shift_before;    // the reference moves only where a score has outgrown it by 2^8
+    bool outgrown = shift != shift_before || lift != lift_before; // else the reference moves only where a score has outgrown it by 2^8
     float best[NT][2], scaled[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -545,6 +549,11 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
           top[nt][col] = higher;
           sum[nt][col] *= moved[col];
         }
+        if constexpr (Q4) {
+          const float lowered = __int_as_float((127 + lift - lift_before) << 23);
+          moved[0] *= lowered;
+          moved[1] *= lowered;
+        }
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -587,6 +596,14 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
 #pragma unroll
         for (int n = 0; n < 4; ++n)
           load_words(sw[n], scale_words(s, m * 16 + 2 * t + (n & 1) + (n >> 1) * 8));
+        if (lift > 0) {
+          const uint32_t power = static_cast<uint32_t>(15 + lift) * 0x04000400u;
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int k = 0; k < NB / 2; ++k)
+              sw[n][k] = mul_f16(sw[n][k], power);
+        }
 #pragma unroll
         for (int k = 0; k < NB; k += 2) {
           uint32_t w[4]; // block k: keys 0-7, 8-15; block k + 1 the same
@@ -671,6 +688,8 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap map_values, const __grid_c
       for (int w = 0; w < kWarps; ++w)
         all = fmaxf(all, warp_max[w][nt * 8 + 2 * t + i]);
       joined[nt][i] = top[nt][i] == -INFINITY ? 0.0f : exp2_approx(top[nt][i] - all);
+      if (Q4)
+        joined[nt][i] *= __int_as_float((127 - lift) << 23);
     }
   // row-major [warp][row][D + 4], over the rings (all copies have landed); the pad keeps the writes off each other's banks
   constexpr int kPitch = D + 4;

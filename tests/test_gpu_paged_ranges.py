@@ -63,6 +63,30 @@ def test_attention_over_4_bit_blocks_of_mixed_sizes(heads, groups, dim, batch, l
     within(got, want, R.attention_bound(want, weight, extent, 4))
 
 
+# ---- light weights over small 4-bit values ---------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("size", [1e4, 1.0, 1e-1, 1e-2, 1e-3, 1e-4, 1e-5, 2e-6])
+@pytest.mark.parametrize("batch", [[(1, 40), (3, 9), (2, 2)], [(1, 700), (2, 6000)], [(40, 90), (70, 333)]], ids=str)
+@pytest.mark.parametrize("heads,groups,dim", SHAPES_4BIT)
+def test_light_weights_over_4_bit_values_of_any_size(heads, groups, dim, batch, size):
+    """Scores that one key dominates: where its value is 0, what is left comes from light weights.
+
+    Few rows: a weight p (the row's largest at least 2^7) and its product with the value's scale d, times 2^j, are rounded to
+    f16, which below 2^-14 is off by up to 2^-25.  Codes are at most 7 and the weights' sum at least 2^7, so a key moves the
+    result by up to 7 (2^-25 d + 2^-25 2^-j) / 2^7 = 7 2^-32 (d + 2^-j).  j brings the largest d to [1/2, 1) but is at most 14 and
+    not negative: 2^-j <= max(2^-14, min(1, 2 d)).  For d of 1 and more the weights are kept lower instead, by less than 2 d."""
+    g = torch.Generator().manual_seed(dim + 7)
+    q_start, kv_len, table, count = R.tables(batch, 64, 1, 5)
+    pages, scales, values = filled_cache(7, batch, table, count, groups, 64, dim, 4, scale=size)
+    q = (10 / size * torch.randn(int(q_start[-1]), heads, dim, generator=g)).to(BF)
+    got = paged.attention(paged.Cache(pages, scales), make_batch(q_start, kv_len, table, batch), q.cuda())
+    want, weight, extent = R.attention(q, values, q_start, kv_len, table, dim ** -0.5)
+    d, keys = float(scales.nan_to_num().max()), torch.cat([torch.arange(t - n, t) + 1 for n, t in batch])[:, None, None]
+    light = keys * 7 * 2.0 ** -32 * max(1.0, 2 * d) * (d + max(2.0 ** -14, min(1.0, 2 * d)))
+    within(got, want, R.attention_bound(want, weight, extent, 4) + light)
+
+
 # ---- rows without keys ---------------------------------------------------------------------------------------------------
 
 
