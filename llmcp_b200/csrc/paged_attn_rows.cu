@@ -27,9 +27,9 @@
 // largest keep f16's relative rounding, 2^-11 twice, for d of 1 and less.
 //
 // One token of 64 sequences over 2000 to 8191 keys of 4 heads of 256 in bf16: 211 us, 6.5 TB/s.  Over 4 bits neither memory
-// (43 % of its rate) nor issue (48 % of the slots, 1182 instructions for 32 keys of 256) is full: scores, maximum, weights and
+// (45 % of its rate) nor issue (50 % of the slots, 1190 instructions for 32 keys of 256) is full: scores, maximum, weights and
 // values of a warp's tile follow on one another, and three warps a scheduler do not hide their latencies.  One token over
-// 131000 keys 44 us, 3.4 TB/s; three tokens of 20 heads of 128, 96 sequences over 1250 to 5000 keys, 90 us, 2 TB/s.
+// 131000 keys 43 us, 3.5 TB/s; three tokens of 20 heads of 128, 96 sequences over 1250 to 5000 keys, 93 us, 1.9 TB/s.
 
 #include "common.cuh"
 #include "paged.h"
