@@ -115,10 +115,13 @@ __device__ __forceinline__ float2 capped_log2(uint64_t x, float cap, float over_
   return make_float2(fabsf(y.x) <= 0.5f ? near.x : far(y.x), fabsf(y.y) <= 0.5f ? near.y : far(y.y));
 }
 
-// x sigmoid(gate) = x / (1 + e^-gate).  Where the divisor is above 2^126 (gates below -87.3, -infinity among them) __fdividef
-// gives 0, and the product would be below f32's normal range; a NaN stays one.
+// x sigmoid(gate) = x h^2 / (1 + h^2), h = 2^(gate log2 e / 2): h^2 leaves f32 at gates below -87, where x times it may still be
+// an ordinary number, so x is multiplied twice.  At h = 2^12 and above the quotient is x to 2^-24.  A NaN stays one.
 __device__ __forceinline__ float times_sigmoid(float x, float gate) {
-  return __fdividef(x, 1.0f + exp2_approx(gate * -1.4426950408889634f));
+  float exponent;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(exponent) : "f"(gate * 0.7213475204444817f), "f"(12.0f));
+  const float h = exp2_approx(exponent);
+  return __fdividef(x * h * h, __fmaf_rn(h, h, 1.0f));
 }
 
 // Eight dimensions of a finished row: times their gate, where there is one, as bf16.

@@ -346,18 +346,9 @@ template <int DIMS> __device__ __forceinline__ void unload_row(uint8_t *to, int 
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float x = empty ? 0.0f : __uint_as_float(o[8 * k + 2 * i]) * scale, y = empty ? 0.0f : __uint_as_float(o[8 * k + 2 * i + 1]) * scale;
-        if (gated) { // as times_sigmoid
-          const float g0 = __uint_as_float(g[i] << 16) * -1.4426950408889634f, g1 = __uint_as_float(g[i] & 0xffff0000u) * -1.4426950408889634f;
-          float2 e;
-          if (k & 1) { // the hardware's 16 a cycle are also the quotients'
-            e = exp2_by_fma(pair(fminf(g0, 126.0f), fminf(g1, 126.0f)));
-            e.x = g0 <= 126.0f ? e.x : g0 * INFINITY; // infinite, or NaN
-            e.y = g1 <= 126.0f ? e.y : g1 * INFINITY;
-          } else {
-            e = make_float2(exp2_approx(g0), exp2_approx(g1));
-          }
-          x = __fdividef(x, 1.0f + e.x);
-          y = __fdividef(y, 1.0f + e.y);
+        if (gated) {
+          x = times_sigmoid(x, __uint_as_float(g[i] << 16));
+          y = times_sigmoid(y, __uint_as_float(g[i] & 0xffff0000u));
         }
         words[i] = pack16<false>(x, y);
       }

@@ -174,6 +174,29 @@ def test_gates_that_close(heads, groups, dim, bits, batch):
     assert near[~gate.isnan() & (gate != -math.inf)].all()
 
 
+# ---- gates beside large values -------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("batch", [[(1, 40), (1, 3)], [(1, 20011)], [(2, 3000)] * 20, [(150, 333), (40, 41)], [(20, 6000)]], ids=str)
+@pytest.mark.parametrize("heads,groups,dim", [(8, 2, 64), (8, 2, 128), (8, 2, 256)])
+def test_gates_that_nearly_close_large_values(heads, groups, dim, batch):
+    """A sigmoid below f32's range times a value of 1e20 is an ordinary number.  Its exponent, gate log2 e, is rounded to f32: at
+    130 off by 2^-17 and 130 2^-24 (the constant), times ln 2, and the two halves' powers by 2^-22 each: below 2^-16."""
+    g = torch.Generator().manual_seed(dim + 8)
+    q_start, kv_len, table, count = R.tables(batch, 64, 1, 5)
+    pages, scales, values = filled_cache(7, batch, table, count, groups, 64, dim, 16, scale=1e20)
+    tokens = int(q_start[-1])
+    q = (torch.randn(tokens, heads, dim, generator=g) * 1e-20).to(BF)
+    choices = torch.tensor([-60.0, -79.5, -86.5, -88.0, -95.0, -110.0, -130.0, -180.0, -math.inf, 3.0])
+    gate = choices[torch.randint(0, len(choices), (tokens, heads, dim), generator=g)].to(BF)
+    got = paged.attention(paged.Cache(pages), make_batch(q_start, kv_len, table, batch), q.cuda(), gate=gate.cuda()).cpu().double()
+    want, weight, extent = R.attention(q, values, q_start, kv_len, table, dim ** -0.5)
+    s = torch.sigmoid(gate.double())
+    bound = R.attention_bound(want, weight, extent, 16) * s + weight * s * 2.0 ** -16 + 2.0 ** -133  # the last: steps of a subnormal result
+    assert ((got - want * s).abs() <= bound).all()
+    assert (got[gate == -math.inf] == 0).all()
+
+
 # ---- queries -----------------------------------------------------------------------------------------------------------
 
 
