@@ -156,23 +156,28 @@ template <int D, int E>
 __device__ __noinline__ Row<E> rotated_in_f64(const uint16_t *src, const uint16_t *weight, float eps, const float *cos, const float *sin, float sign,
                                               int partner) {
   constexpr int kLanes = D / E;
-  double x[E], sum = 0.0;
+  double sum = 0.0;
 #pragma unroll
   for (int i = 0; i < E; ++i) {
-    x[i] = bf16_to_f32(src[i]);
-    sum += x[i] * x[i];
+    const double x = bf16_to_f32(src[i]);
+    sum += x * x;
   }
 #pragma unroll
   for (int o = kLanes / 2; o > 0; o >>= 1)
     sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  const double inv = 1.0 / sqrt(sum * (1.0 / D) + static_cast<double>(eps));
+  // x / root as the product with the reciprocal and its remainder's share: a quotient that puts y half way between two bf16
+  // values has to come out as it is.  (An infinite root has no remainder.)
+  const double root = sqrt(sum * (1.0 / D) + static_cast<double>(eps)), inv = 1.0 / root, back = root <= 1e300 ? root : 0.0;
   Row<E> r;
 #pragma unroll
   for (int i = 0; i < E; ++i) {
-    if (weight)
-      x[i] = x[i] * inv * (1.0 + static_cast<double>(bf16_to_f32(weight[i])));
-    const double other = __shfl_sync(0xffffffffu, x[i], partner);
-    const double y = sign != 0.0f ? x[i] * static_cast<double>(cos[i]) + static_cast<double>(sign) * other * static_cast<double>(sin[i]) : x[i];
+    double x = bf16_to_f32(src[i]);
+    if (weight) {
+      const double quotient = x * inv;
+      x = __fma_rn(__fma_rn(-quotient, back, x), inv, quotient) * (1.0 + static_cast<double>(bf16_to_f32(weight[i])));
+    }
+    const double other = __shfl_sync(0xffffffffu, x, partner);
+    const double y = sign != 0.0f ? x * static_cast<double>(cos[i]) + static_cast<double>(sign) * other * static_cast<double>(sin[i]) : x;
     const uint32_t bits = f64_to_bf16(y);
     r.w[i / 2] = i & 1 ? r.w[i / 2] | bits << 16 : bits;
   }

@@ -341,3 +341,27 @@ def test_append_rounds_products_below_f32s_range_once(heads, dim, rot, norm):
     k, _ = paged.read(cache, call, tokens)
     for y in (got, k):
         assert torch.equal(y.cpu().double(), want.double())
+
+
+# ---- ties -----------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dim,equal", [(64, 1), (64, 4), (128, 2), (128, 32), (256, 1), (256, 64)])
+def test_append_rounds_exact_middles_to_even(dim, equal):
+    """Rows of a few values of one size, whose norm is a power of two times it, with weights that put the result exactly half way
+    between two bf16 values."""
+    g = torch.Generator().manual_seed(dim + equal)
+    tokens, heads = 64, 5
+    order = torch.rand(tokens, heads, dim, generator=g).argsort(-1)
+    size = 2.0 ** torch.randint(-8, 9, (tokens, heads, 1), generator=g) * (1 + torch.randint(0, 128, (tokens, heads, 1), generator=g) / 128)
+    sign = torch.randint(0, 2, (tokens, heads, dim), generator=g) * 2 - 1
+    x = torch.where(order < equal, sign * size, 0.0).to(BF)
+    weight = ((2 * torch.randint(0, 128, (dim,), generator=g) + 1) / 256).to(BF)  # 1 + weight: nine bits, the last one set
+    pages, _ = empty_cache(1, heads, 64, dim, 16)
+    call = make_batch(torch.tensor([0, tokens], dtype=torch.int32), torch.tensor([tokens], dtype=torch.int32), torch.zeros(1, 1, dtype=torch.int32), [(tokens, tokens)])
+    cache = paged.Cache(pages)
+    got = paged.append(cache, call, *cuda(x, x, x), q_norm=weight.cuda(), k_norm=weight.cuda(), eps=0.0)
+    want = R.bf16_round(torch.where(x != 0, sign * (dim / equal) ** 0.5 * (1 + weight.double()), 0.0))
+    k, _ = paged.read(cache, call, tokens)
+    for y in (got, k):
+        assert torch.equal(y.cpu().double(), want)
