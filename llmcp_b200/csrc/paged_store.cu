@@ -156,18 +156,23 @@ template <int D, int E>
 __device__ __noinline__ Row<E> rotated_in_f64(const uint16_t *src, const uint16_t *weight, float eps, const float *cos, const float *sin, float sign,
                                               int partner) {
   constexpr int kLanes = D / E;
-  double sum = 0.0;
-#pragma unroll
-  for (int i = 0; i < E; ++i) {
-    const double x = bf16_to_f32(src[i]);
-    sum += x * x;
-  }
-#pragma unroll
-  for (int o = kLanes / 2; o > 0; o >>= 1)
-    sum += __shfl_xor_sync(0xffffffffu, sum, o);
   // x / root as the product with the reciprocal and its remainder's share: a quotient that puts y half way between two bf16
   // values has to come out as it is.  (An infinite root has no remainder.)
-  const double root = sqrt(sum * (1.0 / D) + static_cast<double>(eps)), inv = 1.0 / root, back = root <= 1e300 ? root : 0.0;
+  double inv = 0.0, back = 0.0;
+  if (weight) {
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const double x = bf16_to_f32(src[i]);
+      sum += x * x;
+    }
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1)
+      sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const double root = sqrt(sum * (1.0 / D) + static_cast<double>(eps));
+    inv = 1.0 / root;
+    back = root <= 1e300 ? root : 0.0;
+  }
   Row<E> r;
 #pragma unroll
   for (int i = 0; i < E; ++i) {
