@@ -12,7 +12,7 @@
 //              issue of its boxes among them: one warp for both bound every tile.)
 //
 // 1024 tokens over 7000 keys in 4 bits, twice, 32 heads of 128: 276 us in a captured graph, 910 TFLOP/s, 29 us of it the
-// expansion; 295 to 301 us as a call among others.  3 x up to 1501 tokens of 8 heads of 64, capped: 46 us a call, of
+// expansion; 295 to 302 us as a call among others.  3 x up to 1501 tokens of 8 heads of 64, capped: 46 us a call, of
 // which the longest rows' 25 tiles of 2000 cycles and a CTA's start and end account for some 31.  A row's scores over two threads (eight softmax
 // warps) measured 5 % (64) to 15 % (128) slower.
 

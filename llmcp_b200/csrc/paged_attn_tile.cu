@@ -23,8 +23,8 @@
 // Queries come in as whole rows through ring slots that are not in use yet, results leave as whole rows through the ring.
 //
 // A key tile is 1024 cycles of products beside a softmax of about 1300; the gates' sigmoids and the results take 7 thousand
-// cycles a CTA.  4 prompts of 1024 to 2048 tokens of 16 heads, gated: 120 us in a captured graph, 730 TFLOP/s (141 us with one
-// loading warp), 132 us as a call among others.
+// cycles a CTA.  4 prompts of 1024 to 2048 tokens of 16 heads, gated: 119 us in a captured graph, 740 TFLOP/s (141 us with one
+// loading warp), 132 to 134 us as a call among others.
 //
 // Every wait on a barrier is bounded; one that runs out raises a flag that all roles observe, the loader waits (bounded)
 // for its copies in flight, tensor memory is released and the status bit is set.

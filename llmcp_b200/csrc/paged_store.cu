@@ -14,8 +14,8 @@
 // share added tells the two apart.
 //
 // Append is bound by instructions (180 for 256 query values, 120 more for 256 values' codes), read by HBM.  In a captured
-// graph, 8192 tokens of 32 + 2 x 8 heads of 128: 63 us over bf16 pages, 65 us over 4 bits, of 26 and 28 us that their bytes
-// take.  30001 tokens of 4 heads of 256 read from bf16 pages: 40 us, 6.2 TB/s.  One token: 4.9 us.  A warp takes a whole token
+// graph, 8192 tokens of 32 + 2 x 8 heads of 128: 62 us over bf16 pages, 64 us over 4 bits, of 26 and 28 us that their bytes
+// take.  30001 tokens of 4 heads of 256 read from bf16 pages: 40 us, 6.2 TB/s.  One token: 5.5 us.  A warp takes a whole token
 // where there are enough of them (a block for each, with four warps that each found sequence, page and angles: 22 % longer,
 // and 12 % to read).
 // A lane takes eight neighbouring dimensions (rows of 64 to 256: 8 to 32 lanes).  Partners of a rotation lie in the same
