@@ -254,8 +254,9 @@ int llmcp_dev_gated_delta_net_noalloc(const uint16_t *conv, const uint16_t *a, c
  *                              multiple of kv_heads, at most 128 times as many.  Products on the tensor cores, sums and softmax in
  *                              f32.  What the pages hold from kv_len on has no influence, whatever it is; the keys and
  *                              values before it have to be finite, values below 2^100 (their sums are f32).  max_q, or tokens where they
- *                              are fewer (times heads / kv_heads: up to 16 rows or more), decides between two kernels; prompts over 4 bits want a workspace of all sequences' rows in 16
- *                              bits, sequences * 2 * kv_heads * max_kv of them, fewer than 2^31.  workspace: device memory of
+ *                              are fewer (times heads / kv_heads: up to 16 rows or more), decides between two kernels; prompts over 4 bits
+ *                              want a workspace of all sequences' rows in 16 bits, sequences * 2 * kv_heads * max_kv of them, fewer than
+ *                              2^31 (for max_q, however few tokens are).  workspace: device memory of
  *                              llmcp_dev_paged_attention_workspace bytes (-1 on error; depends on the host's figures only) that no other call uses
  *                              meanwhile, captured graphs that may run at the same time included; needs no clearing.
  * status (device int, may be null; not cleared): bit 1 is raised if a bounded wait inside a kernel ran out (out is then

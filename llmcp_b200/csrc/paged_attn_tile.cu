@@ -433,7 +433,7 @@ paged_largest_scale_kernel(PagedKv kv, PagedBatch batch, uint32_t *__restrict__ 
 // 16000 rows of 8 heads of 128: 21 us, of 13 that its bytes take, after 6 us for the largest scales.
 template <int DIM>
 __global__ void __launch_bounds__(256)
-paged_expand_kernel(PagedKv kv, PagedBatch batch, uint4 *__restrict__ out, int64_t rows, const uint32_t *__restrict__ largest, int parts,
+paged_expand_kernel(PagedKv kv, PagedBatch batch, uint4 *__restrict__ out, int64_t rows, const uint32_t *largest, int parts,
                     float *__restrict__ divisors, int *__restrict__ status) {
   constexpr int kLanes = DIM / 8, kAhead = 4; // eight dimensions (4 bytes of codes, 16 bytes out) per thread, of four keys at a time
   grid_dependency_sync();

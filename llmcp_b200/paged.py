@@ -211,9 +211,9 @@ def workspace_bytes(cache, batch, tokens, heads):
 @_on_device
 def attention(cache, batch, q, scale=None, softcap=0.0, slopes=None, prefix=None, gate=None, out=None, workspace=None, status=None):
     """softmax(score) v, times sigmoid(gate) where there is a gate: [tokens, heads, head_dim] bf16.  ``out`` may be q or gate
-    where that is contiguous, and overlaps nothing else.  ``q`` as ``append`` returns it; ``scale`` 1 / sqrt(head_dim) by default; ``slopes`` float32 [heads]; ``prefix`` int32 [sequences];
-    ``gate`` like q.  ``workspace``: a uint8 tensor of workspace_bytes() that no other call uses meanwhile; taken from
-    torch's allocator where it is not given."""
+    where that is contiguous, and overlaps nothing else.  ``q`` as ``append`` returns it; ``scale`` 1 / sqrt(head_dim) by
+    default; ``slopes`` float32 [heads]; ``prefix`` int32 [sequences]; ``gate`` like q.  ``workspace``: a uint8 tensor of
+    workspace_bytes() that no other call uses meanwhile; taken from torch's allocator where it is not given."""
     dev, bf = cache.device, torch.bfloat16
     (qp, qs), shape = _tensor(q, "q", bf, 3, dev), q.shape
     tokens, heads, dim = shape
